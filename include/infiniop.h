@@ -1,5 +1,5 @@
 /* Umbrella header for the operator library (the subset this library implements:
- * handle, tensor/operator descriptors, paged_attention, paged_attention_prefill, paged_caching, paged_decode_step, rope, kv_caching, kernel_status). */
+ * handle, tensor/operator descriptors, paged_attention, paged_attention_prefill, paged_caching, paged_decode_step, rope, kv_caching, quant_paged_caching, quant_paged_attention, kernel_status). */
 #ifndef __INFINIOP_API_H__
 #define __INFINIOP_API_H__
 
@@ -11,6 +11,8 @@
 #include "infiniop/ops/paged_attention_prefill.h"
 #include "infiniop/ops/paged_caching.h"
 #include "infiniop/ops/paged_decode_step.h"
+#include "infiniop/ops/quant_paged_attention.h"
+#include "infiniop/ops/quant_paged_caching.h"
 #include "infiniop/ops/rope.h"
 #include "infiniop/tensor_descriptor.h"
 

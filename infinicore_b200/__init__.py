@@ -17,6 +17,9 @@ _LAZY = {
     "paged_caching": "ops",
     "paged_attention_prefill": "ops",
     "paged_decode_step": "ops",
+    "quant_paged_caching": "ops",
+    "quant_paged_cache_read": "ops",
+    "quant_paged_attention": "ops",
     "rope": "ops",
     "kv_caching": "ops",
     "RopeAlgo": "ops",

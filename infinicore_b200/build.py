@@ -49,6 +49,8 @@ OP_SOURCES = [
     "paged_attention/decode_step.cu",
     "rope/rope.cu",
     "kv_caching/kv_caching.cu",
+    "quant_paged_cache/caching.cu",
+    "quant_paged_cache/attention.cu",
     "paged_attention_prefill/operator.cu",
     "paged_attention_prefill/prefill_generic.cu",
     "paged_attention_prefill/prefill_tiles.cu",

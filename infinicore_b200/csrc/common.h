@@ -96,6 +96,9 @@ enum class OpKind : int {
     PagedDecodeStep = 4,
     RoPE = 5,
     KVCaching = 6,
+    QuantPagedCaching = 7,
+    QuantPagedCacheRead = 8,
+    QuantPagedAttention = 9,
 };
 
 struct OpDescriptorBase {

@@ -1,0 +1,76 @@
+// Launch interface between the descriptor of the quantised paged attention and its kernels.
+#ifndef INFINIOP_B200_QUANT_ATTENTION_H
+#define INFINIOP_B200_QUANT_ATTENTION_H
+
+#include "quant_pool.h"
+
+namespace b200::quant_paged_cache {
+
+struct AttentionInfo {
+    Pools pools;
+    infiniDtype_t dtype; // of q and out
+    infiniDtype_t index_dtype;
+    size_t num_seqs, num_heads, head_size, max_blocks;
+    ptrdiff_t q_seq, q_head, o_seq, o_head, table_seq; // element strides
+    bool has_alibi;
+    float scale;
+    unsigned int *kernel_flags;
+    bool check_indices;
+    bool use_pdl;
+};
+
+struct AttentionArgs {
+    void *out;
+    const void *q;
+    const unsigned char *k_codes, *v_codes;
+    const unsigned short *k_scales, *v_scales;
+    const void *block_tables, *seq_lens;
+    const float *alibi;
+
+    int num_seqs, num_heads, num_kv_heads, group; // group: q heads of a kv head
+    int head_size, block_size, max_blocks;
+    int index_is_64, is_bf16;
+    long long q_seq, q_head, o_seq, o_head, table_seq;
+    long long k_block, k_head, k_slot, v_block, v_head, v_slot;             // bytes
+    long long ks_block, ks_head, ks_slot, vs_block, vs_head, vs_slot;       // elements
+    float scale_log2e; // scores are kept in the log2 domain
+
+    unsigned int *kernel_flags;
+    int check_indices;
+    long long num_blocks;
+};
+
+__device__ __forceinline__ long long indexAt(const AttentionArgs &a, const void *base, long long i) {
+    return a.index_is_64 ? static_cast<const long long *>(base)[i] : static_cast<long long>(static_cast<const int *>(base)[i]);
+}
+
+// Length of a sequence, never beyond what its row of the table can name.
+__device__ __forceinline__ int lengthOf(const AttentionArgs &a, int seq) {
+    const long long n = indexAt(a, a.seq_lens, seq);
+    const long long most = static_cast<long long>(a.max_blocks) * a.block_size;
+    const long long len = n < most ? n : most;
+    return len > 0x7fffffffLL ? 0x7fffffff : static_cast<int>(len);
+}
+
+// A block-table entry; in checked mode one outside the pool raises a flag and becomes block 0.
+__device__ __forceinline__ long long blockAt(const AttentionArgs &a, long long row, int i) {
+    const long long b = indexAt(a, a.block_tables, row + i);
+    if (a.check_indices && static_cast<unsigned long long>(b) >= static_cast<unsigned long long>(a.num_blocks)) {
+        atomicOr(a.kernel_flags, INFINIOP_KERNEL_FLAG_BLOCK_OUT_OF_RANGE);
+        return 0;
+    }
+    return b;
+}
+
+// The larger of two, NaN if one is: a NaN score has to reach the result.
+__device__ __forceinline__ float maxNan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+infiniStatus_t launchRows(const AttentionInfo &info, const AttentionArgs &a, cudaStream_t stream);
+
+} // namespace b200::quant_paged_cache
+
+#endif

@@ -94,6 +94,12 @@ INFINIOP_SYMBOLS = [
     "infiniopCreateRoPEDescriptor", "infiniopGetRoPEWorkspaceSize", "infiniopRoPE", "infiniopDestroyRoPEDescriptor",
     "infiniopCreateKVCachingDescriptor", "infiniopGetKVCachingWorkspaceSize", "infiniopKVCaching",
     "infiniopDestroyKVCachingDescriptor",
+    "infiniopCreateQuantPagedCachingDescriptor", "infiniopGetQuantPagedCachingWorkspaceSize", "infiniopQuantPagedCaching",
+    "infiniopDestroyQuantPagedCachingDescriptor",
+    "infiniopCreateQuantPagedCacheReadDescriptor", "infiniopGetQuantPagedCacheReadWorkspaceSize", "infiniopQuantPagedCacheRead",
+    "infiniopDestroyQuantPagedCacheReadDescriptor",
+    "infiniopCreateQuantPagedAttentionDescriptor", "infiniopGetQuantPagedAttentionWorkspaceSize", "infiniopQuantPagedAttention",
+    "infiniopDestroyQuantPagedAttentionDescriptor",
     "infiniopGetKernelStatus",
 ]
 INFINIRT_SYMBOLS = [
@@ -279,6 +285,20 @@ def _bind(lib: InfiniLib) -> None:
         ]
         op.infiniopDestroyKVCachingDescriptor.restype = c_int32
         op.infiniopDestroyKVCachingDescriptor.argtypes = [infiniopOperatorDescriptor_t]
+
+    # No reference counterpart: pools held in 8 or 4 bits - rows written, rows read back, decode attention.
+    for name, tensors, scalars in (("QuantPagedCaching", 7, []), ("QuantPagedCacheRead", 7, []), ("QuantPagedAttention", 9, [c_float])):
+        if not hasattr(op, f"infiniop{name}"):
+            continue
+        create = getattr(op, f"infiniopCreate{name}Descriptor")
+        create.restype = c_int32
+        create.argtypes = [infiniopHandle_t, POINTER(infiniopOperatorDescriptor_t)] + [infiniopTensorDescriptor_t] * tensors + scalars
+        getattr(op, f"infiniopGet{name}WorkspaceSize").restype = c_int32
+        getattr(op, f"infiniopGet{name}WorkspaceSize").argtypes = [infiniopOperatorDescriptor_t, POINTER(c_size_t)]
+        getattr(op, f"infiniop{name}").restype = c_int32
+        getattr(op, f"infiniop{name}").argtypes = [infiniopOperatorDescriptor_t, c_void_p, c_size_t] + [c_void_p] * tensors + [c_void_p]
+        getattr(op, f"infiniopDestroy{name}Descriptor").restype = c_int32
+        getattr(op, f"infiniopDestroy{name}Descriptor").argtypes = [infiniopOperatorDescriptor_t]
 
     # reference test/infiniop/libinfiniop/op_register.py:2231-2269
     op.infiniopCreatePagedCachingDescriptor.restype = c_int32

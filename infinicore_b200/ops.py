@@ -391,3 +391,101 @@ def paged_caching(k_cache, v_cache, k, v, slot_mapping):
             entry["desc"], None, 0, k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(), v.data_ptr(),
             slot_mapping.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
     return (k_cache, v_cache)
+
+
+# ---- pools held in 8 or 4 bits ----------------------------------------------------------------
+#
+# These calls are a decode step's smallest, so their way to the library is short: the cache key is made of the
+# tensors' own metadata objects, and the device is switched only where it is not the current one.
+
+def _one_device(*tensors):
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            return _require_cuda(*tensors)  # says what is wrong
+    return dev
+
+
+def _quant_entry(dev, op, tensors, extra=()):
+    """The cached descriptor of `op` for these tensors (None where an optional one is left out)."""
+    key = (op, extra, *[(t.dtype, t.shape, t.stride()) if t is not None else None for t in tensors])
+    per_dev = getattr(_tls, "per_dev", None)
+    st = per_dev.get(dev) if per_dev is not None else None
+    entry = st["cache"].get(key) if st is not None else None
+    if entry is not None:
+        st["cache"].move_to_end(key)
+        return st, entry
+    st = _state(dev)
+    return st, _lookup(st, key, lambda: _make_quant(st, op, tensors, extra))
+
+
+def _make_quant(st, op, tensors, extra):
+    descs = [_desc(t) if t is not None else None for t in tensors]
+    desc = infiniopOperatorDescriptor_t()
+    try:
+        check_error(getattr(LIBINFINIOP, f"infiniopCreate{op}Descriptor")(
+            st["handle"], ctypes.byref(desc), *[t.descriptor if t is not None else None for t in descs], *extra))
+    finally:
+        for t in descs:
+            if t is not None:
+                t.destroy_desc()
+    size = ctypes.c_size_t(0)
+    check_error(getattr(LIBINFINIOP, f"infiniopGet{op}WorkspaceSize")(desc, ctypes.byref(size)))
+    return {"desc": desc, "workspace": size.value, "run": getattr(LIBINFINIOP, f"infiniop{op}"),
+            "destroy": getattr(LIBINFINIOP, f"infiniopDestroy{op}Descriptor")}
+
+
+def _run_quant(dev, op, tensors, extra=()):
+    st, entry = _quant_entry(dev, op, tensors, extra)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _run_quant(dev, op, tensors, extra)
+    need, ws = entry["workspace"], None
+    if need:
+        # a captured call gets scratch of its own graph's memory: two graphs may be replayed at the same time
+        buf = (torch.empty(need, dtype=torch.uint8, device=f"cuda:{dev}") if torch.cuda.is_current_stream_capturing()
+               else _workspace(st, need, dev))
+        ws = buf.data_ptr()
+    check_error(entry["run"](entry["desc"], ws, need, *[t.data_ptr() if t is not None else None for t in tensors],
+                             torch.cuda.current_stream(dev).cuda_stream))
+
+
+def quant_paged_caching(k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping):
+    """Quantises k/v rows [num_tokens, num_kv_heads, head_size] (fp16 or bf16) into pools of codes at slot_mapping
+    (int64; negative = padding; the others must differ).  int8 pools [num_blocks, num_kv_heads, block_size,
+    head_size] hold 8-bit codes, uint8 pools [.., head_size / 2] two 4-bit codes a byte (the even element in the low
+    half, two's complement); scales are bfloat16 [num_blocks, num_kv_heads, block_size, groups] with groups = 1
+    (8 bits) or head_size / 32 (4 bits).  A group with largest magnitude A gets the scale A / 127 or A / 7 rounded to
+    bfloat16 and the codes x / scale, to the nearest, halves away from zero; one with an infinity or NaN reads back
+    as NaN.  Returns (k_cache, v_cache, k_scales, v_scales)."""
+    tensors = (k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping)
+    _run_quant(_one_device(*tensors), "QuantPagedCaching", tensors)
+    return (k_cache, v_cache, k_scales, v_scales)
+
+
+def quant_paged_cache_read(k_cache, v_cache, k_scales, v_scales, slot_mapping, dtype=torch.bfloat16, *, out=None):
+    """The values (code * scale, rounded to `dtype`: fp16, bf16 or fp32) at slot_mapping (int64, any order, repeats
+    allowed; zeros where negative) of pools that quant_paged_caching wrote, as dense rows k [num_tokens, num_kv_heads,
+    k head size] and v.  `out`: a pair of tensors to write instead of new ones (their dtype counts).  Returns (k, v)."""
+    if out is None:
+        packed = 2 if k_cache.dtype == torch.uint8 else 1
+        out = tuple(torch.empty((slot_mapping.shape[0], c.shape[1], c.shape[3] * packed), dtype=dtype, device=c.device)
+                    for c in (k_cache, v_cache))
+    k, v = out
+    tensors = (k, v, k_cache, v_cache, k_scales, v_scales, slot_mapping)
+    _run_quant(_one_device(*tensors), "QuantPagedCacheRead", tensors)
+    return (k, v)
+
+
+def quant_paged_attention(q, k_cache, v_cache, k_scales, v_scales, block_tables, cache_lens, alibi_slopes=None, scale: float = 1.0, *,
+                          out=None):
+    """paged_attention over pools that quant_paged_caching wrote: decode attention of one query token per sequence,
+    q [num_seqs, num_heads, head_size] with head sizes 64, 128, 192 and 256; block_tables [num_seqs, max_blocks] and
+    cache_lens [num_seqs] int64 or int32.  A sequence of length 0 leaves its rows of `out` as they are (zeros when
+    `out` is allocated here).  Captured into a CUDA graph, each call has scratch of its own.  Returns `out`."""
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    tensors = (out, q, k_cache, v_cache, k_scales, v_scales, block_tables, cache_lens, alibi_slopes)
+    dev = _one_device(*(tensors if alibi_slopes is not None else tensors[:-1]))
+    _run_quant(dev, "QuantPagedAttention", tensors, (float(scale),))
+    return out
