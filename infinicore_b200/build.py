@@ -51,6 +51,7 @@ OP_SOURCES = [
     "kv_caching/kv_caching.cu",
     "quant_paged_cache/caching.cu",
     "quant_paged_cache/attention.cu",
+    "quant_paged_cache/attention_tiles.cu",
     "paged_attention_prefill/operator.cu",
     "paged_attention_prefill/prefill_generic.cu",
     "paged_attention_prefill/prefill_tiles.cu",

@@ -1,4 +1,6 @@
-// infiniopQuantPagedAttention: the descriptor, and the kernel that is right for every layout.
+// infiniopQuantPagedAttention: the descriptor, and the kernel for layouts that the tiles kernel (attention_tiles.cu)
+// does not take: blocks that are no multiple of 8 tokens, strides or addresses that are no multiple of 16 bytes, K and V
+// pools laid out differently.
 //
 // quantAttentionRowsKernel: one CTA of four warps per (sequence, q head).  Warp w walks tokens w, w + 4, ...;
 // its lanes split the head in pairs, a shuffle reduction makes the score, and each warp keeps a running
@@ -17,7 +19,7 @@ namespace b200::quant_paged_cache {
 struct AttentionDescriptor {
     OpDescriptorBase base;
     AttentionInfo info;
-    size_t workspace_bytes;
+    TilesPlan tiles;
 };
 
 constexpr int kRowWarps = 4;
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) quantAttentionRowsKernel(const
     __syncthreads();
     const float slope = a.alibi != nullptr ? a.alibi[head] * 1.4426950408889634f : 0.f;
 
-    float m = -INFINITY, l = 0.f;
+    float m = kLowest, l = 0.f;
     float2 acc[kMaxPairs];
 #pragma unroll
     for (int i = 0; i < kMaxPairs; ++i) {
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) quantAttentionRowsKernel(const
             s += slope * static_cast<float>(t - (len - 1));
         }
         const float m_new = maxNan(m, s);
-        const float alpha = exp2f(m - m_new); // the first token: exp2(-inf) = 0
+        const float alpha = exp2f(m - m_new); // the first token: 0
         const float p = exp2f(s - m_new);
         l = l * alpha + p;
         m = m_new;
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) quantAttentionRowsKernel(const
         }
     }
     __syncthreads();
-    float m_all = -INFINITY;
+    float m_all = kLowest;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
         m_all = maxNan(m_all, merge[w * merge_stride]);
@@ -134,8 +136,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) quantAttentionRowsKernel(const
     float weight[kRowWarps], l_all = 0.f;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
-        const float mw = merge[w * merge_stride]; // -inf: a warp without a token
-        weight[w] = mw == -INFINITY ? 0.f : exp2f(mw - m_all);
+        weight[w] = exp2f(merge[w * merge_stride] - m_all); // a warp without a token has kLowest and 0
         l_all += weight[w] * merge[w * merge_stride + 1];
     }
     const float inv = 1.f / l_all;
@@ -269,8 +270,12 @@ __INFINI_C infiniStatus_t infiniopCreateQuantPagedAttentionDescriptor(
     info.kernel_flags = h->props->kernel_flags;
     info.check_indices = qc::envIs("INFINIOP_PAGED_CHECK_INDICES", '1');
     info.use_pdl = !qc::envIs("INFINIOP_PAGED_DECODE_PDL", '0');
-    auto *d = new (std::nothrow) AttentionDescriptor{{handle->device, handle->device_id, OpKind::QuantPagedAttention, h->props}, info, 0};
+    auto *d = new (std::nothrow) AttentionDescriptor{{handle->device, handle->device_id, OpKind::QuantPagedAttention, h->props}, info, {}};
     B200_RETURN_IF(d == nullptr, INFINI_STATUS_INTERNAL_ERROR);
+    // INFINIOP_QUANT_ATTENTION_PATH = auto (default) | rows
+    if (!qc::envIs("INFINIOP_QUANT_ATTENTION_PATH", 'r')) {
+        d->tiles = qc::planTiles(info, *h->props);
+    }
     *desc_ptr = reinterpret_cast<infiniopQuantPagedAttentionDescriptor_t>(d);
     return INFINI_STATUS_SUCCESS;
 }
@@ -280,7 +285,7 @@ __INFINI_C infiniStatus_t infiniopGetQuantPagedAttentionWorkspaceSize(
     B200_RETURN_IF(desc == nullptr || size == nullptr, INFINI_STATUS_NULL_POINTER);
     auto *d = reinterpret_cast<AttentionDescriptor *>(desc);
     B200_RETURN_IF(d->base.kind != OpKind::QuantPagedAttention, INFINI_STATUS_BAD_PARAM);
-    *size = d->workspace_bytes;
+    *size = d->tiles.workspace_bytes;
     return INFINI_STATUS_SUCCESS;
 }
 
@@ -309,8 +314,8 @@ __INFINI_C infiniStatus_t infiniopQuantPagedAttention(
                        || block_tables == nullptr || seq_lens == nullptr,
                    INFINI_STATUS_NULL_POINTER);
     B200_RETURN_IF(I.has_alibi && alibi_slopes == nullptr, INFINI_STATUS_NULL_POINTER);
-    B200_RETURN_IF(workspace_size < d->workspace_bytes, INFINI_STATUS_INSUFFICIENT_WORKSPACE);
-    B200_RETURN_IF(d->workspace_bytes > 0 && workspace == nullptr, INFINI_STATUS_NULL_POINTER);
+    B200_RETURN_IF(workspace_size < d->tiles.workspace_bytes, INFINI_STATUS_INSUFFICIENT_WORKSPACE);
+    B200_RETURN_IF(d->tiles.workspace_bytes > 0 && workspace == nullptr, INFINI_STATUS_NULL_POINTER);
     qc::AttentionArgs a = qc::makeArgs(I);
     a.out = out;
     a.q = q;
@@ -321,7 +326,8 @@ __INFINI_C infiniStatus_t infiniopQuantPagedAttention(
     a.block_tables = block_tables;
     a.seq_lens = seq_lens;
     a.alibi = I.has_alibi ? static_cast<const float *>(alibi_slopes) : nullptr;
-    return qc::launchRows(I, a, static_cast<cudaStream_t>(stream));
+    auto s = static_cast<cudaStream_t>(stream);
+    return qc::tilesTakePointers(d->tiles, a, workspace) ? qc::launchTiles(I, d->tiles, a, workspace, s) : qc::launchRows(I, a, s);
 }
 
 __INFINI_C infiniStatus_t infiniopDestroyQuantPagedAttentionDescriptor(

@@ -62,6 +62,9 @@ __device__ __forceinline__ long long blockAt(const AttentionArgs &a, long long r
     return b;
 }
 
+// Where a running maximum starts: finite, so that scores of -inf (an overflow) weigh 0 and not NaN.
+constexpr float kLowest = -3.402823466e38f;
+
 // The larger of two, NaN if one is: a NaN score has to reach the result.
 __device__ __forceinline__ float maxNan(float a, float b) {
     float r;
@@ -69,6 +72,22 @@ __device__ __forceinline__ float maxNan(float a, float b) {
     return r;
 }
 
+// The tiles kernel (attention_tiles.cu): whether a layout suits it, and what a launch needs.
+struct TilesPlan {
+    bool eligible = false;
+    int grid = 0;
+    int subs = 0;       // kv heads * head tiles of a group
+    int head_tiles = 0;
+    unsigned half_magic = 0;
+    int half_shift = 0;
+    size_t tasks_bytes = 0;
+    size_t workspace_bytes = 0;
+};
+TilesPlan planTiles(const AttentionInfo &info, const DeviceProps &props);
+bool tilesTakePointers(const TilesPlan &plan, const AttentionArgs &a, const void *workspace);
+infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, const AttentionArgs &a, void *workspace, cudaStream_t stream);
+
+// One CTA for each (sequence, q head), any layout (attention.cu).
 infiniStatus_t launchRows(const AttentionInfo &info, const AttentionArgs &a, cudaStream_t stream);
 
 } // namespace b200::quant_paged_cache

@@ -1,0 +1,920 @@
+// The fast kernel of infiniopQuantPagedAttention: tiles of 16 tokens, matrix instructions on the codes.
+//
+// Work.  A unit is (sequence, kv head, tile of 8 or 16 q heads of its group), ceil(length / 16) token tiles long.
+// All units lie end to end in one line that is cut into equal ranges, one for each CTA of a persistent grid, so
+// that ragged batches and few long sequences load the machine alike.  Within a CTA warp w takes every fourth tile;
+// the four meet in shared memory at the end of a unit.  A unit that is cut leaves partial results (maximum, sum,
+// unnormalised output) in the workspace; the combine kernel adds those in the order of the line, so that the
+// same call gives the same bits.
+//
+// Loads.  Every warp has a ring of tiles of its own in shared memory, filled by 16-byte asynchronous copies several
+// tiles ahead and across the ends of units.  Rows are swizzled in 16-byte chunks so that the matrix loads
+// (ldmatrix) touch every bank once.
+//
+// Arithmetic.  Codes become fp16 exactly by bit operations (1024 + u has u in its low mantissa bits) and one
+// addition; the scales never touch them:
+//   S[head, token] = sum_g k_scale[token, g] * (Q . codes)_g    a 32-element group is two matrix instructions
+//   w[token, g]    = p[token] * v_scale[token, g]               the weights carry the V scales
+//   O[dim, head]   = sum_token codes[token, dim] * w[token, g]
+// so the scores' layout in registers (heads by rows, tokens by columns) is the one that the weights need as second
+// operand, and V^T comes out of a transposing load.  In the 4-bit form every fourth pair of elements keeps a
+// factor of 16 that its output columns are rid of at the end.
+//   q is held in fp16 times a power of two that makes its largest element 1/2..1: exact for every element above
+// 2^-13 of that (fp16 and bf16 both have at most 11 bits).
+//   w is rounded once to fp16.  To keep it in range for scales of any size the running maximum is taken over
+// score + (exponent of the token's largest V scale), so that w <= 2^kSlack; p is relative to the same maximum.  The
+// maximum moves only when a score passes it by more than kSlack, and only then are outputs rescaled.
+//   Sums, maxima and outputs are fp32.
+#include "attention.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace b200::quant_paged_cache {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 16;
+constexpr float kSlack = 8.f;      // in the log2 domain; 2^8 is far inside fp16
+constexpr unsigned kLeastExp = 27; // V scales count as at least 2^-100 for the maximum: an all-zero row stays finite
+
+struct Task {
+    int seq, sub, pieces, pad;
+};
+
+template <int BITS, int HD, int HT>
+struct Cfg {
+    static constexpr int kRowBytes = HD * BITS / 8;
+    static constexpr int kChunks = kRowBytes / 16;            // 16-byte chunks of a row
+    static constexpr int kGroups = BITS == 4 ? HD / 32 : 1;   // scales of a row
+    static constexpr int kStage = 2 * kTile * kRowBytes + 2 * kTile * kGroups * 2;
+    static constexpr int kHeadTiles = HT / 8;
+    static constexpr int kMergeStride = HD + 4;               // floats: rows of two heads apart hit other banks
+    static constexpr int kMerge = kWarps * HT * kMergeStride * 4;
+    static constexpr int kFixed = kMerge + kWarps * HT * 8 + 128 * 4 + 256;
+    // resident CTAs: what the registers of q, outputs and scales leave room for
+    static constexpr int kCtas = HD * HT <= 1024 ? 4 : HD * HT <= 1536 ? 3 : 2;
+    static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
+    static constexpr int kStages = kFit > 6 ? 6 : kFit;
+    static_assert(kStages >= 2, "a ring of two tiles at least");
+    static constexpr int kSmem = kWarps * kStages * kStage + kFixed;
+    static constexpr int kRecord = HT * HD + 2 * HT; // floats of a partial result: outputs, maxima, sums
+};
+
+// ---- instructions ------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ unsigned smemAddr(const void *p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void copy16(unsigned dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void waitCopies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void loadMatrices(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void loadMatricesTransposed(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2Fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ unsigned packHalves(float lo, float hi) {
+    unsigned r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// (x & mask) ^ magic
+template <unsigned MASK, unsigned MAGIC>
+__device__ __forceinline__ unsigned pick(unsigned x) {
+    unsigned r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "n"(MASK), "n"(MAGIC));
+    return r;
+}
+__device__ __forceinline__ unsigned addHalves(unsigned x, unsigned y) {
+    unsigned r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+}
+__device__ __forceinline__ unsigned fmaHalves(unsigned x, unsigned y, unsigned z) {
+    unsigned r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(z));
+    return r;
+}
+
+constexpr unsigned kMinus1032 = 0xe408e408u; // fp16 pairs
+constexpr unsigned kMinus1152 = 0xe480e480u;
+constexpr unsigned kMinus72 = 0xd480d480u;
+constexpr unsigned kSixteenth = 0x2c002c00u;
+
+// 4-bit: a word of eight codes -> pairs (0,4), (1,5), (2,6), (3,7)
+__device__ __forceinline__ void codes4(unsigned w, unsigned (&b)[4]) {
+    const unsigned h = w >> 8;
+    b[0] = addHalves(pick<0x000f000fu, 0x64086408u>(w), kMinus1032);              // 1024 + (c + 8) - 1032
+    b[1] = fmaHalves(pick<0x00f000f0u, 0x64806480u>(w), kSixteenth, kMinus72);    // (1024 + 16 (c + 8)) / 16 - 72
+    b[2] = addHalves(pick<0x000f000fu, 0x64086408u>(h), kMinus1032);
+    b[3] = fmaHalves(pick<0x00f000f0u, 0x64806480u>(h), kSixteenth, kMinus72);
+}
+// The same with the odd ones 16 times too large
+__device__ __forceinline__ void codes4Odd16(unsigned w, unsigned (&b)[4]) {
+    const unsigned h = w >> 8;
+    b[0] = addHalves(pick<0x000f000fu, 0x64086408u>(w), kMinus1032);
+    b[1] = addHalves(pick<0x00f000f0u, 0x64806480u>(w), kMinus1152);
+    b[2] = addHalves(pick<0x000f000fu, 0x64086408u>(h), kMinus1032);
+    b[3] = addHalves(pick<0x00f000f0u, 0x64806480u>(h), kMinus1152);
+}
+// 8-bit: two of a word's codes, by byte selector
+template <unsigned SEL>
+__device__ __forceinline__ unsigned codes8(unsigned flipped) {
+    return addHalves(__byte_perm(flipped, 0x64646464u, SEL), kMinus1152);
+}
+
+// ---- the line of tiles -------------------------------------------------------------------------------------
+
+struct Lens { // lengths of the sequences a CTA meets first, in shared memory
+    const AttentionArgs &a;
+    const int *cached;
+    int base;
+    __device__ __forceinline__ int operator()(int seq) const {
+        const unsigned d = static_cast<unsigned>(seq - base);
+        return d < static_cast<unsigned>(kThreads) ? cached[d] : lengthOf(a, seq);
+    }
+};
+
+__device__ __forceinline__ int tilesOf(int len) { return len > 0 ? (len + kTile - 1) / kTile : 0; }
+
+struct Cursor {
+    int seq, sub, tile, tiles, len;
+};
+
+// `n` tiles on; the caller knows that the line goes on there.
+__device__ __forceinline__ void advance(Cursor &c, int n, int subs, const Lens &lens) {
+    c.tile += n;
+    while (c.tile >= c.tiles) {
+        c.tile -= c.tiles;
+        if (++c.sub == subs) {
+            c.sub = 0;
+            do {
+                ++c.seq;
+                c.len = lens(c.seq);
+                c.tiles = tilesOf(c.len);
+            } while (c.tiles == 0);
+        }
+    }
+}
+
+struct TilesArgs {
+    unsigned char *workspace; // Task[ctas] | records
+    long long tasks_bytes;
+    int subs;                 // kv heads * head tiles of a group
+    int head_tiles;
+    int min_range;            // tiles of a range at least
+    unsigned half_magic;      // division by block_size / 8
+    int half_shift;
+};
+
+// ---- kernel ------------------------------------------------------------------------------------------------
+
+template <int BITS, int HD, int HT>
+__global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAttentionTilesKernel(const AttentionArgs a, const TilesArgs p) {
+    using C = Cfg<BITS, HD, HT>;
+    constexpr int NG = C::kGroups, NH = C::kHeadTiles, CPR = C::kChunks, S = C::kStages;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float *merge = reinterpret_cast<float *>(smem + kWarps * S * C::kStage);
+    float2 *merge_ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(merge) + C::kMerge); // [warp][head]
+    int *lens_s = reinterpret_cast<int *>(merge_ml + kWarps * HT);
+    long long *plan_s = reinterpret_cast<long long *>(lens_s + kThreads); // sums of warps, then the start
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, t = lane & 3;
+
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // where this CTA's range starts and ends
+    const int per = (a.num_seqs + kThreads - 1) / kThreads;
+    long long mine = 0;
+    for (int i = 0; i < per; ++i) {
+        const int s = tid * per + i;
+        const int len = s < a.num_seqs ? lengthOf(a, s) : 0;
+        mine += tilesOf(len);
+        if (per == 1) {
+            lens_s[tid] = len;
+        }
+    }
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) {
+            upto += x;
+        }
+    }
+    if (lane == 31) {
+        plan_s[warp] = upto;
+    }
+    __syncthreads();
+    long long all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        all += plan_s[w];
+        upto += w < warp ? plan_s[w] : 0;
+    }
+    const long long total = all * p.subs;
+    long long range = (total + gridDim.x - 1) / gridDim.x;
+    range = range > p.min_range ? range : p.min_range;
+    const long long start = range * blockIdx.x;
+    Task *task = reinterpret_cast<Task *>(p.workspace) + blockIdx.x;
+    if (start >= total) {
+        if (tid == 0) {
+            task->pieces = 0;
+        }
+        return;
+    }
+    const int count = static_cast<int>((start + range < total ? start + range : total) - start);
+    if ((upto - mine) * p.subs <= start && start < upto * p.subs) { // one thread
+        long long pos = start - (upto - mine) * p.subs;
+        int s = tid * per, tiles = tilesOf(lengthOf(a, s));
+        while (pos >= static_cast<long long>(tiles) * p.subs) {
+            pos -= static_cast<long long>(tiles) * p.subs;
+            ++s;
+            tiles = tilesOf(lengthOf(a, s));
+        }
+        plan_s[4] = s;
+        plan_s[5] = pos;
+    }
+    __syncthreads();
+    Cursor cur;
+    cur.seq = static_cast<int>(plan_s[4]);
+    const Lens lens{a, lens_s, per == 1 ? 0 : cur.seq};
+    if (per != 1) {
+        lens_s[tid] = cur.seq + tid < a.num_seqs ? lengthOf(a, cur.seq + tid) : 0;
+        __syncthreads();
+    }
+    cur.len = lens(cur.seq);
+    cur.tiles = tilesOf(cur.len);
+    cur.sub = static_cast<int>(plan_s[5] / cur.tiles);
+    cur.tile = static_cast<int>(plan_s[5] - static_cast<long long>(cur.sub) * cur.tiles);
+
+    // ---- this warp's copies: its next tile, the blocks of that tile's two halves
+    unsigned char *ring = smem + warp * S * C::kStage;
+    Cursor next = cur;
+    int next_at = warp; // within the range
+    long long block0 = 0, block1 = 0;
+    int half0 = 0, half1 = 0; // first slots of the halves within their blocks
+    auto look = [&]() {
+        // a half of 8 tokens lies in one block; one behind the sequence's end is read where the first one is
+        const unsigned h0 = 2 * next.tile, halves = a.block_size / 8;
+        const unsigned b0 = static_cast<unsigned>((static_cast<unsigned long long>(h0) * p.half_magic) >> p.half_shift);
+        half0 = 8 * static_cast<int>(h0 - b0 * halves);
+        const long long row = next.seq * a.table_seq;
+        block0 = blockAt(a, row, b0);
+        if (8 * static_cast<int>(h0 + 1) < next.len) {
+            const unsigned b1 = half0 + 8 == a.block_size ? b0 + 1 : b0;
+            half1 = b1 == b0 ? half0 + 8 : 0;
+            block1 = b1 == b0 ? block0 : blockAt(a, row, b1);
+        } else {
+            half1 = half0;
+            block1 = block0;
+        }
+    };
+    auto fetch = [&](int slot) { // the next tile into a slot
+        if (next_at < count) {
+            const int kv = next.sub / p.head_tiles;
+            const unsigned dst = smemAddr(ring + slot * C::kStage);
+            const long long c0 = block0 * a.k_block + kv * a.k_head + half0 * a.k_slot;
+            const long long c1 = block1 * a.k_block + kv * a.k_head + half1 * a.k_slot;
+#pragma unroll
+            for (int j = 0; j < CPR / 2; ++j) {
+                const int i = lane + 32 * j, r = i / CPR, c = i % CPR;
+                const int swz = CPR % 8 == 0 ? (r & 7) : CPR % 4 == 0 ? ((r >> 1) & 3) : ((r >> 2) & 1);
+                const unsigned to = dst + r * C::kRowBytes + ((c ^ swz) << 4);
+                const long long from = (r < 8 ? c0 : c1) + (r & 7) * a.k_slot + c * 16;
+                copy16(to, a.k_codes + from);
+                copy16(to + kTile * C::kRowBytes, a.v_codes + from);
+            }
+            // scales: a half's 8 rows are one run of NG chunks
+            if (lane < 4 * NG) {
+                const bool v = lane >= 2 * NG;
+                const int i = v ? lane - 2 * NG : lane, h = i >= NG;
+                const long long from = (h ? block1 : block0) * a.ks_block + kv * a.ks_head + (h ? half1 : half0) * NG + (i - h * NG) * 8;
+                copy16(dst + 2 * kTile * C::kRowBytes + lane * 16, (v ? a.v_scales : a.k_scales) + from);
+            }
+            next_at += kWarps;
+            if (next_at < count) {
+                advance(next, kWarps, p.subs, lens);
+                look();
+            }
+        }
+        commitCopies();
+    };
+    if (warp < count) {
+        if (warp > 0) {
+            advance(next, warp, p.subs, lens);
+        }
+        look();
+    }
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) {
+        fetch(i);
+    }
+    int slot = 0;
+
+    // lane's part of the matrix loads: matrix lane / 8, row lane % 8; matrices are (tokens 0-7 | 8-15) x (chunk, chunk + 1)
+    const int m_row = (lane & 7) + ((lane >> 3) & 1) * 8, m_chunk = lane >> 4;
+    const int m_swz = CPR % 8 == 0 ? (m_row & 7) : CPR % 4 == 0 ? ((m_row >> 1) & 3) : ((m_row >> 2) & 1);
+
+    Task cut = {0, 0, 0, 0};
+    int at = warp; // this warp's next tile within the range
+    for (int seg = 0; seg < count;) {
+        const int seg_tiles = min(cur.tiles - cur.tile, count - seg), seg_end = seg + seg_tiles;
+        const int kv = cur.sub / p.head_tiles;
+        const int head0 = (cur.sub - kv * p.head_tiles) * HT;      // within the group
+        const int heads = min(HT, a.group - head0);
+        const long long head_at = static_cast<long long>(kv) * a.group + head0;
+
+        // q as first operand, scaled by a power of two for each head; the scores' factor takes it back
+        unsigned qr[NH][HD / 16][2]; // [.][k step][a0 | a2]
+        float factor[NH], slope[NH];
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+            const int h = g + 8 * n;
+            unsigned raw[HD / 16][2];
+            unsigned largest = 0;
+            const unsigned short *q = static_cast<const unsigned short *>(a.q) + cur.seq * a.q_seq + (head_at + h) * a.q_head;
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) { // 4 bits: 8 elements from 32 j + 8 t; 8 bits: 4 from 32 j + 4 t and 4 from + 16
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (h < heads) {
+                    if constexpr (BITS == 4) {
+                        x = *reinterpret_cast<const uint4 *>(q + 32 * j + 8 * t);
+                    } else {
+                        const uint2 lo = *reinterpret_cast<const uint2 *>(q + 32 * j + 4 * t);
+                        const uint2 hi = *reinterpret_cast<const uint2 *>(q + 32 * j + 16 + 4 * t);
+                        x = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    }
+                }
+                raw[2 * j][0] = x.x;
+                raw[2 * j][1] = x.y;
+                raw[2 * j + 1][0] = x.z;
+                raw[2 * j + 1][1] = x.w;
+                const unsigned m = 0x7fff7fffu;
+                const unsigned b = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
+                largest = max(largest, max(b & 0xffffu, b >> 16));
+            }
+            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            auto wide = [&](unsigned half) {
+                return a.is_bf16 ? __uint_as_float(half << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(half)));
+            };
+            const int e = static_cast<int>(__float_as_uint(wide(largest)) >> 23); // biased
+            const int down = max(253 - e, 1);                                     // 2^(126 - e)
+            const float scale_q = __uint_as_float(static_cast<unsigned>(down) << 23);
+            factor[n] = a.scale_log2e * __uint_as_float(static_cast<unsigned>(254 - down) << 23);
+            slope[n] = a.alibi != nullptr && h < heads ? a.alibi[head_at + h] * 1.4426950408889634f : 0.f;
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned w = raw[2 * j + (i >> 1)][i & 1];
+                    x[2 * i] = wide(w & 0xffffu) * scale_q;
+                    x[2 * i + 1] = wide(w >> 16) * scale_q;
+                }
+                if constexpr (BITS == 4) { // the order of codes4
+                    qr[n][2 * j][0] = packHalves(x[0], x[4]);
+                    qr[n][2 * j][1] = packHalves(x[1], x[5]);
+                    qr[n][2 * j + 1][0] = packHalves(x[2], x[6]);
+                    qr[n][2 * j + 1][1] = packHalves(x[3], x[7]);
+                } else {
+                    qr[n][2 * j][0] = packHalves(x[0], x[1]);
+                    qr[n][2 * j][1] = packHalves(x[2], x[3]);
+                    qr[n][2 * j + 1][0] = packHalves(x[4], x[5]);
+                    qr[n][2 * j + 1][1] = packHalves(x[6], x[7]);
+                }
+            }
+        }
+
+        float top[NH], sum[NH], o[NH][HD / 16][4];
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+            top[n] = kLowest;
+            sum[n] = 0.f;
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[n][j][i] = 0.f;
+                }
+            }
+        }
+
+        for (; at < seg_end; at += kWarps) {
+            waitCopies<S - 2>();
+            __syncwarp();
+            const unsigned char *stage = ring + slot * C::kStage;
+            fetch(slot == 0 ? S - 1 : slot - 1);
+            slot = slot == S - 1 ? 0 : slot + 1;
+            const int token0 = (cur.tile + at - seg) * kTile;
+            const unsigned k_addr = smemAddr(stage) + m_row * C::kRowBytes, v_addr = k_addr + kTile * C::kRowBytes;
+
+            // scales of the lane's tokens 2t, 2t + 1 (pair 0) and 2t + 8, 2t + 9 (pair 1): words [pair][token][group / 2]
+            constexpr int kWords = NG == 1 ? 1 : NG; // of a pair
+            unsigned ks[2][kWords], vs[2][kWords];
+            {
+                const unsigned char *s = stage + 2 * kTile * C::kRowBytes;
+#pragma unroll
+                for (int pair = 0; pair < 2; ++pair) {
+                    const unsigned *kp = reinterpret_cast<const unsigned *>(s) + (pair * 4 + t) * kWords;
+                    const unsigned *vp = kp + kTile * NG / 2;
+                    if constexpr (kWords % 4 == 0) {
+#pragma unroll
+                        for (int i = 0; i < kWords / 4; ++i) {
+                            const uint4 x = reinterpret_cast<const uint4 *>(kp)[i], y = reinterpret_cast<const uint4 *>(vp)[i];
+                            ks[pair][4 * i] = x.x, ks[pair][4 * i + 1] = x.y, ks[pair][4 * i + 2] = x.z, ks[pair][4 * i + 3] = x.w;
+                            vs[pair][4 * i] = y.x, vs[pair][4 * i + 1] = y.y, vs[pair][4 * i + 2] = y.z, vs[pair][4 * i + 3] = y.w;
+                        }
+                    } else if constexpr (kWords % 2 == 0) {
+#pragma unroll
+                        for (int i = 0; i < kWords / 2; ++i) {
+                            const uint2 x = reinterpret_cast<const uint2 *>(kp)[i], y = reinterpret_cast<const uint2 *>(vp)[i];
+                            ks[pair][2 * i] = x.x, ks[pair][2 * i + 1] = x.y;
+                            vs[pair][2 * i] = y.x, vs[pair][2 * i + 1] = y.y;
+                        }
+                    } else {
+                        ks[pair][0] = kp[0];
+                        vs[pair][0] = vp[0];
+                    }
+                }
+            }
+            // scale of token x (0, 1) of a pair and group j: NG == 1 keeps both tokens in one word
+            auto scaleAt = [](const unsigned (&w)[kWords], int x, int j) {
+                const unsigned word = NG == 1 ? w[0] : w[x * (NG / 2) + j / 2];
+                return __uint_as_float((NG == 1 ? x : j & 1) ? word & 0xffff0000u : word << 16);
+            };
+
+            // scores
+            float s[2][NH][2]; // [pair][head tile][token]
+            {
+                float acc[2][4];
+#pragma unroll
+                for (int pair = 0; pair < 2; ++pair) {
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        s[pair][n][0] = s[pair][n][1] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[pair][i] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < CPR; c += 2) {
+                    unsigned w[4];
+                    loadMatrices(w, k_addr + (((c + m_chunk) ^ m_swz) << 4));
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) { // the two chunks
+#pragma unroll
+                        for (int pair = 0; pair < 2; ++pair) {
+                            const unsigned word = w[2 * x + pair];
+                            if constexpr (BITS == 4) {
+                                const int j = c + x;
+                                unsigned b[4];
+                                codes4(word, b);
+                                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma(d, qr[0][2 * j][0], NH == 2 ? qr[NH - 1][2 * j][0] : 0u, qr[0][2 * j][1], NH == 2 ? qr[NH - 1][2 * j][1] : 0u,
+                                    b[0], b[1]);
+                                mma(d, qr[0][2 * j + 1][0], NH == 2 ? qr[NH - 1][2 * j + 1][0] : 0u, qr[0][2 * j + 1][1],
+                                    NH == 2 ? qr[NH - 1][2 * j + 1][1] : 0u, b[2], b[3]);
+                                const float s0 = scaleAt(ks[pair], 0, j), s1 = scaleAt(ks[pair], 1, j);
+#pragma unroll
+                                for (int n = 0; n < NH; ++n) {
+                                    s[pair][n][0] = fmaf(s0, d[2 * n], s[pair][n][0]);
+                                    s[pair][n][1] = fmaf(s1, d[2 * n + 1], s[pair][n][1]);
+                                }
+                            } else {
+                                const int j = c + x;
+                                const unsigned f = word ^ 0x80808080u;
+                                mma(acc[pair], qr[0][j][0], NH == 2 ? qr[NH - 1][j][0] : 0u, qr[0][j][1], NH == 2 ? qr[NH - 1][j][1] : 0u,
+                                    codes8<0x4140>(f), codes8<0x4342>(f));
+                            }
+                        }
+                    }
+                }
+                if constexpr (BITS == 8) {
+#pragma unroll
+                    for (int pair = 0; pair < 2; ++pair) {
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+                            s[pair][n][0] = acc[pair][2 * n] * scaleAt(ks[pair], 0, 0);
+                            s[pair][n][1] = acc[pair][2 * n + 1] * scaleAt(ks[pair], 1, 0);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int pair = 0; pair < 2; ++pair) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int token = token0 + 8 * pair + 2 * t + x;
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        s[pair][n][x] *= factor[n];
+                        if (a.alibi != nullptr) {
+                            s[pair][n][x] += slope[n] * static_cast<float>(token - (cur.len - 1));
+                        }
+                    }
+                    if (token0 + kTile > cur.len && token >= cur.len) { // behind the end: no weight, whatever the scales are
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+                            s[pair][n][x] = -INFINITY;
+                        }
+                        if constexpr (NG == 1) {
+                            vs[pair][0] &= x ? 0x0000ffffu : 0xffff0000u;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < NG / 2; ++i) {
+                                vs[pair][x * (NG / 2) + i] = 0u;
+                            }
+                        }
+                    }
+                }
+            }
+
+            // how far a token's weights can reach above its p: the exponent of its largest V scale, NaN ones left out
+            float reach[2][2];
+#pragma unroll
+            for (int pair = 0; pair < 2; ++pair) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    unsigned most;
+                    if constexpr (NG == 1) {
+                        most = x ? vs[pair][0] >> 16 : vs[pair][0] & 0xffffu;
+                        most = most < 0x7f80u ? most : 0u;
+                    } else {
+                        unsigned m = vs[pair][x * (NG / 2)];
+#pragma unroll
+                        for (int i = 1; i < NG / 2; ++i) {
+                            m = __vmaxu2(m, vs[pair][x * (NG / 2) + i]);
+                        }
+                        most = max(m & 0xffffu, m >> 16);
+                        if (most >= 0x7f80u) {
+                            most = 0;
+#pragma unroll
+                            for (int i = 0; i < NG / 2; ++i) {
+                                const unsigned w = vs[pair][x * (NG / 2) + i], lo = w & 0xffffu, hi = w >> 16;
+                                most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+                            }
+                        }
+                    }
+                    const unsigned e = max(most >> 7, kLeastExp);
+                    reach[pair][x] = __uint_as_float(0x4b000000u | e) - (8388608.f + 126.f); // >= log2 of the scale
+                }
+            }
+
+            // the maximum moves rarely
+            float high[NH];
+            bool move = false;
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+                high[n] = fmaxf(fmaxf(s[0][n][0] + reach[0][0], s[0][n][1] + reach[0][1]), fmaxf(s[1][n][0] + reach[1][0], s[1][n][1] + reach[1][1]));
+                move |= high[n] > top[n] + kSlack;
+            }
+            if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+                    high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 1));
+                    high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 2));
+                    const float now = fmaxf(top[n], high[n]);
+                    const float alpha = exp2Fast(top[n] - now); // the first time: 0
+                    top[n] = now;
+                    sum[n] *= alpha;
+                    const float alpha0 = __shfl_sync(0xffffffffu, alpha, 8 * t), alpha1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
+#pragma unroll
+                    for (int j = 0; j < HD / 16; ++j) {
+                        o[n][j][0] *= alpha0;
+                        o[n][j][1] *= alpha1;
+                        o[n][j][2] *= alpha0;
+                        o[n][j][3] *= alpha1;
+                    }
+                }
+            }
+#pragma unroll
+            for (int pair = 0; pair < 2; ++pair) {
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        s[pair][n][x] = exp2Fast(s[pair][n][x] - top[n]);
+                    }
+                    sum[n] += s[pair][n][0] + s[pair][n][1];
+                }
+            }
+
+            // outputs
+            unsigned weight[NH][2];
+#pragma unroll
+            for (int c = 0; c < CPR; c += 2) {
+                unsigned w[4];
+                loadMatricesTransposed(w, v_addr + (((c + m_chunk) ^ m_swz) << 4));
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int j = c + x;
+                    if (BITS == 4 || j == 0) { // the weights of this group
+#pragma unroll
+                        for (int pair = 0; pair < 2; ++pair) {
+                            const float v0 = scaleAt(vs[pair], 0, BITS == 4 ? j : 0), v1 = scaleAt(vs[pair], 1, BITS == 4 ? j : 0);
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                weight[n][pair] = packHalves(s[pair][n][0] * v0, s[pair][n][1] * v1);
+                            }
+                        }
+                    }
+                    if constexpr (BITS == 4) {
+                        unsigned lo[4], hi[4];
+                        codes4Odd16(w[2 * x], lo);
+                        codes4Odd16(w[2 * x + 1], hi);
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+                            mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], weight[n][0], weight[n][1]);
+                            mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], weight[n][0], weight[n][1]);
+                        }
+                    } else {
+                        const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
+                        const unsigned a0 = codes8<0x4240>(lo), a1 = codes8<0x4341>(lo), a2 = codes8<0x4240>(hi), a3 = codes8<0x4341>(hi);
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+                            mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
+                        }
+                    }
+                }
+            }
+        }
+
+        // the four warps' results of this unit meet
+        float *mine_o = merge + warp * HT * C::kMergeStride;
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+            sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
+            sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
+            if (t == 0) {
+                merge_ml[warp * HT + 8 * n + g] = make_float2(top[n], sum[n]);
+            }
+            float *row0 = mine_o + (8 * n + 2 * t) * C::kMergeStride, *row1 = row0 + C::kMergeStride;
+            if constexpr (BITS == 4) {
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) {
+                    const float(&x)[4] = o[n][2 * j], (&y)[4] = o[n][2 * j + 1];
+                    *reinterpret_cast<float4 *>(row0 + 32 * j + 4 * g) = make_float4(x[0], x[2] * 0.0625f, y[0], y[2] * 0.0625f);
+                    *reinterpret_cast<float4 *>(row1 + 32 * j + 4 * g) = make_float4(x[1], x[3] * 0.0625f, y[1], y[3] * 0.0625f);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    *reinterpret_cast<float2 *>(row0 + 16 * j + 2 * g) = make_float2(o[n][j][0], o[n][j][2]);
+                    *reinterpret_cast<float2 *>(row1 + 16 * j + 2 * g) = make_float2(o[n][j][1], o[n][j][3]);
+                }
+            }
+        }
+        __syncthreads();
+        const bool first = cur.tile == 0, last = cur.tile + seg_tiles == cur.tiles;
+        float *record = reinterpret_cast<float *>(p.workspace + p.tasks_bytes) + (2ll * blockIdx.x + (first ? 1 : 0)) * C::kRecord;
+        for (int i = tid; i < heads * (HD / 4); i += kThreads) {
+            const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
+            float m = kLowest;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                m = fmaxf(m, merge_ml[w * HT + h].x);
+            }
+            float l = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 ml = merge_ml[w * HT + h];
+                const float f = exp2Fast(ml.x - m); // a warp without a token has kLowest and 0
+                const float4 x = *reinterpret_cast<const float4 *>(merge + (w * HT + h) * C::kMergeStride + d);
+                l = fmaf(f, ml.y, l);
+                v.x = fmaf(f, x.x, v.x);
+                v.y = fmaf(f, x.y, v.y);
+                v.z = fmaf(f, x.z, v.z);
+                v.w = fmaf(f, x.w, v.w);
+            }
+            if (first && last) {
+                const float inv = 1.f / l;
+                unsigned short *dst = static_cast<unsigned short *>(a.out) + cur.seq * a.o_seq + (head_at + h) * a.o_head + d;
+                const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    dst[k] = a.is_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y[k])) : __half_as_ushort(__float2half_rn(y[k]));
+                }
+            } else {
+                *reinterpret_cast<float4 *>(record + h * HD + d) = v;
+                if (d == 0) {
+                    record[HT * HD + h] = m;
+                    record[HT * HD + HT + h] = l;
+                }
+            }
+        }
+        if (first && !last) { // this CTA's last unit: it names the pieces for the combine kernel
+            cut.seq = cur.seq;
+            cut.sub = cur.sub;
+            cut.pieces = static_cast<int>((start + seg + cur.tiles - 1) / range - blockIdx.x) + 1;
+        }
+        __syncthreads();
+        seg = seg_end;
+        if (seg < count) {
+            advance(cur, seg_tiles, p.subs, lens);
+        }
+    }
+    if (tid == 0) {
+        *task = cut;
+    }
+}
+
+// Adds the pieces of the unit that CTA x of the tiles kernel began and did not end.
+template <int HD, int HT>
+__global__ void __launch_bounds__(256) quantAttentionCombineKernel(const AttentionArgs a, const TilesArgs p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr int kRecord = HT * HD + 2 * HT;
+    const Task task = reinterpret_cast<const Task *>(p.workspace)[blockIdx.x];
+    if (task.pieces == 0) {
+        return;
+    }
+    const float *records = reinterpret_cast<const float *>(p.workspace + p.tasks_bytes);
+    // piece 0 is this CTA's second record, piece i the first one of CTA x + i
+    auto recordOf = [&](int i) { return records + (2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kRecord; };
+    const int kv = task.sub / p.head_tiles;
+    const int head0 = (task.sub - kv * p.head_tiles) * HT;
+    const int heads = min(HT, a.group - head0);
+    for (int i = threadIdx.x; i < heads * (HD / 4); i += blockDim.x) {
+        const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
+        float m = kLowest;
+        for (int k = 0; k < task.pieces; ++k) {
+            m = fmaxf(m, recordOf(k)[HT * HD + h]);
+        }
+        float l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < task.pieces; ++k) {
+            const float *r = recordOf(k);
+            const float mk = r[HT * HD + h], lk = r[HT * HD + HT + h];
+            const float f = exp2Fast(mk - m);
+            const float4 x = *reinterpret_cast<const float4 *>(r + h * HD + d);
+            l = fmaf(f, lk, l);
+            v.x = fmaf(f, x.x, v.x);
+            v.y = fmaf(f, x.y, v.y);
+            v.z = fmaf(f, x.z, v.z);
+            v.w = fmaf(f, x.w, v.w);
+        }
+        const float inv = 1.f / l;
+        unsigned short *dst =
+            static_cast<unsigned short *>(a.out) + task.seq * a.o_seq + (static_cast<long long>(kv) * a.group + head0 + h) * a.o_head + d;
+        const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            dst[k] = a.is_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y[k])) : __half_as_ushort(__float2half_rn(y[k]));
+        }
+    }
+}
+
+using TilesKernel = void (*)(AttentionArgs, TilesArgs);
+
+struct Variant {
+    TilesKernel tiles, combine;
+    int ctas, smem, record, heads;
+};
+
+template <int BITS, int HD, int HT>
+Variant variant() {
+    using C = Cfg<BITS, HD, HT>;
+    return {quantAttentionTilesKernel<BITS, HD, HT>, quantAttentionCombineKernel<HD, HT>, C::kCtas, C::kSmem, C::kRecord, HT};
+}
+
+template <int BITS>
+Variant variantFor(size_t head, size_t group) {
+    // 16 heads share a pass over the codes where a group has more than 8; at heads of 192 and 256 their outputs would not
+    // fit the registers
+    switch (head) {
+    case 64:
+        return group > 8 ? variant<BITS, 64, 16>() : variant<BITS, 64, 8>();
+    case 128:
+        return group > 8 ? variant<BITS, 128, 16>() : variant<BITS, 128, 8>();
+    case 192:
+        return variant<BITS, 192, 8>();
+    default:
+        return variant<BITS, 256, 8>();
+    }
+}
+
+Variant variantFor(const AttentionInfo &I) {
+    const size_t group = I.num_heads / I.pools.num_kv_heads;
+    return I.pools.bits == 4 ? variantFor<4>(I.head_size, group) : variantFor<8>(I.head_size, group);
+}
+
+constexpr int kMinRange = 8; // tiles
+
+} // namespace
+
+TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
+    TilesPlan plan;
+    const Pools &P = I.pools;
+    const Pool &k = P.k, &v = P.v;
+    const ptrdiff_t groups = static_cast<ptrdiff_t>(k.groups);
+    auto whole = [](ptrdiff_t stride, ptrdiff_t unit) { return stride % unit == 0; };
+    // copies of 16 bytes: 8 tokens of a block at a time, their scales one run; K and V laid out alike
+    plan.eligible = P.block_size % 8 == 0 && k.block == v.block && k.kv_head == v.kv_head && k.slot == v.slot && k.s_block == v.s_block
+                 && k.s_head == v.s_head && k.s_slot == v.s_slot && k.s_slot == groups && whole(k.block, 16) && whole(k.kv_head, 16)
+                 && whole(k.slot, 16) && whole(k.s_block, 8) && whole(k.s_head, 8) && whole(I.q_seq, 8) && whole(I.q_head, 8);
+    if (!plan.eligible || I.num_seqs == 0 || I.num_heads == 0 || I.max_blocks == 0) {
+        plan.eligible = false;
+        return plan;
+    }
+    const Variant var = variantFor(I);
+    const unsigned long long group = I.num_heads / P.num_kv_heads;
+    const unsigned long long head_tiles = (group + var.heads - 1) / var.heads;
+    const unsigned long long tiles = (static_cast<unsigned long long>(I.max_blocks) * P.block_size + kTile - 1) / kTile;
+    const unsigned long long subs = head_tiles * P.num_kv_heads;
+    const long double line = static_cast<long double>(tiles) * subs * I.num_seqs;
+    if (tiles > 0x0fffffffull || line > 9e17L) {
+        plan.eligible = false; // positions would not fit
+        return plan;
+    }
+    const unsigned long long most = (static_cast<unsigned long long>(line) + kMinRange - 1) / kMinRange;
+    const unsigned long long ctas = static_cast<unsigned long long>(props.sm_count) * var.ctas;
+    plan.grid = static_cast<int>(most < ctas ? most : ctas);
+    if (static_cast<unsigned long long>(line) / plan.grid > 0x3fffffffull) {
+        plan.eligible = false;
+        return plan;
+    }
+    plan.head_tiles = static_cast<int>(head_tiles);
+    plan.subs = static_cast<int>(subs);
+    plan.tasks_bytes = (sizeof(Task) * plan.grid + 255) / 256 * 256;
+    plan.workspace_bytes = plan.tasks_bytes + sizeof(float) * 2 * plan.grid * static_cast<size_t>(var.record);
+    const unsigned halves = static_cast<unsigned>(P.block_size / 8);
+    int l = 0;
+    while ((1u << l) < halves) {
+        ++l;
+    }
+    // n / halves for n < 2^31 as (n * magic) >> (31 + l)
+    plan.half_magic = static_cast<unsigned>((1ull << (31 + l)) / halves + 1);
+    plan.half_shift = 31 + l;
+    return plan;
+}
+
+bool tilesTakePointers(const TilesPlan &plan, const AttentionArgs &a, const void *workspace) {
+    return plan.eligible && alignedTo(a.k_codes, 16) && alignedTo(a.v_codes, 16) && alignedTo(a.k_scales, 16) && alignedTo(a.v_scales, 16)
+        && alignedTo(a.q, 16) && alignedTo(workspace, 16);
+}
+
+infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, const AttentionArgs &a, void *workspace, cudaStream_t stream) {
+    const Variant var = variantFor(info);
+    TilesArgs p;
+    p.workspace = static_cast<unsigned char *>(workspace);
+    p.tasks_bytes = static_cast<long long>(plan.tasks_bytes);
+    p.subs = plan.subs;
+    p.head_tiles = plan.head_tiles;
+    p.min_range = kMinRange;
+    p.half_magic = plan.half_magic;
+    p.half_shift = plan.half_shift;
+    // an attribute of the current device's function, so it is set for each launch
+    if (cudaFuncSetAttribute(var.tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem) != cudaSuccess) {
+        return checkLaunch("quantAttentionTilesKernel: shared memory");
+    }
+    cudaLaunchAttribute pdl;
+    pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl.val.programmaticStreamSerializationAllowed = info.use_pdl ? 1 : 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(plan.grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(var.smem);
+    cfg.stream = stream;
+    cfg.attrs = &pdl;
+    cfg.numAttrs = 1;
+    (void)cudaLaunchKernelEx(&cfg, var.tiles, a, p);
+    const infiniStatus_t st = checkLaunch("quantAttentionTilesKernel");
+    B200_RETURN_IF(st != INFINI_STATUS_SUCCESS, st);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    (void)cudaLaunchKernelEx(&cfg, var.combine, a, p);
+    return checkLaunch("quantAttentionCombineKernel");
+}
+
+} // namespace b200::quant_paged_cache

@@ -212,6 +212,24 @@ def test_reading_is_the_rounded_product(ib, shape, bits, dtype):
 
 # ---- attention --------------------------------------------------------------------------------------------
 
+@contextlib.contextmanager
+def rows_path():
+    """Descriptors made here use the kernel for any layout; none of them is kept."""
+    from infinicore_b200 import ops
+
+    with environment(INFINIOP_QUANT_ATTENTION_PATH="rows"):
+        forget(ops)
+        yield
+    forget(ops)
+
+
+def forget(ops):
+    cache = ops._tls.per_dev[0]["cache"]
+    for key in [k for k in cache if k[0] == "QuantPagedAttention"]:
+        entry = cache.pop(key)
+        entry["destroy"](entry["desc"])
+
+
 def check_attention(ib, gen, lens, heads, kvh, hd, bs, bits, dtype, scale=None, alibi=False, ix=torch.int64, std=1.0, qstd=1.0, what=""):
     lens_t = torch.tensor(lens)
     blocks = max(1, sum(-(-max(0, n) // bs) for n in lens)) + 2
@@ -224,9 +242,12 @@ def check_attention(ib, gen, lens, heads, kvh, hd, bs, bits, dtype, scale=None, 
     got = ib.quant_paged_attention(q, *pools, tables, lens_t.to(ix).cuda(), slopes, scale, out=out)
     want, bound = qh.attend_bound(q, pools, tables, lens_t, scale, bits, dtype, slopes, torch.full_like(out, 3.0))
     qh.close(got, want, bound, what)
+    with rows_path():
+        other = ib.quant_paged_attention(q, *pools, tables, lens_t.to(ix).cuda(), slopes, scale, out=torch.full_like(out, 3.0))
+    qh.close(other, want, bound, what + " (rows)")
     for i, n in enumerate(lens):
         if n <= 0:
-            assert bool((got[i] == 3).all())
+            assert bool((got[i] == 3).all()) and bool((other[i] == 3).all())
     return q, pools, tables, lens_t, got
 
 
@@ -603,6 +624,7 @@ def test_checked_indices_raise_flags_and_touch_nothing_foreign(ib):
         assert ib.kernel_status() == 0
         # descriptors made here must not serve later tests
         from infinicore_b200 import ops
+
         cache = ops._tls.per_dev[0]["cache"]
         for key in [k for k in cache if str(k[0]).startswith("QuantPaged")]:
             entry = cache.pop(key)

@@ -53,7 +53,8 @@ target("infiniop")
               csrc .. "/paged_attention/decode_stream.cu", csrc .. "/paged_attention/static_workspace.cu",
               csrc .. "/paged_attention/decode_step.cu")
     add_files(csrc .. "/rope/rope.cu", csrc .. "/kv_caching/kv_caching.cu")
-    add_files(csrc .. "/quant_paged_cache/caching.cu", csrc .. "/quant_paged_cache/attention.cu")
+    add_files(csrc .. "/quant_paged_cache/caching.cu", csrc .. "/quant_paged_cache/attention.cu",
+              csrc .. "/quant_paged_cache/attention_tiles.cu")
     add_files(csrc .. "/paged_attention_prefill/operator.cu", csrc .. "/paged_attention_prefill/prefill_generic.cu",
               csrc .. "/paged_attention_prefill/prefill_tiles.cu", csrc .. "/paged_attention_prefill/prefill_umma.cu")
     add_rpathdirs("$ORIGIN")
