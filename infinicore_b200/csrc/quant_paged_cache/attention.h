@@ -78,8 +78,9 @@ struct TilesPlan {
     int grid = 0;
     int subs = 0;       // kv heads * head tiles of a group
     int head_tiles = 0;
-    unsigned half_magic = 0;
+    unsigned half_magic = 0, half_self = 0; // division by block_size / 8
     int half_shift = 0;
+    bool out_words = false;
     size_t tasks_bytes = 0;
     size_t workspace_bytes = 0;
 };

@@ -1,11 +1,12 @@
 // The fast kernel of infiniopQuantPagedAttention: tiles of 16 tokens, matrix instructions on the codes.
 //
 // Work.  A unit is (sequence, kv head, tile of 8 or 16 q heads of its group), ceil(length / 16) token tiles long.
-// All units lie end to end in one line that is cut into equal ranges, one for each CTA of a persistent grid, so
-// that ragged batches and few long sequences load the machine alike.  Within a CTA warp w takes every fourth tile;
-// the four meet in shared memory at the end of a unit.  A unit that is cut leaves partial results (maximum, sum,
-// unnormalised output) in the workspace; the combine kernel adds those in the order of the line, so that the
-// same call gives the same bits.
+// All units lie end to end in one line, each with kUnitCost tiles in front for what a unit costs by itself (q, results),
+// and the line is cut into equal ranges, one for each warp of a persistent grid, so that ragged batches, many short and
+// few long sequences load the machine alike.  A warp that has a unit to itself stores its rows; pieces of a unit in one
+// CTA meet in shared memory at the CTA's end; a unit that is cut between CTAs leaves partial results (maximum, sum,
+// unnormalised output) in the workspace, and the combine kernel adds those in the order of the line.  Every sum has
+// one order, so the same call gives the same bits.
 //
 // Loads.  Every warp has a ring of tiles of its own in shared memory, filled by 16-byte asynchronous copies several
 // tiles ahead and across the ends of units.  Rows are swizzled in 16-byte chunks so that the matrix loads
@@ -37,11 +38,19 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;
+constexpr int kUnitCost = 1;       // tiles' worth of time that a unit costs beside its tiles
+constexpr int kMinRange = 3;       // of a warp: at least two tiles of a unit's first range
 constexpr float kSlack = 8.f;      // in the log2 domain; 2^8 is far inside fp16
-constexpr unsigned kLeastExp = 27; // V scales count as at least 2^-100 for the maximum: an all-zero row stays finite
+constexpr unsigned kLeastScale = 27u << 7; // V scales count as at least 2^-100 for the maximum: an all-zero row stays finite
 
 struct Task {
     int seq, sub, pieces, pad;
+};
+
+// A part of a unit that one warp has done: first tile's position on the line, tiles of the whole unit.
+struct Piece {
+    long long first;
+    int seq, sub, tiles, used;
 };
 
 template <int BITS, int HD, int HT>
@@ -51,15 +60,17 @@ struct Cfg {
     static constexpr int kGroups = BITS == 4 ? HD / 32 : 1;   // scales of a row
     static constexpr int kStage = 2 * kTile * kRowBytes + 2 * kTile * kGroups * 2;
     static constexpr int kHeadTiles = HT / 8;
-    static constexpr int kMergeStride = HD + 4;               // floats: rows of two heads apart hit other banks
-    static constexpr int kMerge = kWarps * HT * kMergeStride * 4;
-    static constexpr int kFixed = kMerge + kWarps * HT * 8 + 128 * 4 + 256;
+    static constexpr int kStride = HD + 4;                    // floats: rows of two heads apart hit other banks
+    static constexpr int kResult = HT * kStride * 4;
+    static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece))) + kThreads * 4 + 256;
     // resident CTAs: what the registers of q, outputs and scales leave room for
     static constexpr int kCtas = HD * HT <= 1024 ? 4 : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
     static constexpr int kStages = kFit > 6 ? 6 : kFit;
     static_assert(kStages >= 2, "a ring of two tiles at least");
-    static constexpr int kSmem = kWarps * kStages * kStage + kFixed;
+    static constexpr int kRing = kStages * kStage;
+    static_assert(kRing >= kResult, "a finished ring holds a result");
+    static constexpr int kSmem = kWarps * kRing + kFixed;
     static constexpr int kRecord = HT * HD + 2 * HT; // floats of a partial result: outputs, maxima, sums
 };
 
@@ -149,6 +160,19 @@ __device__ __forceinline__ unsigned codes8(unsigned flipped) {
 
 // ---- the line of tiles -------------------------------------------------------------------------------------
 
+struct TilesArgs {
+    unsigned char *workspace; // Task[ctas] | records
+    long long tasks_bytes;
+    int subs;                 // kv heads * head tiles of a group
+    int head_tiles;
+    unsigned half_magic;      // division by block_size / 8
+    unsigned half_self;       // all ones where that is a division by 1
+    int half_shift;
+    int index_shift;          // log2 of the bytes of a table entry
+    int pages_of_16;          // block_size is a multiple of 16
+    int out_words;            // rows of out can be stored 8 bytes at a time
+};
+
 struct Lens { // lengths of the sequences a CTA meets first, in shared memory
     const AttentionArgs &a;
     const int *cached;
@@ -160,64 +184,89 @@ struct Lens { // lengths of the sequences a CTA meets first, in shared memory
 };
 
 __device__ __forceinline__ int tilesOf(int len) { return len > 0 ? (len + kTile - 1) / kTile : 0; }
+__device__ __forceinline__ long long costOf(int len) { return len > 0 ? tilesOf(len) + kUnitCost : 0; }
 
+// A walk over the tiles of a warp's range.  `budget`: what is left of the range, the present tile included.
 struct Cursor {
-    int seq, sub, tile, tiles, len;
-};
+    int seq, sub, tile, tiles, len, budget;
 
-// `n` tiles on; the caller knows that the line goes on there.
-__device__ __forceinline__ void advance(Cursor &c, int n, int subs, const Lens &lens) {
-    c.tile += n;
-    while (c.tile >= c.tiles) {
-        c.tile -= c.tiles;
-        if (++c.sub == subs) {
-            c.sub = 0;
-            do {
-                ++c.seq;
-                c.len = lens(c.seq);
-                c.tiles = tilesOf(c.len);
-            } while (c.tiles == 0);
+    // To the next tile; true where that is in another unit.
+    __device__ __forceinline__ bool step(int subs, const Lens &lens) {
+        --budget;
+        if (++tile < tiles || budget <= 0) {
+            return false;
         }
+        tile = 0;
+        budget -= kUnitCost; // behind 0: the range ends in front of the next unit's first tile
+        if (budget > 0 && ++sub == subs) {
+            sub = 0;
+            do {
+                len = lens(++seq);
+            } while (len <= 0);
+            tiles = tilesOf(len);
+        }
+        return true;
     }
-}
-
-struct TilesArgs {
-    unsigned char *workspace; // Task[ctas] | records
-    long long tasks_bytes;
-    int subs;                 // kv heads * head tiles of a group
-    int head_tiles;
-    int min_range;            // tiles of a range at least
-    unsigned half_magic;      // division by block_size / 8
-    int half_shift;
 };
 
 // ---- kernel ------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ unsigned short roundOut(float v, int is_bf16) {
+    return is_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+
+// N neighbouring elements of a row of out.
+template <int N>
+__device__ __forceinline__ void storeOut(const AttentionArgs &a, const TilesArgs &p, long long at, const float (&v)[N]) {
+    unsigned short *dst = static_cast<unsigned short *>(a.out) + at;
+    unsigned short r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        r[i] = roundOut(v[i], a.is_bf16);
+    }
+    if (p.out_words) {
+        if constexpr (N == 4) {
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(r[0] | (static_cast<unsigned>(r[1]) << 16), r[2] | (static_cast<unsigned>(r[3]) << 16));
+        } else {
+            *reinterpret_cast<unsigned *>(dst) = r[0] | (static_cast<unsigned>(r[1]) << 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            dst[i] = r[i];
+        }
+    }
+}
 
 template <int BITS, int HD, int HT>
 __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAttentionTilesKernel(const AttentionArgs a, const TilesArgs p) {
     using C = Cfg<BITS, HD, HT>;
     constexpr int NG = C::kGroups, NH = C::kHeadTiles, CPR = C::kChunks, S = C::kStages;
     extern __shared__ __align__(128) unsigned char smem[];
-    float *merge = reinterpret_cast<float *>(smem + kWarps * S * C::kStage);
-    float2 *merge_ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(merge) + C::kMerge); // [warp][head]
-    int *lens_s = reinterpret_cast<int *>(merge_ml + kWarps * HT);
-    long long *plan_s = reinterpret_cast<long long *>(lens_s + kThreads); // sums of warps, then the start
+    float *results = reinterpret_cast<float *>(smem + kWarps * C::kRing);                                     // [warp][head][kStride]
+    float2 *sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(results) + kWarps * C::kResult); // [warp][2][head]
+    Piece *pieces = reinterpret_cast<Piece *>(sums + kWarps * 2 * HT);                                        // [warp][2]
+    int *lens_s = reinterpret_cast<int *>(pieces + kWarps * 2);
+    long long *plan_s = reinterpret_cast<long long *>(lens_s + kThreads); // sums of warps; then seq and position of each start
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // where this CTA's range starts and ends
+    // the ranges of this CTA's warps
     const int per = (a.num_seqs + kThreads - 1) / kThreads;
     long long mine = 0;
     for (int i = 0; i < per; ++i) {
         const int s = tid * per + i;
         const int len = s < a.num_seqs ? lengthOf(a, s) : 0;
-        mine += tilesOf(len);
+        mine += costOf(len);
         if (per == 1) {
             lens_s[tid] = len;
         }
+    }
+    if (tid < kWarps * 2) {
+        pieces[tid].used = 0;
     }
     long long upto = mine;
 #pragma unroll
@@ -238,510 +287,632 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         upto += w < warp ? plan_s[w] : 0;
     }
     const long long total = all * p.subs;
-    long long range = (total + gridDim.x - 1) / gridDim.x;
-    range = range > p.min_range ? range : p.min_range;
-    const long long start = range * blockIdx.x;
+    const int workers = static_cast<int>(gridDim.x) * kWarps;
+    long long range = (total + workers - 1) / workers;
+    range = range > kMinRange ? range : kMinRange;
+    const long long cta_range = range * kWarps, cta_start = cta_range * blockIdx.x;
     Task *task = reinterpret_cast<Task *>(p.workspace) + blockIdx.x;
-    if (start >= total) {
+    if (cta_start >= total) {
         if (tid == 0) {
             task->pieces = 0;
         }
         return;
     }
-    const int count = static_cast<int>((start + range < total ? start + range : total) - start);
-    if ((upto - mine) * p.subs <= start && start < upto * p.subs) { // one thread
-        long long pos = start - (upto - mine) * p.subs;
-        int s = tid * per, tiles = tilesOf(lengthOf(a, s));
-        while (pos >= static_cast<long long>(tiles) * p.subs) {
-            pos -= static_cast<long long>(tiles) * p.subs;
-            ++s;
-            tiles = tilesOf(lengthOf(a, s));
+    if (mine > 0) {
+#pragma unroll 1
+        for (int w = 0; w < kWarps; ++w) {
+            long long pos = cta_start + w * range - (upto - mine) * p.subs;
+            if (pos >= 0 && pos < mine * p.subs) { // one thread for each start
+                int s = tid * per;
+                long long cost = costOf(lengthOf(a, s)) * p.subs;
+                while (pos >= cost) {
+                    pos -= cost;
+                    cost = costOf(lengthOf(a, ++s)) * p.subs;
+                }
+                plan_s[4 + 2 * w] = s;
+                plan_s[5 + 2 * w] = pos;
+            }
         }
-        plan_s[4] = s;
-        plan_s[5] = pos;
     }
     __syncthreads();
-    Cursor cur;
-    cur.seq = static_cast<int>(plan_s[4]);
-    const Lens lens{a, lens_s, per == 1 ? 0 : cur.seq};
+    const Lens lens{a, lens_s, per == 1 ? 0 : static_cast<int>(plan_s[4])};
     if (per != 1) {
-        lens_s[tid] = cur.seq + tid < a.num_seqs ? lengthOf(a, cur.seq + tid) : 0;
+        lens_s[tid] = lens.base + tid < a.num_seqs ? lengthOf(a, lens.base + tid) : 0;
         __syncthreads();
     }
-    cur.len = lens(cur.seq);
-    cur.tiles = tilesOf(cur.len);
-    cur.sub = static_cast<int>(plan_s[5] / cur.tiles);
-    cur.tile = static_cast<int>(plan_s[5] - static_cast<long long>(cur.sub) * cur.tiles);
+    const long long start = cta_start + warp * range, end = start + range < total ? start + range : total;
 
-    // ---- this warp's copies: its next tile, the blocks of that tile's two halves
-    unsigned char *ring = smem + warp * S * C::kStage;
-    Cursor next = cur;
-    int next_at = warp; // within the range
-    long long block0 = 0, block1 = 0;
-    int half0 = 0, half1 = 0; // first slots of the halves within their blocks
-    auto look = [&]() {
-        // a half of 8 tokens lies in one block; one behind the sequence's end is read where the first one is
-        const unsigned h0 = 2 * next.tile, halves = a.block_size / 8;
-        const unsigned b0 = static_cast<unsigned>((static_cast<unsigned long long>(h0) * p.half_magic) >> p.half_shift);
-        half0 = 8 * static_cast<int>(h0 - b0 * halves);
-        const long long row = next.seq * a.table_seq;
-        block0 = blockAt(a, row, b0);
-        if (8 * static_cast<int>(h0 + 1) < next.len) {
-            const unsigned b1 = half0 + 8 == a.block_size ? b0 + 1 : b0;
-            half1 = b1 == b0 ? half0 + 8 : 0;
-            block1 = b1 == b0 ? block0 : blockAt(a, row, b1);
-        } else {
-            half1 = half0;
-            block1 = block0;
+    unsigned char *ring = smem + warp * C::kRing;
+    if (start < total) {
+        Cursor cur;
+        long long place; // of the present tile on the line
+        {
+            cur.seq = static_cast<int>(plan_s[4 + 2 * warp]);
+            cur.len = lens(cur.seq);
+            cur.tiles = tilesOf(cur.len);
+            const long long pos = plan_s[5 + 2 * warp], cost = cur.tiles + kUnitCost;
+            cur.sub = static_cast<int>(pos / cost);
+            const int in = static_cast<int>(pos - cur.sub * cost) - kUnitCost; // below 0: in front of the unit's first tile
+            cur.tile = in > 0 ? in : 0;
+            place = start + (cur.tile - in);
+            cur.budget = static_cast<int>(end - place);
         }
-    };
-    auto fetch = [&](int slot) { // the next tile into a slot
-        if (next_at < count) {
+
+        // ---- copies: the tile after those in flight, its blocks already looked up
+        Cursor next = cur;
+        const unsigned char *table_row = nullptr;
+        long long code_unit = 0, scale_unit = 0; // offsets of the kv head
+        unsigned block0 = 0, block1 = 0;
+        int half0 = 0, half1 = 0; // first slots of the tile's halves within their blocks
+        const unsigned code_block = static_cast<unsigned>(a.k_block), scale_block = static_cast<unsigned>(a.ks_block);
+        const unsigned code_slot = static_cast<unsigned>(a.k_slot);
+        auto unit = [&]() {
             const int kv = next.sub / p.head_tiles;
-            const unsigned dst = smemAddr(ring + slot * C::kStage);
-            const long long c0 = block0 * a.k_block + kv * a.k_head + half0 * a.k_slot;
-            const long long c1 = block1 * a.k_block + kv * a.k_head + half1 * a.k_slot;
-#pragma unroll
-            for (int j = 0; j < CPR / 2; ++j) {
-                const int i = lane + 32 * j, r = i / CPR, c = i % CPR;
-                const int swz = CPR % 8 == 0 ? (r & 7) : CPR % 4 == 0 ? ((r >> 1) & 3) : ((r >> 2) & 1);
-                const unsigned to = dst + r * C::kRowBytes + ((c ^ swz) << 4);
-                const long long from = (r < 8 ? c0 : c1) + (r & 7) * a.k_slot + c * 16;
-                copy16(to, a.k_codes + from);
-                copy16(to + kTile * C::kRowBytes, a.v_codes + from);
-            }
-            // scales: a half's 8 rows are one run of NG chunks
-            if (lane < 4 * NG) {
-                const bool v = lane >= 2 * NG;
-                const int i = v ? lane - 2 * NG : lane, h = i >= NG;
-                const long long from = (h ? block1 : block0) * a.ks_block + kv * a.ks_head + (h ? half1 : half0) * NG + (i - h * NG) * 8;
-                copy16(dst + 2 * kTile * C::kRowBytes + lane * 16, (v ? a.v_scales : a.k_scales) + from);
-            }
-            next_at += kWarps;
-            if (next_at < count) {
-                advance(next, kWarps, p.subs, lens);
-                look();
-            }
-        }
-        commitCopies();
-    };
-    if (warp < count) {
-        if (warp > 0) {
-            advance(next, warp, p.subs, lens);
-        }
-        look();
-    }
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) {
-        fetch(i);
-    }
-    int slot = 0;
-
-    // lane's part of the matrix loads: matrix lane / 8, row lane % 8; matrices are (tokens 0-7 | 8-15) x (chunk, chunk + 1)
-    const int m_row = (lane & 7) + ((lane >> 3) & 1) * 8, m_chunk = lane >> 4;
-    const int m_swz = CPR % 8 == 0 ? (m_row & 7) : CPR % 4 == 0 ? ((m_row >> 1) & 3) : ((m_row >> 2) & 1);
-
-    Task cut = {0, 0, 0, 0};
-    int at = warp; // this warp's next tile within the range
-    for (int seg = 0; seg < count;) {
-        const int seg_tiles = min(cur.tiles - cur.tile, count - seg), seg_end = seg + seg_tiles;
-        const int kv = cur.sub / p.head_tiles;
-        const int head0 = (cur.sub - kv * p.head_tiles) * HT;      // within the group
-        const int heads = min(HT, a.group - head0);
-        const long long head_at = static_cast<long long>(kv) * a.group + head0;
-
-        // q as first operand, scaled by a power of two for each head; the scores' factor takes it back
-        unsigned qr[NH][HD / 16][2]; // [.][k step][a0 | a2]
-        float factor[NH], slope[NH];
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-            const int h = g + 8 * n;
-            unsigned raw[HD / 16][2];
-            unsigned largest = 0;
-            const unsigned short *q = static_cast<const unsigned short *>(a.q) + cur.seq * a.q_seq + (head_at + h) * a.q_head;
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j) { // 4 bits: 8 elements from 32 j + 8 t; 8 bits: 4 from 32 j + 4 t and 4 from + 16
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (h < heads) {
-                    if constexpr (BITS == 4) {
-                        x = *reinterpret_cast<const uint4 *>(q + 32 * j + 8 * t);
-                    } else {
-                        const uint2 lo = *reinterpret_cast<const uint2 *>(q + 32 * j + 4 * t);
-                        const uint2 hi = *reinterpret_cast<const uint2 *>(q + 32 * j + 16 + 4 * t);
-                        x = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                    }
+            table_row = static_cast<const unsigned char *>(a.block_tables) + ((next.seq * a.table_seq) << p.index_shift);
+            code_unit = kv * a.k_head;
+            scale_unit = kv * a.ks_head;
+        };
+        auto entry = [&](unsigned page) { // the low word of a 64-bit entry says all that a block in the pool can be
+            const unsigned char *at = table_row + (static_cast<unsigned long long>(page) << p.index_shift);
+            unsigned b = *reinterpret_cast<const unsigned *>(at);
+            if (a.check_indices) {
+                const long long whole = p.index_shift == 3 ? *reinterpret_cast<const long long *>(at) : static_cast<long long>(static_cast<int>(b));
+                if (static_cast<unsigned long long>(whole) >= static_cast<unsigned long long>(a.num_blocks)) {
+                    atomicOr(a.kernel_flags, INFINIOP_KERNEL_FLAG_BLOCK_OUT_OF_RANGE);
+                    b = 0;
                 }
-                raw[2 * j][0] = x.x;
-                raw[2 * j][1] = x.y;
-                raw[2 * j + 1][0] = x.z;
-                raw[2 * j + 1][1] = x.w;
-                const unsigned m = 0x7fff7fffu;
-                const unsigned b = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
-                largest = max(largest, max(b & 0xffffu, b >> 16));
             }
-            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-            auto wide = [&](unsigned half) {
-                return a.is_bf16 ? __uint_as_float(half << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(half)));
-            };
-            const int e = static_cast<int>(__float_as_uint(wide(largest)) >> 23); // biased
-            const int down = max(253 - e, 1);                                     // 2^(126 - e)
-            const float scale_q = __uint_as_float(static_cast<unsigned>(down) << 23);
-            factor[n] = a.scale_log2e * __uint_as_float(static_cast<unsigned>(254 - down) << 23);
-            slope[n] = a.alibi != nullptr && h < heads ? a.alibi[head_at + h] * 1.4426950408889634f : 0.f;
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const unsigned w = raw[2 * j + (i >> 1)][i & 1];
-                    x[2 * i] = wide(w & 0xffffu) * scale_q;
-                    x[2 * i + 1] = wide(w >> 16) * scale_q;
-                }
-                if constexpr (BITS == 4) { // the order of codes4
-                    qr[n][2 * j][0] = packHalves(x[0], x[4]);
-                    qr[n][2 * j][1] = packHalves(x[1], x[5]);
-                    qr[n][2 * j + 1][0] = packHalves(x[2], x[6]);
-                    qr[n][2 * j + 1][1] = packHalves(x[3], x[7]);
+            return b;
+        };
+        auto look = [&]() {
+            const unsigned h0 = 2u * static_cast<unsigned>(next.tile), halves = static_cast<unsigned>(a.block_size) >> 3;
+            const unsigned page = (__umulhi(h0, p.half_magic) + (h0 & p.half_self)) >> p.half_shift;
+            half0 = 8 * static_cast<int>(h0 - page * halves);
+            block0 = entry(page);
+            half1 = half0 + 8;
+            block1 = block0;
+            if (!p.pages_of_16 && half1 == a.block_size) {
+                // the second half is the next block's; behind the sequence's end it is read where the first is
+                if (8 * static_cast<int>(h0 + 1) < next.len) {
+                    block1 = entry(page + 1);
+                    half1 = 0;
                 } else {
-                    qr[n][2 * j][0] = packHalves(x[0], x[1]);
-                    qr[n][2 * j][1] = packHalves(x[2], x[3]);
-                    qr[n][2 * j + 1][0] = packHalves(x[4], x[5]);
-                    qr[n][2 * j + 1][1] = packHalves(x[6], x[7]);
+                    half1 = half0;
                 }
             }
+        };
+        auto fetch = [&](int slot) {
+            if (next.budget > 0) {
+                const unsigned dst = smemAddr(ring + slot * C::kStage);
+                const long long c0 = code_unit + static_cast<unsigned long long>(block0) * code_block + static_cast<unsigned long long>(half0) * code_slot;
+                const long long c1 = p.pages_of_16 ? c0 + 8ull * code_slot
+                                                   : code_unit + static_cast<unsigned long long>(block1) * code_block
+                                                         + static_cast<unsigned long long>(half1) * code_slot;
+#pragma unroll
+                for (int j = 0; j < CPR / 2; ++j) {
+                    const int i = lane + 32 * j, r = i / CPR, c = i % CPR;
+                    const int swz = CPR % 8 == 0 ? (r & 7) : CPR % 4 == 0 ? ((r >> 1) & 3) : ((r >> 2) & 1);
+                    const unsigned to = dst + r * C::kRowBytes + ((c ^ swz) << 4);
+                    const long long from = (r < 8 ? c0 : c1) + (static_cast<unsigned>(r & 7) * code_slot + c * 16);
+                    copy16(to, a.k_codes + from);
+                    copy16(to + kTile * C::kRowBytes, a.v_codes + from);
+                }
+                // scales: a half's 8 rows are one run of NG chunks
+                if (lane < 4 * NG) {
+                    const bool v = lane >= 2 * NG;
+                    const int i = v ? lane - 2 * NG : lane;
+                    const bool h = i >= NG;
+                    const long long from = scale_unit + static_cast<unsigned long long>(h ? block1 : block0) * scale_block
+                                         + ((h ? half1 : half0) * NG + (h ? i - NG : i) * 8);
+                    copy16(dst + 2 * kTile * C::kRowBytes + lane * 16, (v ? a.v_scales : a.k_scales) + from);
+                }
+                if (next.step(p.subs, lens)) {
+                    unit();
+                }
+                if (next.budget > 0) {
+                    look();
+                }
+            }
+            commitCopies();
+        };
+        unit();
+        look();
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) {
+            fetch(i);
         }
+        int slot = 0;
 
-        float top[NH], sum[NH], o[NH][HD / 16][4];
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-            top[n] = kLowest;
-            sum[n] = 0.f;
-#pragma unroll
-            for (int j = 0; j < HD / 16; ++j) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[n][j][i] = 0.f;
-                }
-            }
-        }
+        // lane's part of the matrix loads: matrix lane / 8, row lane % 8; matrices are (tokens 0-7 | 8-15) x (chunk, chunk + 1)
+        const int m_row = (lane & 7) + ((lane >> 3) & 1) * 8, m_chunk = lane >> 4;
+        const int m_swz = CPR % 8 == 0 ? (m_row & 7) : CPR % 4 == 0 ? ((m_row >> 1) & 3) : ((m_row >> 2) & 1);
 
-        for (; at < seg_end; at += kWarps) {
-            waitCopies<S - 2>();
-            __syncwarp();
-            const unsigned char *stage = ring + slot * C::kStage;
-            fetch(slot == 0 ? S - 1 : slot - 1);
-            slot = slot == S - 1 ? 0 : slot + 1;
-            const int token0 = (cur.tile + at - seg) * kTile;
-            const unsigned k_addr = smemAddr(stage) + m_row * C::kRowBytes, v_addr = k_addr + kTile * C::kRowBytes;
+        while (cur.budget > 0) { // a unit, or what of it is in the range
+            const int kv = cur.sub / p.head_tiles;
+            const int head0 = (cur.sub - kv * p.head_tiles) * HT; // within the group
+            const int heads = min(HT, a.group - head0);
+            const long long head_at = static_cast<long long>(kv) * a.group + head0;
+            const long long unit_first = place - cur.tile;
+            const int unit_seq = cur.seq, unit_sub = cur.sub, unit_tiles = cur.tiles, len = cur.len;
 
-            // scales of the lane's tokens 2t, 2t + 1 (pair 0) and 2t + 8, 2t + 9 (pair 1): words [pair][token][group / 2]
-            constexpr int kWords = NG == 1 ? 1 : NG; // of a pair
-            unsigned ks[2][kWords], vs[2][kWords];
-            {
-                const unsigned char *s = stage + 2 * kTile * C::kRowBytes;
+            // q as first operand, scaled by a power of two for each head; the scores' factor takes it back
+            unsigned qr[NH][HD / 16][2]; // [.][k step][a0 | a2]
+            float factor[NH], slope[NH];
 #pragma unroll
-                for (int pair = 0; pair < 2; ++pair) {
-                    const unsigned *kp = reinterpret_cast<const unsigned *>(s) + (pair * 4 + t) * kWords;
-                    const unsigned *vp = kp + kTile * NG / 2;
-                    if constexpr (kWords % 4 == 0) {
+            for (int n = 0; n < NH; ++n) {
+                const int h = g + 8 * n;
+                unsigned raw[HD / 16][2];
+                unsigned largest = 0;
+                const unsigned short *q = static_cast<const unsigned short *>(a.q) + cur.seq * a.q_seq + (head_at + h) * a.q_head;
 #pragma unroll
-                        for (int i = 0; i < kWords / 4; ++i) {
-                            const uint4 x = reinterpret_cast<const uint4 *>(kp)[i], y = reinterpret_cast<const uint4 *>(vp)[i];
-                            ks[pair][4 * i] = x.x, ks[pair][4 * i + 1] = x.y, ks[pair][4 * i + 2] = x.z, ks[pair][4 * i + 3] = x.w;
-                            vs[pair][4 * i] = y.x, vs[pair][4 * i + 1] = y.y, vs[pair][4 * i + 2] = y.z, vs[pair][4 * i + 3] = y.w;
+                for (int j = 0; j < HD / 32; ++j) { // 4 bits: 8 elements from 32 j + 8 t; 8 bits: 4 from 32 j + 4 t and 4 from + 16
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (h < heads) {
+                        if constexpr (BITS == 4) {
+                            x = *reinterpret_cast<const uint4 *>(q + 32 * j + 8 * t);
+                        } else {
+                            const uint2 lo = *reinterpret_cast<const uint2 *>(q + 32 * j + 4 * t);
+                            const uint2 hi = *reinterpret_cast<const uint2 *>(q + 32 * j + 16 + 4 * t);
+                            x = make_uint4(lo.x, lo.y, hi.x, hi.y);
                         }
-                    } else if constexpr (kWords % 2 == 0) {
-#pragma unroll
-                        for (int i = 0; i < kWords / 2; ++i) {
-                            const uint2 x = reinterpret_cast<const uint2 *>(kp)[i], y = reinterpret_cast<const uint2 *>(vp)[i];
-                            ks[pair][2 * i] = x.x, ks[pair][2 * i + 1] = x.y;
-                            vs[pair][2 * i] = y.x, vs[pair][2 * i + 1] = y.y;
-                        }
-                    } else {
-                        ks[pair][0] = kp[0];
-                        vs[pair][0] = vp[0];
                     }
+                    raw[2 * j][0] = x.x;
+                    raw[2 * j][1] = x.y;
+                    raw[2 * j + 1][0] = x.z;
+                    raw[2 * j + 1][1] = x.w;
+                    const unsigned m = 0x7fff7fffu;
+                    const unsigned b = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
+                    largest = max(largest, max(b & 0xffffu, b >> 16));
                 }
-            }
-            // scale of token x (0, 1) of a pair and group j: NG == 1 keeps both tokens in one word
-            auto scaleAt = [](const unsigned (&w)[kWords], int x, int j) {
-                const unsigned word = NG == 1 ? w[0] : w[x * (NG / 2) + j / 2];
-                return __uint_as_float((NG == 1 ? x : j & 1) ? word & 0xffff0000u : word << 16);
-            };
-
-            // scores
-            float s[2][NH][2]; // [pair][head tile][token]
-            {
-                float acc[2][4];
+                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                auto wide = [&](unsigned half) {
+                    return a.is_bf16 ? __uint_as_float(half << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(half)));
+                };
+                const int e = static_cast<int>(__float_as_uint(wide(largest)) >> 23); // biased
+                const int down = max(253 - e, 1);                                     // 2^(126 - e)
+                const float scale_q = __uint_as_float(static_cast<unsigned>(down) << 23);
+                factor[n] = a.scale_log2e * __uint_as_float(static_cast<unsigned>(254 - down) << 23);
+                slope[n] = a.alibi != nullptr && h < heads ? a.alibi[head_at + h] * 1.4426950408889634f : 0.f;
 #pragma unroll
-                for (int pair = 0; pair < 2; ++pair) {
-#pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-                        s[pair][n][0] = s[pair][n][1] = 0.f;
-                    }
+                for (int j = 0; j < HD / 32; ++j) {
+                    float x[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        acc[pair][i] = 0.f;
+                        const unsigned w = raw[2 * j + (i >> 1)][i & 1];
+                        x[2 * i] = wide(w & 0xffffu) * scale_q;
+                        x[2 * i + 1] = wide(w >> 16) * scale_q;
+                    }
+                    if constexpr (BITS == 4) { // the order of codes4
+                        qr[n][2 * j][0] = packHalves(x[0], x[4]);
+                        qr[n][2 * j][1] = packHalves(x[1], x[5]);
+                        qr[n][2 * j + 1][0] = packHalves(x[2], x[6]);
+                        qr[n][2 * j + 1][1] = packHalves(x[3], x[7]);
+                    } else {
+                        qr[n][2 * j][0] = packHalves(x[0], x[1]);
+                        qr[n][2 * j][1] = packHalves(x[2], x[3]);
+                        qr[n][2 * j + 1][0] = packHalves(x[4], x[5]);
+                        qr[n][2 * j + 1][1] = packHalves(x[6], x[7]);
                     }
                 }
+            }
+
+            float top[NH], sum[NH], o[NH][HD / 16][4];
 #pragma unroll
-                for (int c = 0; c < CPR; c += 2) {
-                    unsigned w[4];
-                    loadMatrices(w, k_addr + (((c + m_chunk) ^ m_swz) << 4));
+            for (int n = 0; n < NH; ++n) {
+                top[n] = kLowest;
+                sum[n] = 0.f;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) { // the two chunks
+                for (int j = 0; j < HD / 16; ++j) {
 #pragma unroll
-                        for (int pair = 0; pair < 2; ++pair) {
-                            const unsigned word = w[2 * x + pair];
-                            if constexpr (BITS == 4) {
-                                const int j = c + x;
-                                unsigned b[4];
-                                codes4(word, b);
-                                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma(d, qr[0][2 * j][0], NH == 2 ? qr[NH - 1][2 * j][0] : 0u, qr[0][2 * j][1], NH == 2 ? qr[NH - 1][2 * j][1] : 0u,
-                                    b[0], b[1]);
-                                mma(d, qr[0][2 * j + 1][0], NH == 2 ? qr[NH - 1][2 * j + 1][0] : 0u, qr[0][2 * j + 1][1],
-                                    NH == 2 ? qr[NH - 1][2 * j + 1][1] : 0u, b[2], b[3]);
-                                const float s0 = scaleAt(ks[pair], 0, j), s1 = scaleAt(ks[pair], 1, j);
+                    for (int i = 0; i < 4; ++i) {
+                        o[n][j][i] = 0.f;
+                    }
+                }
+            }
+
+            bool more;
+            int token0 = cur.tile * kTile;
+            do {
+                waitCopies<S - 2>();
+                __syncwarp();
+                const unsigned char *stage = ring + slot * C::kStage;
+                fetch(slot == 0 ? S - 1 : slot - 1);
+                slot = slot == S - 1 ? 0 : slot + 1;
+                const unsigned k_addr = smemAddr(stage) + m_row * C::kRowBytes, v_addr = k_addr + kTile * C::kRowBytes;
+
+                // scales of the lane's tokens 2t, 2t + 1 (pair 0) and 2t + 8, 2t + 9 (pair 1): words [pair][token][group / 2]
+                constexpr int kWords = NG; // of a pair
+                unsigned ks[2][kWords], vs[2][kWords];
+                {
+                    const unsigned char *sc = stage + 2 * kTile * C::kRowBytes;
 #pragma unroll
-                                for (int n = 0; n < NH; ++n) {
-                                    s[pair][n][0] = fmaf(s0, d[2 * n], s[pair][n][0]);
-                                    s[pair][n][1] = fmaf(s1, d[2 * n + 1], s[pair][n][1]);
-                                }
-                            } else {
-                                const int j = c + x;
-                                const unsigned f = word ^ 0x80808080u;
-                                mma(acc[pair], qr[0][j][0], NH == 2 ? qr[NH - 1][j][0] : 0u, qr[0][j][1], NH == 2 ? qr[NH - 1][j][1] : 0u,
-                                    codes8<0x4140>(f), codes8<0x4342>(f));
+                    for (int pair = 0; pair < 2; ++pair) {
+                        const unsigned *kp = reinterpret_cast<const unsigned *>(sc) + (pair * 4 + t) * kWords;
+                        const unsigned *vp = kp + kTile * NG / 2;
+                        if constexpr (kWords % 4 == 0) {
+#pragma unroll
+                            for (int i = 0; i < kWords / 4; ++i) {
+                                const uint4 x = reinterpret_cast<const uint4 *>(kp)[i], y = reinterpret_cast<const uint4 *>(vp)[i];
+                                ks[pair][4 * i] = x.x, ks[pair][4 * i + 1] = x.y, ks[pair][4 * i + 2] = x.z, ks[pair][4 * i + 3] = x.w;
+                                vs[pair][4 * i] = y.x, vs[pair][4 * i + 1] = y.y, vs[pair][4 * i + 2] = y.z, vs[pair][4 * i + 3] = y.w;
                             }
+                        } else if constexpr (kWords % 2 == 0) {
+#pragma unroll
+                            for (int i = 0; i < kWords / 2; ++i) {
+                                const uint2 x = reinterpret_cast<const uint2 *>(kp)[i], y = reinterpret_cast<const uint2 *>(vp)[i];
+                                ks[pair][2 * i] = x.x, ks[pair][2 * i + 1] = x.y;
+                                vs[pair][2 * i] = y.x, vs[pair][2 * i + 1] = y.y;
+                            }
+                        } else {
+                            ks[pair][0] = kp[0];
+                            vs[pair][0] = vp[0];
                         }
                     }
                 }
-                if constexpr (BITS == 8) {
+                // scale of token x (0, 1) of a pair and group j: NG == 1 keeps both tokens in one word
+                auto scaleAt = [](const unsigned (&w)[kWords], int x, int j) {
+                    const unsigned word = NG == 1 ? w[0] : w[x * (NG / 2) + j / 2];
+                    return __uint_as_float((NG == 1 ? x : j & 1) ? word & 0xffff0000u : word << 16);
+                };
+
+                // scores
+                float s[2][NH][2]; // [pair][head tile][token]
+                {
+                    float acc[2][4];
 #pragma unroll
                     for (int pair = 0; pair < 2; ++pair) {
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
-                            s[pair][n][0] = acc[pair][2 * n] * scaleAt(ks[pair], 0, 0);
-                            s[pair][n][1] = acc[pair][2 * n + 1] * scaleAt(ks[pair], 1, 0);
+                            s[pair][n][0] = s[pair][n][1] = 0.f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            acc[pair][i] = 0.f;
                         }
                     }
-                }
-            }
 #pragma unroll
-            for (int pair = 0; pair < 2; ++pair) {
+                    for (int c = 0; c < CPR; c += 2) {
+                        unsigned w[4];
+                        loadMatrices(w, k_addr + (((c + m_chunk) ^ m_swz) << 4));
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int token = token0 + 8 * pair + 2 * t + x;
+                        for (int x = 0; x < 2; ++x) { // the two chunks
+                            const int j = c + x;
 #pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-                        s[pair][n][x] *= factor[n];
-                        if (a.alibi != nullptr) {
-                            s[pair][n][x] += slope[n] * static_cast<float>(token - (cur.len - 1));
+                            for (int pair = 0; pair < 2; ++pair) {
+                                const unsigned word = w[2 * x + pair];
+                                if constexpr (BITS == 4) {
+                                    unsigned b[4];
+                                    codes4(word, b);
+                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma(d, qr[0][2 * j][0], NH == 2 ? qr[NH - 1][2 * j][0] : 0u, qr[0][2 * j][1], NH == 2 ? qr[NH - 1][2 * j][1] : 0u,
+                                        b[0], b[1]);
+                                    mma(d, qr[0][2 * j + 1][0], NH == 2 ? qr[NH - 1][2 * j + 1][0] : 0u, qr[0][2 * j + 1][1],
+                                        NH == 2 ? qr[NH - 1][2 * j + 1][1] : 0u, b[2], b[3]);
+                                    const float s0 = scaleAt(ks[pair], 0, j), s1 = scaleAt(ks[pair], 1, j);
+#pragma unroll
+                                    for (int n = 0; n < NH; ++n) {
+                                        s[pair][n][0] = fmaf(s0, d[2 * n], s[pair][n][0]);
+                                        s[pair][n][1] = fmaf(s1, d[2 * n + 1], s[pair][n][1]);
+                                    }
+                                } else {
+                                    const unsigned f = word ^ 0x80808080u;
+                                    mma(acc[pair], qr[0][j][0], NH == 2 ? qr[NH - 1][j][0] : 0u, qr[0][j][1], NH == 2 ? qr[NH - 1][j][1] : 0u,
+                                        codes8<0x4140>(f), codes8<0x4342>(f));
+                                }
+                            }
                         }
                     }
-                    if (token0 + kTile > cur.len && token >= cur.len) { // behind the end: no weight, whatever the scales are
+#pragma unroll
+                    for (int pair = 0; pair < 2; ++pair) {
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
-                            s[pair][n][x] = -INFINITY;
-                        }
-                        if constexpr (NG == 1) {
-                            vs[pair][0] &= x ? 0x0000ffffu : 0xffff0000u;
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < NG / 2; ++i) {
-                                vs[pair][x * (NG / 2) + i] = 0u;
+                            if constexpr (BITS == 8) {
+                                s[pair][n][0] = acc[pair][2 * n] * scaleAt(ks[pair], 0, 0);
+                                s[pair][n][1] = acc[pair][2 * n + 1] * scaleAt(ks[pair], 1, 0);
                             }
+                            s[pair][n][0] *= factor[n];
+                            s[pair][n][1] *= factor[n];
                         }
                     }
                 }
-            }
-
-            // how far a token's weights can reach above its p: the exponent of its largest V scale, NaN ones left out
-            float reach[2][2];
+                if (a.alibi != nullptr) {
 #pragma unroll
-            for (int pair = 0; pair < 2; ++pair) {
+                    for (int i = 0; i < 4; ++i) {
+                        const float far = static_cast<float>(token0 + 8 * (i >> 1) + 2 * t + (i & 1) - (len - 1));
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    unsigned most;
-                    if constexpr (NG == 1) {
-                        most = x ? vs[pair][0] >> 16 : vs[pair][0] & 0xffffu;
-                        most = most < 0x7f80u ? most : 0u;
-                    } else {
-                        unsigned m = vs[pair][x * (NG / 2)];
-#pragma unroll
-                        for (int i = 1; i < NG / 2; ++i) {
-                            m = __vmaxu2(m, vs[pair][x * (NG / 2) + i]);
-                        }
-                        most = max(m & 0xffffu, m >> 16);
-                        if (most >= 0x7f80u) {
-                            most = 0;
-#pragma unroll
-                            for (int i = 0; i < NG / 2; ++i) {
-                                const unsigned w = vs[pair][x * (NG / 2) + i], lo = w & 0xffffu, hi = w >> 16;
-                                most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-                            }
+                        for (int n = 0; n < NH; ++n) {
+                            s[i >> 1][n][i & 1] += slope[n] * far;
                         }
                     }
-                    const unsigned e = max(most >> 7, kLeastExp);
-                    reach[pair][x] = __uint_as_float(0x4b000000u | e) - (8388608.f + 126.f); // >= log2 of the scale
                 }
-            }
-
-            // the maximum moves rarely
-            float high[NH];
-            bool move = false;
+                if (token0 + kTile > len) { // tokens behind the end have no weight, whatever their scales are
 #pragma unroll
-            for (int n = 0; n < NH; ++n) {
-                high[n] = fmaxf(fmaxf(s[0][n][0] + reach[0][0], s[0][n][1] + reach[0][1]), fmaxf(s[1][n][0] + reach[1][0], s[1][n][1] + reach[1][1]));
-                move |= high[n] > top[n] + kSlack;
-            }
-            if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-                for (int n = 0; n < NH; ++n) {
-                    high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 1));
-                    high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 2));
-                    const float now = fmaxf(top[n], high[n]);
-                    const float alpha = exp2Fast(top[n] - now); // the first time: 0
-                    top[n] = now;
-                    sum[n] *= alpha;
-                    const float alpha0 = __shfl_sync(0xffffffffu, alpha, 8 * t), alpha1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
-#pragma unroll
-                    for (int j = 0; j < HD / 16; ++j) {
-                        o[n][j][0] *= alpha0;
-                        o[n][j][1] *= alpha1;
-                        o[n][j][2] *= alpha0;
-                        o[n][j][3] *= alpha1;
-                    }
-                }
-            }
-#pragma unroll
-            for (int pair = 0; pair < 2; ++pair) {
-#pragma unroll
-                for (int n = 0; n < NH; ++n) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        s[pair][n][x] = exp2Fast(s[pair][n][x] - top[n]);
-                    }
-                    sum[n] += s[pair][n][0] + s[pair][n][1];
-                }
-            }
-
-            // outputs
-            unsigned weight[NH][2];
-#pragma unroll
-            for (int c = 0; c < CPR; c += 2) {
-                unsigned w[4];
-                loadMatricesTransposed(w, v_addr + (((c + m_chunk) ^ m_swz) << 4));
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int j = c + x;
-                    if (BITS == 4 || j == 0) { // the weights of this group
-#pragma unroll
-                        for (int pair = 0; pair < 2; ++pair) {
-                            const float v0 = scaleAt(vs[pair], 0, BITS == 4 ? j : 0), v1 = scaleAt(vs[pair], 1, BITS == 4 ? j : 0);
+                    for (int i = 0; i < 4; ++i) {
+                        const int pair = i >> 1, x = i & 1;
+                        if (token0 + 8 * pair + 2 * t + x >= len) {
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
-                                weight[n][pair] = packHalves(s[pair][n][0] * v0, s[pair][n][1] * v1);
+                                s[pair][n][x] = -INFINITY;
+                            }
+                            if constexpr (NG == 1) {
+                                vs[pair][0] &= x ? 0x0000ffffu : 0xffff0000u;
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < NG / 2; ++k) {
+                                    vs[pair][x * (NG / 2) + k] = 0u;
+                                }
                             }
                         }
                     }
-                    if constexpr (BITS == 4) {
-                        unsigned lo[4], hi[4];
-                        codes4Odd16(w[2 * x], lo);
-                        codes4Odd16(w[2 * x + 1], hi);
+                }
+
+                // How far a token's weights can reach above its p: log2 of its largest V scale is at most bits / 128 - 126.9 for a
+                // bf16 with these bits (log2(1 + f) <= f + 0.0861).  The constant stays out; it is taken off with the maximum.
+                float high[NH];
+                {
+                    float bits[2][2];
 #pragma unroll
-                        for (int n = 0; n < NH; ++n) {
-                            mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], weight[n][0], weight[n][1]);
-                            mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], weight[n][0], weight[n][1]);
+                    for (int pair = 0; pair < 2; ++pair) {
+                        unsigned both = vs[pair][0]; // tokens 0 | 1, their largest
+                        if constexpr (NG > 1) {
+                            unsigned m0 = vs[pair][0], m1 = vs[pair][NG / 2];
+#pragma unroll
+                            for (int k = 1; k < NG / 2; ++k) {
+                                m0 = __vmaxu2(m0, vs[pair][k]);
+                                m1 = __vmaxu2(m1, vs[pair][NG / 2 + k]);
+                            }
+                            both = __vmaxu2(__byte_perm(m0, m1, 0x5410), __byte_perm(m0, m1, 0x7632));
                         }
-                    } else {
-                        const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
-                        const unsigned a0 = codes8<0x4240>(lo), a1 = codes8<0x4341>(lo), a2 = codes8<0x4240>(hi), a3 = codes8<0x4341>(hi);
+                        both = __vmaxu2(both, kLeastScale | (kLeastScale << 16));
+                        bits[pair][0] = __uint_as_float(__byte_perm(both, 0x4b000000u, 0x7610)); // 2^23 + bits
+                        bits[pair][1] = __uint_as_float(__byte_perm(both, 0x4b000000u, 0x7632));
+                    }
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        high[n] = kLowest;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            high[n] = fmaxf(high[n], fmaf(bits[i >> 1][i & 1], 0.0078125f, s[i >> 1][n][i & 1]));
+                        }
+                    }
+                }
+                constexpr float kBias = 65536.f + 126.9f; // 2^23 / 128 and the constant
+                // the maximum moves rarely
+                bool move = false;
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+                    high[n] -= kBias;
+                    move |= high[n] > top[n] + kSlack;
+                }
+                if (__any_sync(0xffffffffu, move)) {
+                    // a NaN scale would count as 2^129: such tokens count without theirs
+                    bool nan_scale = false;
+#pragma unroll
+                    for (int pair = 0; pair < 2; ++pair) {
+#pragma unroll
+                        for (int k = 0; k < kWords; ++k) {
+                            nan_scale |= (vs[pair][k] & 0xffffu) >= 0x7f80u || (vs[pair][k] >> 16) >= 0x7f80u;
+                        }
+                    }
+                    if (nan_scale) {
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
-                            mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
+                            high[n] = kLowest;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            unsigned most = kLeastScale;
+#pragma unroll
+                            for (int k = 0; k < (NG == 1 ? 1 : NG / 2); ++k) {
+                                const unsigned w = vs[i >> 1][NG == 1 ? 0 : (i & 1) * (NG / 2) + k], lo = w & 0xffffu, hi = w >> 16;
+                                if (NG > 1 || (i & 1) == 0) {
+                                    most = max(most, lo < 0x7f80u ? lo : 0u);
+                                }
+                                if (NG > 1 || (i & 1) == 1) {
+                                    most = max(most, hi < 0x7f80u ? hi : 0u);
+                                }
+                            }
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                high[n] = fmaxf(high[n], s[i >> 1][n][i & 1] + (static_cast<float>(most) * 0.0078125f - 126.9f));
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 1));
+                        high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 2));
+                        const float now = fmaxf(top[n], high[n]);
+                        const float alpha = exp2Fast(top[n] - now); // the first time: 0
+                        top[n] = now;
+                        sum[n] *= alpha;
+                        const float alpha0 = __shfl_sync(0xffffffffu, alpha, 8 * t), alpha1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
+#pragma unroll
+                        for (int j = 0; j < HD / 16; ++j) {
+                            o[n][j][0] *= alpha0;
+                            o[n][j][1] *= alpha1;
+                            o[n][j][2] *= alpha0;
+                            o[n][j][3] *= alpha1;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int pair = 0; pair < 2; ++pair) {
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            s[pair][n][x] = exp2Fast(s[pair][n][x] - top[n]);
+                        }
+                        sum[n] += s[pair][n][0] + s[pair][n][1];
+                    }
+                }
+
+                // outputs
+                unsigned weight[NH][2];
+#pragma unroll
+                for (int c = 0; c < CPR; c += 2) {
+                    unsigned w[4];
+                    loadMatricesTransposed(w, v_addr + (((c + m_chunk) ^ m_swz) << 4));
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int j = c + x;
+                        if (BITS == 4 || j == 0) { // the weights of this group
+#pragma unroll
+                            for (int pair = 0; pair < 2; ++pair) {
+                                const float v0 = scaleAt(vs[pair], 0, BITS == 4 ? j : 0), v1 = scaleAt(vs[pair], 1, BITS == 4 ? j : 0);
+#pragma unroll
+                                for (int n = 0; n < NH; ++n) {
+                                    weight[n][pair] = packHalves(s[pair][n][0] * v0, s[pair][n][1] * v1);
+                                }
+                            }
+                        }
+                        if constexpr (BITS == 4) {
+                            unsigned lo[4], hi[4];
+                            codes4Odd16(w[2 * x], lo);
+                            codes4Odd16(w[2 * x + 1], hi);
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], weight[n][0], weight[n][1]);
+                                mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], weight[n][0], weight[n][1]);
+                            }
+                        } else {
+                            const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
+                            const unsigned a0 = codes8<0x4240>(lo), a1 = codes8<0x4341>(lo), a2 = codes8<0x4240>(hi), a3 = codes8<0x4341>(hi);
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
+                            }
+                        }
+                    }
+                }
+                token0 += kTile;
+                ++place;
+                more = !cur.step(p.subs, lens) && cur.budget > 0;
+            } while (more);
+
+            // the unit's rows, or this warp's piece of it
+            const bool first = unit_first >= start, last = unit_first + unit_tiles <= end;
+            place = unit_first + unit_tiles + kUnitCost; // if the range goes on, it does with the next unit
+            float inv[NH];
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+                sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
+                sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
+                inv[n] = 1.f / sum[n];
+            }
+            if (!(first && last) && lane == 0) {
+                pieces[2 * warp + first] = {unit_first, unit_seq, unit_sub, unit_tiles, 1};
+            }
+            // a piece in front is kept beside the ring, one at the range's end in the ring, which is empty then
+            float *mine_o = first ? reinterpret_cast<float *>(ring) : results + warp * HT * C::kStride;
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+                constexpr int kPer = BITS == 4 ? 4 : 2; // neighbouring elements of a row that a lane has
+                constexpr int kRuns = HD / (8 * kPer);
+                if (first && last) {
+                    const float inv0 = __shfl_sync(0xffffffffu, inv[n], 8 * t), inv1 = __shfl_sync(0xffffffffu, inv[n], 8 * t + 4);
+                    const long long row = unit_seq * a.o_seq + (head_at + 8 * n + 2 * t) * a.o_head;
+#pragma unroll
+                    for (int j = 0; j < kRuns; ++j) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float f = x ? inv1 : inv0;
+                            float v[kPer];
+                            v[0] = o[n][BITS == 4 ? 2 * j : j][x] * f;
+                            v[1] = o[n][BITS == 4 ? 2 * j : j][2 + x] * (BITS == 4 ? f * 0.0625f : f);
+                            if constexpr (BITS == 4) {
+                                v[2] = o[n][2 * j + 1][x] * f;
+                                v[3] = o[n][2 * j + 1][2 + x] * (f * 0.0625f);
+                            }
+                            if (8 * n + 2 * t + x < heads) {
+                                storeOut(a, p, row + x * a.o_head + 8 * kPer * j + kPer * g, v);
+                            }
+                        }
+                    }
+                } else {
+                    if (t == 0) {
+                        sums[(2 * warp + first) * HT + 8 * n + g] = make_float2(top[n], sum[n]);
+                    }
+                    float *row0 = mine_o + (8 * n + 2 * t) * C::kStride, *row1 = row0 + C::kStride;
+#pragma unroll
+                    for (int j = 0; j < kRuns; ++j) {
+                        if constexpr (BITS == 4) {
+                            const float(&x)[4] = o[n][2 * j], (&y)[4] = o[n][2 * j + 1];
+                            *reinterpret_cast<float4 *>(row0 + 32 * j + 4 * g) = make_float4(x[0], x[2] * 0.0625f, y[0], y[2] * 0.0625f);
+                            *reinterpret_cast<float4 *>(row1 + 32 * j + 4 * g) = make_float4(x[1], x[3] * 0.0625f, y[1], y[3] * 0.0625f);
+                        } else {
+                            *reinterpret_cast<float2 *>(row0 + 16 * j + 2 * g) = make_float2(o[n][j][0], o[n][j][2]);
+                            *reinterpret_cast<float2 *>(row1 + 16 * j + 2 * g) = make_float2(o[n][j][1], o[n][j][3]);
                         }
                     }
                 }
             }
         }
+    }
 
-        // the four warps' results of this unit meet
-        float *mine_o = merge + warp * HT * C::kMergeStride;
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-            sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
-            sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
-            if (t == 0) {
-                merge_ml[warp * HT + 8 * n + g] = make_float2(top[n], sum[n]);
-            }
-            float *row0 = mine_o + (8 * n + 2 * t) * C::kMergeStride, *row1 = row0 + C::kMergeStride;
-            if constexpr (BITS == 4) {
-#pragma unroll
-                for (int j = 0; j < HD / 32; ++j) {
-                    const float(&x)[4] = o[n][2 * j], (&y)[4] = o[n][2 * j + 1];
-                    *reinterpret_cast<float4 *>(row0 + 32 * j + 4 * g) = make_float4(x[0], x[2] * 0.0625f, y[0], y[2] * 0.0625f);
-                    *reinterpret_cast<float4 *>(row1 + 32 * j + 4 * g) = make_float4(x[1], x[3] * 0.0625f, y[1], y[3] * 0.0625f);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j) {
-                    *reinterpret_cast<float2 *>(row0 + 16 * j + 2 * g) = make_float2(o[n][j][0], o[n][j][2]);
-                    *reinterpret_cast<float2 *>(row1 + 16 * j + 2 * g) = make_float2(o[n][j][1], o[n][j][3]);
-                }
-            }
+    // ---- the pieces that this CTA's warps left: those of one unit are neighbours
+    __syncthreads();
+    Task cut = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int k = 0; k < 2 * kWarps;) {
+        const Piece piece = pieces[k];
+        if (!piece.used) {
+            ++k;
+            continue;
         }
-        __syncthreads();
-        const bool first = cur.tile == 0, last = cur.tile + seg_tiles == cur.tiles;
+        int upto_k = k + 1; // members: used pieces from k on with the same unit
+        while (upto_k < 2 * kWarps && (!pieces[upto_k].used || pieces[upto_k].first == piece.first)) {
+            ++upto_k;
+        }
+        const int kv = piece.sub / p.head_tiles, head0 = (piece.sub - kv * p.head_tiles) * HT, heads = min(HT, a.group - head0);
+        const long long head_at = static_cast<long long>(kv) * a.group + head0;
+        const bool first = piece.first >= cta_start, last = piece.first + piece.tiles <= cta_start + cta_range;
         float *record = reinterpret_cast<float *>(p.workspace + p.tasks_bytes) + (2ll * blockIdx.x + (first ? 1 : 0)) * C::kRecord;
         for (int i = tid; i < heads * (HD / 4); i += kThreads) {
             const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
             float m = kLowest;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                m = fmaxf(m, merge_ml[w * HT + h].x);
+            for (int w = k; w < upto_k; ++w) {
+                m = pieces[w].used ? fmaxf(m, sums[w * HT + h].x) : m;
             }
             float l = 0.f;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float2 ml = merge_ml[w * HT + h];
-                const float f = exp2Fast(ml.x - m); // a warp without a token has kLowest and 0
-                const float4 x = *reinterpret_cast<const float4 *>(merge + (w * HT + h) * C::kMergeStride + d);
-                l = fmaf(f, ml.y, l);
-                v.x = fmaf(f, x.x, v.x);
-                v.y = fmaf(f, x.y, v.y);
-                v.z = fmaf(f, x.z, v.z);
-                v.w = fmaf(f, x.w, v.w);
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int w = k; w < upto_k; ++w) {
+                if (pieces[w].used) {
+                    const float2 ml = sums[w * HT + h];
+                    const float f = exp2Fast(ml.x - m);
+                    const float *from = (w & 1) ? reinterpret_cast<const float *>(smem + (w >> 1) * C::kRing) : results + (w >> 1) * HT * C::kStride;
+                    const float4 x = *reinterpret_cast<const float4 *>(from + h * C::kStride + d);
+                    l = fmaf(f, ml.y, l);
+                    v[0] = fmaf(f, x.x, v[0]);
+                    v[1] = fmaf(f, x.y, v[1]);
+                    v[2] = fmaf(f, x.z, v[2]);
+                    v[3] = fmaf(f, x.w, v[3]);
+                }
             }
             if (first && last) {
                 const float inv = 1.f / l;
-                unsigned short *dst = static_cast<unsigned short *>(a.out) + cur.seq * a.o_seq + (head_at + h) * a.o_head + d;
-                const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    dst[k] = a.is_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y[k])) : __half_as_ushort(__float2half_rn(y[k]));
+                for (int x = 0; x < 4; ++x) {
+                    v[x] *= inv;
                 }
+                storeOut(a, p, piece.seq * a.o_seq + (head_at + h) * a.o_head + d, v);
             } else {
-                *reinterpret_cast<float4 *>(record + h * HD + d) = v;
+                *reinterpret_cast<float4 *>(record + h * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
                 if (d == 0) {
                     record[HT * HD + h] = m;
                     record[HT * HD + HT + h] = l;
                 }
             }
         }
-        if (first && !last) { // this CTA's last unit: it names the pieces for the combine kernel
-            cut.seq = cur.seq;
-            cut.sub = cur.sub;
-            cut.pieces = static_cast<int>((start + seg + cur.tiles - 1) / range - blockIdx.x) + 1;
+        if (first && !last) { // the CTA's last unit: it names the pieces for the combine kernel
+            cut.seq = piece.seq;
+            cut.sub = piece.sub;
+            cut.pieces = static_cast<int>((piece.first + piece.tiles - 1) / cta_range - blockIdx.x) + 1;
         }
-        __syncthreads();
-        seg = seg_end;
-        if (seg < count) {
-            advance(cur, seg_tiles, p.subs, lens);
-        }
+        k = upto_k;
     }
     if (tid == 0) {
         *task = cut;
@@ -785,13 +956,8 @@ __global__ void __launch_bounds__(256) quantAttentionCombineKernel(const Attenti
             v.w = fmaf(f, x.w, v.w);
         }
         const float inv = 1.f / l;
-        unsigned short *dst =
-            static_cast<unsigned short *>(a.out) + task.seq * a.o_seq + (static_cast<long long>(kv) * a.group + head0 + h) * a.o_head + d;
         const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            dst[k] = a.is_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(y[k])) : __half_as_ushort(__float2half_rn(y[k]));
-        }
+        storeOut(a, p, task.seq * a.o_seq + (static_cast<long long>(kv) * a.group + head0 + h) * a.o_head + d, y);
     }
 }
 
@@ -829,8 +995,6 @@ Variant variantFor(const AttentionInfo &I) {
     return I.pools.bits == 4 ? variantFor<4>(I.head_size, group) : variantFor<8>(I.head_size, group);
 }
 
-constexpr int kMinRange = 8; // tiles
-
 } // namespace
 
 TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
@@ -839,10 +1003,12 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     const Pool &k = P.k, &v = P.v;
     const ptrdiff_t groups = static_cast<ptrdiff_t>(k.groups);
     auto whole = [](ptrdiff_t stride, ptrdiff_t unit) { return stride % unit == 0; };
-    // copies of 16 bytes: 8 tokens of a block at a time, their scales one run; K and V laid out alike
+    auto narrow = [](ptrdiff_t stride) { return stride >= 0 && stride <= 0x7fffffff; };
+    // copies of 16 bytes: 8 tokens of a block at a time, their scales one run; K and V laid out alike; strides of 32 bits
     plan.eligible = P.block_size % 8 == 0 && k.block == v.block && k.kv_head == v.kv_head && k.slot == v.slot && k.s_block == v.s_block
                  && k.s_head == v.s_head && k.s_slot == v.s_slot && k.s_slot == groups && whole(k.block, 16) && whole(k.kv_head, 16)
-                 && whole(k.slot, 16) && whole(k.s_block, 8) && whole(k.s_head, 8) && whole(I.q_seq, 8) && whole(I.q_head, 8);
+                 && whole(k.slot, 16) && whole(k.s_block, 8) && whole(k.s_head, 8) && whole(I.q_seq, 8) && whole(I.q_head, 8)
+                 && narrow(k.block) && narrow(k.slot) && narrow(k.slot * 8) && narrow(k.s_block);
     if (!plan.eligible || I.num_seqs == 0 || I.num_heads == 0 || I.max_blocks == 0) {
         plan.eligible = false;
         return plan;
@@ -852,30 +1018,35 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     const unsigned long long head_tiles = (group + var.heads - 1) / var.heads;
     const unsigned long long tiles = (static_cast<unsigned long long>(I.max_blocks) * P.block_size + kTile - 1) / kTile;
     const unsigned long long subs = head_tiles * P.num_kv_heads;
-    const long double line = static_cast<long double>(tiles) * subs * I.num_seqs;
-    if (tiles > 0x0fffffffull || line > 9e17L) {
+    const long double line = static_cast<long double>(tiles + kUnitCost) * subs * I.num_seqs;
+    const unsigned long long at_most = static_cast<unsigned long long>(props.sm_count) * var.ctas;
+    if (tiles > 0x0fffffffull || line > 9e17L || line / at_most > 1e9L) {
         plan.eligible = false; // positions would not fit
         return plan;
     }
-    const unsigned long long most = (static_cast<unsigned long long>(line) + kMinRange - 1) / kMinRange;
-    const unsigned long long ctas = static_cast<unsigned long long>(props.sm_count) * var.ctas;
-    plan.grid = static_cast<int>(most < ctas ? most : ctas);
-    if (static_cast<unsigned long long>(line) / plan.grid > 0x3fffffffull) {
-        plan.eligible = false;
-        return plan;
-    }
+    const unsigned long long useful = (static_cast<unsigned long long>(line) + kWarps * kMinRange - 1) / (kWarps * kMinRange);
+    plan.grid = static_cast<int>(useful < at_most ? useful : at_most);
     plan.head_tiles = static_cast<int>(head_tiles);
     plan.subs = static_cast<int>(subs);
     plan.tasks_bytes = (sizeof(Task) * plan.grid + 255) / 256 * 256;
     plan.workspace_bytes = plan.tasks_bytes + sizeof(float) * 2 * plan.grid * static_cast<size_t>(var.record);
+    // n / halves for n < 2^31 as mulhi(n, magic) >> shift: magic = floor(2^(32 + shift) / halves) + 1 with 2^shift < halves, which is
+    // below 2^32 and off by at most halves, and n * halves < 2^(32 + shift); 2^(31) and one shift less for a power of two
     const unsigned halves = static_cast<unsigned>(P.block_size / 8);
-    int l = 0;
-    while ((1u << l) < halves) {
-        ++l;
+    plan.half_self = halves == 1 ? 0xffffffffu : 0u;
+    if (halves > 1) {
+        while ((2u << plan.half_shift) <= halves) {
+            ++plan.half_shift;
+        }
+        if ((1u << plan.half_shift) == halves) {
+            plan.half_magic = 0x80000000u;
+            --plan.half_shift;
+        } else {
+            plan.half_magic = static_cast<unsigned>((1ull << (32 + plan.half_shift)) / halves + 1);
+        }
     }
-    // n / halves for n < 2^31 as (n * magic) >> (31 + l)
-    plan.half_magic = static_cast<unsigned>((1ull << (31 + l)) / halves + 1);
-    plan.half_shift = 31 + l;
+    auto words = [](ptrdiff_t stride) { return stride % 4 == 0; };
+    plan.out_words = words(I.o_seq) && words(I.o_head);
     return plan;
 }
 
@@ -891,9 +1062,12 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     p.tasks_bytes = static_cast<long long>(plan.tasks_bytes);
     p.subs = plan.subs;
     p.head_tiles = plan.head_tiles;
-    p.min_range = kMinRange;
     p.half_magic = plan.half_magic;
+    p.half_self = plan.half_self;
     p.half_shift = plan.half_shift;
+    p.index_shift = a.index_is_64 ? 3 : 2;
+    p.pages_of_16 = a.block_size % 16 == 0 ? 1 : 0;
+    p.out_words = plan.out_words && alignedTo(a.out, 8) ? 1 : 0;
     // an attribute of the current device's function, so it is set for each launch
     if (cudaFuncSetAttribute(var.tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem) != cudaSuccess) {
         return checkLaunch("quantAttentionTilesKernel: shared memory");
