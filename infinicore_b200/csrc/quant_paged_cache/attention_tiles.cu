@@ -53,6 +53,8 @@ struct Piece {
     int seq, sub, tiles, used;
 };
 
+constexpr int kWalkBytes = 24;
+
 template <int BITS, int HD, int HT>
 struct Cfg {
     static constexpr int kRowBytes = HD * BITS / 8;
@@ -62,7 +64,7 @@ struct Cfg {
     static constexpr int kHeadTiles = HT / 8;
     static constexpr int kStride = HD + 4;                    // floats: rows of two heads apart hit other banks
     static constexpr int kResult = HT * kStride * 4;
-    static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece))) + kThreads * 4 + 256;
+    static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes) + kThreads * 4 + 256;
     // resident CTAs: what the registers of q, outputs and scales leave room for
     static constexpr int kCtas = HD * HT <= 1024 ? 4 : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
@@ -89,19 +91,23 @@ __device__ __forceinline__ void waitCopies() {
 __device__ __forceinline__ void loadMatrices(unsigned (&r)[4], unsigned addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
+                 : "r"(addr));
 }
 __device__ __forceinline__ void loadMatricesTransposed(unsigned (&r)[4], unsigned addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
+                 : "r"(addr));
 }
 __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same onto zeros
+__device__ __forceinline__ void mmaFirst(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float exp2Fast(float x) {
     float r;
@@ -114,10 +120,16 @@ __device__ __forceinline__ unsigned packHalves(float lo, float hi) {
     return r;
 }
 // (x & mask) ^ magic
-template <unsigned MASK, unsigned MAGIC>
-__device__ __forceinline__ unsigned pick(unsigned x) {
+template <unsigned MASK>
+__device__ __forceinline__ unsigned pick(unsigned x, unsigned magic) {
     unsigned r;
-    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "n"(MASK), "n"(MAGIC));
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "n"(MASK), "r"(magic));
+    return r;
+}
+// A constant that stays in a register: an instruction takes one immediate, and a second one costs a move each time.
+__device__ __forceinline__ unsigned pinned(unsigned c) {
+    unsigned r;
+    asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(c));
     return r;
 }
 __device__ __forceinline__ unsigned addHalves(unsigned x, unsigned y) {
@@ -134,28 +146,34 @@ __device__ __forceinline__ unsigned fmaHalves(unsigned x, unsigned y, unsigned z
 constexpr unsigned kMinus1032 = 0xe408e408u; // fp16 pairs
 constexpr unsigned kMinus1152 = 0xe480e480u;
 constexpr unsigned kMinus72 = 0xd480d480u;
-constexpr unsigned kSixteenth = 0x2c002c00u;
+
+struct Magic { // fp16 pairs and bytes
+    unsigned low = pinned(0x64086408u);       // 1024 + 8
+    unsigned high = pinned(0x64806480u);      // 1024 + 128
+    unsigned sixteenth = pinned(0x2c002c00u);
+    unsigned byte = pinned(0x64646464u);
+};
 
 // 4-bit: a word of eight codes -> pairs (0,4), (1,5), (2,6), (3,7)
-__device__ __forceinline__ void codes4(unsigned w, unsigned (&b)[4]) {
+__device__ __forceinline__ void codes4(const Magic &m, unsigned w, unsigned (&b)[4]) {
     const unsigned h = w >> 8;
-    b[0] = addHalves(pick<0x000f000fu, 0x64086408u>(w), kMinus1032);              // 1024 + (c + 8) - 1032
-    b[1] = fmaHalves(pick<0x00f000f0u, 0x64806480u>(w), kSixteenth, kMinus72);    // (1024 + 16 (c + 8)) / 16 - 72
-    b[2] = addHalves(pick<0x000f000fu, 0x64086408u>(h), kMinus1032);
-    b[3] = fmaHalves(pick<0x00f000f0u, 0x64806480u>(h), kSixteenth, kMinus72);
+    b[0] = addHalves(pick<0x000f000fu>(w, m.low), kMinus1032);                 // 1024 + (c + 8) - 1032
+    b[1] = fmaHalves(pick<0x00f000f0u>(w, m.high), m.sixteenth, kMinus72);     // (1024 + 16 (c + 8)) / 16 - 72
+    b[2] = addHalves(pick<0x000f000fu>(h, m.low), kMinus1032);
+    b[3] = fmaHalves(pick<0x00f000f0u>(h, m.high), m.sixteenth, kMinus72);
 }
 // The same with the odd ones 16 times too large
-__device__ __forceinline__ void codes4Odd16(unsigned w, unsigned (&b)[4]) {
+__device__ __forceinline__ void codes4Odd16(const Magic &m, unsigned w, unsigned (&b)[4]) {
     const unsigned h = w >> 8;
-    b[0] = addHalves(pick<0x000f000fu, 0x64086408u>(w), kMinus1032);
-    b[1] = addHalves(pick<0x00f000f0u, 0x64806480u>(w), kMinus1152);
-    b[2] = addHalves(pick<0x000f000fu, 0x64086408u>(h), kMinus1032);
-    b[3] = addHalves(pick<0x00f000f0u, 0x64806480u>(h), kMinus1152);
+    b[0] = addHalves(pick<0x000f000fu>(w, m.low), kMinus1032);
+    b[1] = addHalves(pick<0x00f000f0u>(w, m.high), kMinus1152);
+    b[2] = addHalves(pick<0x000f000fu>(h, m.low), kMinus1032);
+    b[3] = addHalves(pick<0x00f000f0u>(h, m.high), kMinus1152);
 }
 // 8-bit: two of a word's codes, by byte selector
 template <unsigned SEL>
-__device__ __forceinline__ unsigned codes8(unsigned flipped) {
-    return addHalves(__byte_perm(flipped, 0x64646464u, SEL), kMinus1152);
+__device__ __forceinline__ unsigned codes8(const Magic &m, unsigned flipped) {
+    return addHalves(__byte_perm(flipped, m.byte, SEL), kMinus1152);
 }
 
 // ---- the line of tiles -------------------------------------------------------------------------------------
@@ -165,11 +183,11 @@ struct TilesArgs {
     long long tasks_bytes;
     int subs;                 // kv heads * head tiles of a group
     int head_tiles;
-    unsigned half_magic;      // division by block_size / 8
+    unsigned halves;          // block_size / 8
+    unsigned half_magic;      // division by that
     unsigned half_self;       // all ones where that is a division by 1
     int half_shift;
     int index_shift;          // log2 of the bytes of a table entry
-    int pages_of_16;          // block_size is a multiple of 16
     int out_words;            // rows of out can be stored 8 bytes at a time
 };
 
@@ -186,28 +204,31 @@ struct Lens { // lengths of the sequences a CTA meets first, in shared memory
 __device__ __forceinline__ int tilesOf(int len) { return len > 0 ? (len + kTile - 1) / kTile : 0; }
 __device__ __forceinline__ long long costOf(int len) { return len > 0 ? tilesOf(len) + kUnitCost : 0; }
 
-// A walk over the tiles of a warp's range.  `budget`: what is left of the range, the present tile included.
-struct Cursor {
-    int seq, sub, tile, tiles, len, budget;
+// Where a walk over a warp's range is: the unit, how much of the range lies behind what it takes of that unit.  Kept in
+// shared memory, read and written by all lanes alike: the loop over a unit's tiles has no use for it.
+struct Walk {
+    int seq, sub, tiles, len, budget, pad;
 
-    // To the next tile; true where that is in another unit.
-    __device__ __forceinline__ bool step(int subs, const Lens &lens) {
-        --budget;
-        if (++tile < tiles || budget <= 0) {
-            return false;
+    // To the next unit: how many of its tiles are in the range (0: the range has ended).
+    __device__ __forceinline__ int step(int subs, const Lens &lens) {
+        budget -= kUnitCost; // at or below 0: the range ends in front of the unit's first tile
+        if (budget <= 0) {
+            return 0;
         }
-        tile = 0;
-        budget -= kUnitCost; // behind 0: the range ends in front of the next unit's first tile
-        if (budget > 0 && ++sub == subs) {
+        if (++sub == subs) {
             sub = 0;
             do {
                 len = lens(++seq);
             } while (len <= 0);
             tiles = tilesOf(len);
         }
-        return true;
+        const int n = min(tiles, budget);
+        budget -= n;
+        return n;
     }
 };
+
+static_assert(sizeof(Walk) == kWalkBytes);
 
 // ---- kernel ------------------------------------------------------------------------------------------------
 
@@ -238,7 +259,8 @@ __device__ __forceinline__ void storeOut(const AttentionArgs &a, const TilesArgs
     }
 }
 
-template <int BITS, int HD, int HT>
+// P16: blocks are multiples of 16 tokens, so a tile lies in one; otherwise of 8, and a half of a tile does.
+template <int BITS, int HD, int HT, bool P16>
 __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAttentionTilesKernel(const AttentionArgs a, const TilesArgs p) {
     using C = Cfg<BITS, HD, HT>;
     constexpr int NG = C::kGroups, NH = C::kHeadTiles, CPR = C::kChunks, S = C::kStages;
@@ -246,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     float *results = reinterpret_cast<float *>(smem + kWarps * C::kRing);                                     // [warp][head][kStride]
     float2 *sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(results) + kWarps * C::kResult); // [warp][2][head]
     Piece *pieces = reinterpret_cast<Piece *>(sums + kWarps * 2 * HT);                                        // [warp][2]
-    int *lens_s = reinterpret_cast<int *>(pieces + kWarps * 2);
+    Walk *walks = reinterpret_cast<Walk *>(pieces + kWarps * 2);                                              // [warp][copies | arithmetic]
+    int *lens_s = reinterpret_cast<int *>(walks + kWarps * 2);
     long long *plan_s = reinterpret_cast<long long *>(lens_s + kThreads); // sums of warps; then seq and position of each start
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -324,33 +347,43 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 
     unsigned char *ring = smem + warp * C::kRing;
     if (start < total) {
-        Cursor cur;
+        const Magic magic;
+        Walk &copies = walks[2 * warp], &work = walks[2 * warp + 1];
+        int tile, left;  // of the unit in work: present tile, tiles from there on in the range
         long long place; // of the present tile on the line
         {
-            cur.seq = static_cast<int>(plan_s[4 + 2 * warp]);
-            cur.len = lens(cur.seq);
-            cur.tiles = tilesOf(cur.len);
-            const long long pos = plan_s[5 + 2 * warp], cost = cur.tiles + kUnitCost;
-            cur.sub = static_cast<int>(pos / cost);
-            const int in = static_cast<int>(pos - cur.sub * cost) - kUnitCost; // below 0: in front of the unit's first tile
-            cur.tile = in > 0 ? in : 0;
-            place = start + (cur.tile - in);
-            cur.budget = static_cast<int>(end - place);
+            Walk w;
+            w.seq = static_cast<int>(plan_s[4 + 2 * warp]);
+            w.len = lens(w.seq);
+            w.tiles = tilesOf(w.len);
+            const long long pos = plan_s[5 + 2 * warp], cost = w.tiles + kUnitCost;
+            w.sub = static_cast<int>(pos / cost);
+            const int in = static_cast<int>(pos - w.sub * cost) - kUnitCost; // below 0: in front of the unit's first tile
+            tile = in > 0 ? in : 0;
+            place = start + (tile - in);
+            const int budget = static_cast<int>(end - place);
+            left = min(w.tiles - tile, budget);
+            w.budget = budget - left;
+            copies = work = w;
+            __syncwarp();
         }
 
-        // ---- copies: the tile after those in flight, its blocks already looked up
-        Cursor next = cur;
+        // ---- copies: the next tile's block is already looked up
+        unsigned f_half = 2u * static_cast<unsigned>(tile); // first half (8 tokens) of the next tile, within its unit
+        int f_left = left;
         const unsigned char *table_row = nullptr;
-        long long code_unit = 0, scale_unit = 0; // offsets of the kv head
-        unsigned block0 = 0, block1 = 0;
-        int half0 = 0, half1 = 0; // first slots of the tile's halves within their blocks
-        const unsigned code_block = static_cast<unsigned>(a.k_block), scale_block = static_cast<unsigned>(a.ks_block);
-        const unsigned code_slot = static_cast<unsigned>(a.k_slot);
+        // this lane's first 16 bytes of K and V codes and of scales in block 0 of the unit's kv head
+        const unsigned char *k_lane = nullptr, *v_lane = nullptr, *s_lane = nullptr;
+        unsigned block0 = 0, block1 = 0, slot0 = 0, slot1 = 0; // blocks of the halves, their first slots there
+        const unsigned code_block = static_cast<unsigned>(a.k_block), code_slot = static_cast<unsigned>(a.k_slot);
+        const unsigned scale_block = 2u * static_cast<unsigned>(a.ks_block);
         auto unit = [&]() {
-            const int kv = next.sub / p.head_tiles;
-            table_row = static_cast<const unsigned char *>(a.block_tables) + ((next.seq * a.table_seq) << p.index_shift);
-            code_unit = kv * a.k_head;
-            scale_unit = kv * a.ks_head;
+            const int kv = copies.sub / p.head_tiles;
+            table_row = static_cast<const unsigned char *>(a.block_tables) + ((copies.seq * a.table_seq) << p.index_shift);
+            k_lane = a.k_codes + kv * a.k_head;
+            v_lane = a.v_codes + kv * a.k_head;
+            const bool v = lane >= 2 * NG;
+            s_lane = reinterpret_cast<const unsigned char *>((v ? a.v_scales : a.k_scales) + kv * a.ks_head) + (lane % NG) * 16;
         };
         auto entry = [&](unsigned page) { // the low word of a 64-bit entry says all that a block in the pool can be
             const unsigned char *at = table_row + (static_cast<unsigned long long>(page) << p.index_shift);
@@ -365,51 +398,55 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             return b;
         };
         auto look = [&]() {
-            const unsigned h0 = 2u * static_cast<unsigned>(next.tile), halves = static_cast<unsigned>(a.block_size) >> 3;
-            const unsigned page = (__umulhi(h0, p.half_magic) + (h0 & p.half_self)) >> p.half_shift;
-            half0 = 8 * static_cast<int>(h0 - page * halves);
+            const unsigned page = (__umulhi(f_half, p.half_magic) + (f_half & p.half_self)) >> p.half_shift;
+            slot0 = 8u * (f_half - page * p.halves);
             block0 = entry(page);
-            half1 = half0 + 8;
-            block1 = block0;
-            if (!p.pages_of_16 && half1 == a.block_size) {
-                // the second half is the next block's; behind the sequence's end it is read where the first is
-                if (8 * static_cast<int>(h0 + 1) < next.len) {
-                    block1 = entry(page + 1);
-                    half1 = 0;
-                } else {
-                    half1 = half0;
+            if constexpr (!P16) {
+                block1 = block0;
+                slot1 = slot0 + 8u;
+                if (slot1 == static_cast<unsigned>(a.block_size)) {
+                    // the second half is the next block's; behind the sequence's end it is read where the first is
+                    if (8 * static_cast<int>(f_half + 1) < copies.len) {
+                        block1 = entry(page + 1);
+                        slot1 = 0;
+                    } else {
+                        slot1 = slot0;
+                    }
                 }
             }
         };
-        auto fetch = [&](int slot) {
-            if (next.budget > 0) {
-                const unsigned dst = smemAddr(ring + slot * C::kStage);
-                const long long c0 = code_unit + static_cast<unsigned long long>(block0) * code_block + static_cast<unsigned long long>(half0) * code_slot;
-                const long long c1 = p.pages_of_16 ? c0 + 8ull * code_slot
-                                                   : code_unit + static_cast<unsigned long long>(block1) * code_block
-                                                         + static_cast<unsigned long long>(half1) * code_slot;
+        auto fetch = [&](unsigned dst) { // the next tile into a slot of the ring
+            if (f_left > 0) {
+                const unsigned long long c0 = static_cast<unsigned long long>(block0) * code_block + static_cast<unsigned long long>(slot0) * code_slot;
+                const unsigned long long c1 = P16 ? c0 + 8ull * code_slot
+                                                  : static_cast<unsigned long long>(block1) * code_block + static_cast<unsigned long long>(slot1) * code_slot;
 #pragma unroll
                 for (int j = 0; j < CPR / 2; ++j) {
                     const int i = lane + 32 * j, r = i / CPR, c = i % CPR;
                     const int swz = CPR % 8 == 0 ? (r & 7) : CPR % 4 == 0 ? ((r >> 1) & 3) : ((r >> 2) & 1);
                     const unsigned to = dst + r * C::kRowBytes + ((c ^ swz) << 4);
-                    const long long from = (r < 8 ? c0 : c1) + (static_cast<unsigned>(r & 7) * code_slot + c * 16);
-                    copy16(to, a.k_codes + from);
-                    copy16(to + kTile * C::kRowBytes, a.v_codes + from);
+                    const unsigned in = static_cast<unsigned>(r & 7) * code_slot + c * 16;
+                    const unsigned long long from = (r < 8 ? c0 : c1) + in;
+                    copy16(to, k_lane + from);
+                    copy16(to + kTile * C::kRowBytes, v_lane + from);
                 }
                 // scales: a half's 8 rows are one run of NG chunks
                 if (lane < 4 * NG) {
-                    const bool v = lane >= 2 * NG;
-                    const int i = v ? lane - 2 * NG : lane;
-                    const bool h = i >= NG;
-                    const long long from = scale_unit + static_cast<unsigned long long>(h ? block1 : block0) * scale_block
-                                         + ((h ? half1 : half0) * NG + (h ? i - NG : i) * 8);
-                    copy16(dst + 2 * kTile * C::kRowBytes + lane * 16, (v ? a.v_scales : a.k_scales) + from);
+                    const bool h = (lane / NG) & 1;
+                    const unsigned b = P16 || !h ? block0 : block1, at = h ? (P16 ? slot0 + 8u : slot1) : slot0;
+                    copy16(dst + 2 * kTile * C::kRowBytes + lane * 16, s_lane + static_cast<unsigned long long>(b) * scale_block + at * (2u * NG));
                 }
-                if (next.step(p.subs, lens)) {
+                f_half += 2u;
+                if (--f_left == 0) {
+                    Walk w = copies;
+                    f_left = w.step(p.subs, lens);
+                    __syncwarp();
+                    copies = w;
+                    __syncwarp();
+                    f_half = 0;
                     unit();
                 }
-                if (next.budget > 0) {
+                if (f_left > 0) {
                     look();
                 }
             }
@@ -417,23 +454,23 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         };
         unit();
         look();
+        const unsigned ring_addr = smemAddr(ring);
 #pragma unroll
         for (int i = 0; i < S - 1; ++i) {
-            fetch(i);
+            fetch(ring_addr + i * C::kStage);
         }
-        int slot = 0;
+        unsigned stage = ring_addr, spare = ring_addr + (S - 1) * C::kStage; // the tile to work on, the slot to fill
 
         // lane's part of the matrix loads: matrix lane / 8, row lane % 8; matrices are (tokens 0-7 | 8-15) x (chunk, chunk + 1)
         const int m_row = (lane & 7) + ((lane >> 3) & 1) * 8, m_chunk = lane >> 4;
         const int m_swz = CPR % 8 == 0 ? (m_row & 7) : CPR % 4 == 0 ? ((m_row >> 1) & 3) : ((m_row >> 2) & 1);
 
-        while (cur.budget > 0) { // a unit, or what of it is in the range
-            const int kv = cur.sub / p.head_tiles;
-            const int head0 = (cur.sub - kv * p.head_tiles) * HT; // within the group
+        while (left > 0) { // a unit, or what of it is in the range
+            const int kv = work.sub / p.head_tiles;
+            const int head0 = (work.sub - kv * p.head_tiles) * HT; // within the group
             const int heads = min(HT, a.group - head0);
             const long long head_at = static_cast<long long>(kv) * a.group + head0;
-            const long long unit_first = place - cur.tile;
-            const int unit_seq = cur.seq, unit_sub = cur.sub, unit_tiles = cur.tiles, len = cur.len;
+            const int len = work.len;
 
             // q as first operand, scaled by a power of two for each head; the scores' factor takes it back
             unsigned qr[NH][HD / 16][2]; // [.][k step][a0 | a2]
@@ -443,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 const int h = g + 8 * n;
                 unsigned raw[HD / 16][2];
                 unsigned largest = 0;
-                const unsigned short *q = static_cast<const unsigned short *>(a.q) + cur.seq * a.q_seq + (head_at + h) * a.q_head;
+                const unsigned short *q = static_cast<const unsigned short *>(a.q) + work.seq * a.q_seq + (head_at + h) * a.q_head;
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) { // 4 bits: 8 elements from 32 j + 8 t; 8 bits: 4 from 32 j + 4 t and 4 from + 16
                     uint4 x = make_uint4(0, 0, 0, 0);
@@ -511,21 +548,20 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 }
             }
 
-            bool more;
-            int token0 = cur.tile * kTile;
+            int token0 = tile * kTile;
+            // from this token on a tile needs more than the plain arithmetic: a distance bias, tokens behind the end
+            const int special = a.alibi != nullptr ? 0 : len - kTile + 1;
             do {
                 waitCopies<S - 2>();
                 __syncwarp();
-                const unsigned char *stage = ring + slot * C::kStage;
-                fetch(slot == 0 ? S - 1 : slot - 1);
-                slot = slot == S - 1 ? 0 : slot + 1;
-                const unsigned k_addr = smemAddr(stage) + m_row * C::kRowBytes, v_addr = k_addr + kTile * C::kRowBytes;
+                fetch(spare);
+                const unsigned k_addr = stage + m_row * C::kRowBytes, v_addr = k_addr + kTile * C::kRowBytes;
 
                 // scales of the lane's tokens 2t, 2t + 1 (pair 0) and 2t + 8, 2t + 9 (pair 1): words [pair][token][group / 2]
                 constexpr int kWords = NG; // of a pair
                 unsigned ks[2][kWords], vs[2][kWords];
                 {
-                    const unsigned char *sc = stage + 2 * kTile * C::kRowBytes;
+                    const unsigned char *sc = ring + (stage - ring_addr) + 2 * kTile * C::kRowBytes;
 #pragma unroll
                     for (int pair = 0; pair < 2; ++pair) {
                         const unsigned *kp = reinterpret_cast<const unsigned *>(sc) + (pair * 4 + t) * kWords;
@@ -583,9 +619,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                                 const unsigned word = w[2 * x + pair];
                                 if constexpr (BITS == 4) {
                                     unsigned b[4];
-                                    codes4(word, b);
-                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                                    mma(d, qr[0][2 * j][0], NH == 2 ? qr[NH - 1][2 * j][0] : 0u, qr[0][2 * j][1], NH == 2 ? qr[NH - 1][2 * j][1] : 0u,
+                                    codes4(magic, word, b);
+                                    float d[4];
+                                    mmaFirst(d, qr[0][2 * j][0], NH == 2 ? qr[NH - 1][2 * j][0] : 0u, qr[0][2 * j][1], NH == 2 ? qr[NH - 1][2 * j][1] : 0u,
                                         b[0], b[1]);
                                     mma(d, qr[0][2 * j + 1][0], NH == 2 ? qr[NH - 1][2 * j + 1][0] : 0u, qr[0][2 * j + 1][1],
                                         NH == 2 ? qr[NH - 1][2 * j + 1][1] : 0u, b[2], b[3]);
@@ -598,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                                 } else {
                                     const unsigned f = word ^ 0x80808080u;
                                     mma(acc[pair], qr[0][j][0], NH == 2 ? qr[NH - 1][j][0] : 0u, qr[0][j][1], NH == 2 ? qr[NH - 1][j][1] : 0u,
-                                        codes8<0x4140>(f), codes8<0x4342>(f));
+                                        codes8<0x4140>(magic, f), codes8<0x4342>(magic, f));
                                 }
                             }
                         }
@@ -616,21 +652,15 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         }
                     }
                 }
-                if (a.alibi != nullptr) {
+                if (token0 >= special) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float far = static_cast<float>(token0 + 8 * (i >> 1) + 2 * t + (i & 1) - (len - 1));
+                        const int pair = i >> 1, x = i & 1, token = token0 + 8 * pair + 2 * t + x;
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
-                            s[i >> 1][n][i & 1] += slope[n] * far;
+                            s[pair][n][x] += slope[n] * static_cast<float>(token - (len - 1));
                         }
-                    }
-                }
-                if (token0 + kTile > len) { // tokens behind the end have no weight, whatever their scales are
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int pair = i >> 1, x = i & 1;
-                        if (token0 + 8 * pair + 2 * t + x >= len) {
+                        if (token >= len) { // no weight, whatever the scales are
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
                                 s[pair][n][x] = -INFINITY;
@@ -770,8 +800,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         }
                         if constexpr (BITS == 4) {
                             unsigned lo[4], hi[4];
-                            codes4Odd16(w[2 * x], lo);
-                            codes4Odd16(w[2 * x + 1], hi);
+                            codes4Odd16(magic, w[2 * x], lo);
+                            codes4Odd16(magic, w[2 * x + 1], hi);
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
                                 mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], weight[n][0], weight[n][1]);
@@ -779,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                             }
                         } else {
                             const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
-                            const unsigned a0 = codes8<0x4240>(lo), a1 = codes8<0x4341>(lo), a2 = codes8<0x4240>(hi), a3 = codes8<0x4341>(hi);
+                            const unsigned a0 = codes8<0x4240>(magic, lo), a1 = codes8<0x4341>(magic, lo), a2 = codes8<0x4240>(magic, hi), a3 = codes8<0x4341>(magic, hi);
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
                                 mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
@@ -788,13 +818,22 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     }
                 }
                 token0 += kTile;
-                ++place;
-                more = !cur.step(p.subs, lens) && cur.budget > 0;
-            } while (more);
+                spare = stage;
+                stage = stage == ring_addr + (S - 1) * C::kStage ? ring_addr : stage + C::kStage;
+            } while (--left > 0);
 
             // the unit's rows, or this warp's piece of it
-            const bool first = unit_first >= start, last = unit_first + unit_tiles <= end;
-            place = unit_first + unit_tiles + kUnitCost; // if the range goes on, it does with the next unit
+            const Walk done = work;
+            const long long unit_first = place - tile;
+            const bool first = unit_first >= start, last = unit_first + done.tiles <= end;
+            {
+                Walk w = done;
+                left = last ? w.step(p.subs, lens) : 0;
+                __syncwarp();
+                work = w;
+            }
+            place = unit_first + done.tiles + kUnitCost; // if the range goes on, it does with the next unit
+            tile = 0;
             float inv[NH];
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
@@ -803,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 inv[n] = 1.f / sum[n];
             }
             if (!(first && last) && lane == 0) {
-                pieces[2 * warp + first] = {unit_first, unit_seq, unit_sub, unit_tiles, 1};
+                pieces[2 * warp + first] = {unit_first, done.seq, done.sub, done.tiles, 1};
             }
             // a piece in front is kept beside the ring, one at the range's end in the ring, which is empty then
             float *mine_o = first ? reinterpret_cast<float *>(ring) : results + warp * HT * C::kStride;
@@ -814,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 constexpr int kRuns = HD / (8 * kPer);
                 if (first && last) {
                     const float inv0 = __shfl_sync(0xffffffffu, inv[n], 8 * t), inv1 = __shfl_sync(0xffffffffu, inv[n], 8 * t + 4);
-                    const long long row = unit_seq * a.o_seq + (head_at + 8 * n + 2 * t) * a.o_head;
+                    const long long row = done.seq * a.o_seq + (head_at + 8 * n + 2 * t) * a.o_head;
 #pragma unroll
                     for (int j = 0; j < kRuns; ++j) {
 #pragma unroll
@@ -964,14 +1003,14 @@ __global__ void __launch_bounds__(256) quantAttentionCombineKernel(const Attenti
 using TilesKernel = void (*)(AttentionArgs, TilesArgs);
 
 struct Variant {
-    TilesKernel tiles, combine;
+    TilesKernel tiles[2], combine; // blocks of 8 | 16 tokens
     int ctas, smem, record, heads;
 };
 
 template <int BITS, int HD, int HT>
 Variant variant() {
     using C = Cfg<BITS, HD, HT>;
-    return {quantAttentionTilesKernel<BITS, HD, HT>, quantAttentionCombineKernel<HD, HT>, C::kCtas, C::kSmem, C::kRecord, HT};
+    return {{quantAttentionTilesKernel<BITS, HD, HT, false>, quantAttentionTilesKernel<BITS, HD, HT, true>}, quantAttentionCombineKernel<HD, HT>, C::kCtas, C::kSmem, C::kRecord, HT};
 }
 
 template <int BITS>
@@ -1066,10 +1105,11 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     p.half_self = plan.half_self;
     p.half_shift = plan.half_shift;
     p.index_shift = a.index_is_64 ? 3 : 2;
-    p.pages_of_16 = a.block_size % 16 == 0 ? 1 : 0;
+    p.halves = static_cast<unsigned>(a.block_size / 8);
     p.out_words = plan.out_words && alignedTo(a.out, 8) ? 1 : 0;
     // an attribute of the current device's function, so it is set for each launch
-    if (cudaFuncSetAttribute(var.tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem) != cudaSuccess) {
+    const TilesKernel kernel = var.tiles[a.block_size % 16 == 0];
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem) != cudaSuccess) {
         return checkLaunch("quantAttentionTilesKernel: shared memory");
     }
     cudaLaunchAttribute pdl;
@@ -1082,7 +1122,7 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     cfg.stream = stream;
     cfg.attrs = &pdl;
     cfg.numAttrs = 1;
-    (void)cudaLaunchKernelEx(&cfg, var.tiles, a, p);
+    (void)cudaLaunchKernelEx(&cfg, kernel, a, p);
     const infiniStatus_t st = checkLaunch("quantAttentionTilesKernel");
     B200_RETURN_IF(st != INFINI_STATUS_SUCCESS, st);
     cfg.blockDim = dim3(256);
