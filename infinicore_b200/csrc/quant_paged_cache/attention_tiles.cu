@@ -14,12 +14,12 @@
 //
 // Arithmetic.  Codes become fp16 exactly by bit operations (1024 + u has u in its low mantissa bits) and one
 // addition; the scales never touch them:
-//   S[head, token] = sum_g k_scale[token, g] * (Q . codes)_g    a 32-element group is two matrix instructions
+//   S[token, head] = sum_g k_scale[token, g] * (codes . Q)_g    a 32-element group is two matrix instructions
 //   w[token, g]    = p[token] * v_scale[token, g]               the weights carry the V scales
 //   O[dim, head]   = sum_token codes[token, dim] * w[token, g]
-// so the scores' layout in registers (heads by rows, tokens by columns) is the one that the weights need as second
-// operand, and V^T comes out of a transposing load.  In the 4-bit form every fourth pair of elements keeps a
-// factor of 16 that its output columns are rid of at the end.
+// The codes are the first operand both times (all 16 of its rows are used whatever the number of heads): K by rows, V
+// through a transposing load.  The weights are transposed in registers, 8 tokens by 8 heads at a time.  In the 4-bit form
+// every second element of V keeps a factor of 16 that its output is rid of at the end.
 //   q is held in fp16 times a power of two that makes its largest element 1/2..1: exact for every element above
 // 2^-13 of that (fp16 and bf16 both have at most 11 bits).
 //   w is rounded once to fp16.  To keep it in range for scales of any size the running maximum is taken over
@@ -108,6 +108,11 @@ __device__ __forceinline__ void mmaFirst(float (&d)[4], unsigned a0, unsigned a1
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ unsigned transposed(unsigned x) {
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 __device__ __forceinline__ float exp2Fast(float x) {
     float r;
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     Walk *walks = reinterpret_cast<Walk *>(pieces + kWarps * 2);                                              // [warp][copies | arithmetic]
     int *lens_s = reinterpret_cast<int *>(walks + kWarps * 2);
     long long *plan_s = reinterpret_cast<long long *>(lens_s + kThreads); // sums of warps; then seq and position of each start
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = static_cast<int>(pinned(threadIdx.x)), warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -472,9 +477,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             const long long head_at = static_cast<long long>(kv) * a.group + head0;
             const int len = work.len;
 
-            // q as first operand, scaled by a power of two for each head; the scores' factor takes it back
-            unsigned qr[NH][HD / 16][2]; // [.][k step][a0 | a2]
-            float factor[NH], slope[NH];
+            // q, scaled by a power of two for each head; the scores' factor takes it back
+            unsigned qr[NH][HD / 16][2];             // of head g: second operand, [.][k step][.]
+            float factor[NH][2], slope[NH][2];       // of the scores' columns, heads 2t and 2t + 1
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
                 const int h = g + 8 * n;
@@ -509,8 +514,13 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 const int e = static_cast<int>(__float_as_uint(wide(largest)) >> 23); // biased
                 const int down = max(253 - e, 1);                                     // 2^(126 - e)
                 const float scale_q = __uint_as_float(static_cast<unsigned>(down) << 23);
-                factor[n] = a.scale_log2e * __uint_as_float(static_cast<unsigned>(254 - down) << 23);
-                slope[n] = a.alibi != nullptr && h < heads ? a.alibi[head_at + h] * 1.4426950408889634f : 0.f;
+                const float back = a.scale_log2e * __uint_as_float(static_cast<unsigned>(254 - down) << 23);
+                const float bias = a.alibi != nullptr && h < heads ? a.alibi[head_at + h] * 1.4426950408889634f : 0.f;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    factor[n][x] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * x);
+                    slope[n][x] = __shfl_sync(0xffffffffu, bias, 8 * t + 4 * x);
+                }
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
                     float x[8];
@@ -534,11 +544,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 }
             }
 
-            float top[NH], sum[NH], o[NH][HD / 16][4];
+            float top[NH][2], sum[NH][2], o[NH][HD / 16][4];
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
-                top[n] = kLowest;
-                sum[n] = 0.f;
+                top[n][0] = top[n][1] = kLowest;
+                sum[n][0] = sum[n][1] = 0.f;
 #pragma unroll
                 for (int j = 0; j < HD / 16; ++j) {
 #pragma unroll
@@ -557,121 +567,108 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 fetch(spare);
                 const unsigned k_addr = stage + m_row * C::kRowBytes, v_addr = k_addr + kTile * C::kRowBytes;
 
-                // scales of the lane's tokens 2t, 2t + 1 (pair 0) and 2t + 8, 2t + 9 (pair 1): words [pair][token][group / 2]
-                constexpr int kWords = NG; // of a pair
+                // scales of the lane's tokens g and g + 8, two groups a word (one scale: the low half)
+                constexpr int kWords = NG == 1 ? 1 : NG / 2;
                 unsigned ks[2][kWords], vs[2][kWords];
                 {
-                    const unsigned char *sc = ring + (stage - ring_addr) + 2 * kTile * C::kRowBytes;
+                    const unsigned char *sc = ring + (stage - ring_addr) + 2 * kTile * C::kRowBytes + g * (2 * NG);
 #pragma unroll
-                    for (int pair = 0; pair < 2; ++pair) {
-                        const unsigned *kp = reinterpret_cast<const unsigned *>(sc) + (pair * 4 + t) * kWords;
-                        const unsigned *vp = kp + kTile * NG / 2;
-                        if constexpr (kWords % 4 == 0) {
-#pragma unroll
-                            for (int i = 0; i < kWords / 4; ++i) {
-                                const uint4 x = reinterpret_cast<const uint4 *>(kp)[i], y = reinterpret_cast<const uint4 *>(vp)[i];
-                                ks[pair][4 * i] = x.x, ks[pair][4 * i + 1] = x.y, ks[pair][4 * i + 2] = x.z, ks[pair][4 * i + 3] = x.w;
-                                vs[pair][4 * i] = y.x, vs[pair][4 * i + 1] = y.y, vs[pair][4 * i + 2] = y.z, vs[pair][4 * i + 3] = y.w;
-                            }
-                        } else if constexpr (kWords % 2 == 0) {
-#pragma unroll
-                            for (int i = 0; i < kWords / 2; ++i) {
-                                const uint2 x = reinterpret_cast<const uint2 *>(kp)[i], y = reinterpret_cast<const uint2 *>(vp)[i];
-                                ks[pair][2 * i] = x.x, ks[pair][2 * i + 1] = x.y;
-                                vs[pair][2 * i] = y.x, vs[pair][2 * i + 1] = y.y;
-                            }
+                    for (int r = 0; r < 2; ++r) {
+                        const unsigned char *kp = sc + r * (16 * NG), *vp = kp + 32 * NG;
+                        if constexpr (NG == 1) {
+                            ks[r][0] = *reinterpret_cast<const unsigned short *>(kp);
+                            vs[r][0] = *reinterpret_cast<const unsigned short *>(vp);
+                        } else if constexpr (kWords % 4 == 0) {
+                            const uint4 x = *reinterpret_cast<const uint4 *>(kp), y = *reinterpret_cast<const uint4 *>(vp);
+                            ks[r][0] = x.x, ks[r][1] = x.y, ks[r][2] = x.z, ks[r][3] = x.w;
+                            vs[r][0] = y.x, vs[r][1] = y.y, vs[r][2] = y.z, vs[r][3] = y.w;
+                        } else if constexpr (kWords == 2) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(kp), y = *reinterpret_cast<const uint2 *>(vp);
+                            ks[r][0] = x.x, ks[r][1] = x.y;
+                            vs[r][0] = y.x, vs[r][1] = y.y;
                         } else {
-                            ks[pair][0] = kp[0];
-                            vs[pair][0] = vp[0];
+#pragma unroll
+                            for (int i = 0; i < kWords; ++i) {
+                                ks[r][i] = reinterpret_cast<const unsigned *>(kp)[i];
+                                vs[r][i] = reinterpret_cast<const unsigned *>(vp)[i];
+                            }
                         }
                     }
                 }
-                // scale of token x (0, 1) of a pair and group j: NG == 1 keeps both tokens in one word
-                auto scaleAt = [](const unsigned (&w)[kWords], int x, int j) {
-                    const unsigned word = NG == 1 ? w[0] : w[x * (NG / 2) + j / 2];
-                    return __uint_as_float((NG == 1 ? x : j & 1) ? word & 0xffff0000u : word << 16);
+                auto scaleAt = [](const unsigned (&w)[kWords], int j) {
+                    return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
                 };
 
                 // scores
-                float s[2][NH][2]; // [pair][head tile][token]
-                {
-                    float acc[2][4];
+                float s[NH][4]; // [.][tokens g, heads 2t and 2t + 1 | tokens g + 8]
 #pragma unroll
-                    for (int pair = 0; pair < 2; ++pair) {
+                for (int n = 0; n < NH; ++n) {
 #pragma unroll
-                        for (int n = 0; n < NH; ++n) {
-                            s[pair][n][0] = s[pair][n][1] = 0.f;
+                    for (int i = 0; i < 4; ++i) {
+                        s[n][i] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < CPR; c += 2) {
+                    unsigned w[4];
+                    loadMatrices(w, k_addr + (((c + m_chunk) ^ m_swz) << 4));
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) { // the two chunks
+                        const int j = c + x;
+                        if constexpr (BITS == 4) {
+                            unsigned lo[4], hi[4];
+                            codes4(magic, w[2 * x], lo);
+                            codes4(magic, w[2 * x + 1], hi);
+                            const float s0 = scaleAt(ks[0], j), s1 = scaleAt(ks[1], j);
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                float d[4];
+                                mmaFirst(d, lo[0], hi[0], lo[1], hi[1], qr[n][2 * j][0], qr[n][2 * j][1]);
+                                mma(d, lo[2], hi[2], lo[3], hi[3], qr[n][2 * j + 1][0], qr[n][2 * j + 1][1]);
+                                s[n][0] = fmaf(s0, d[0], s[n][0]);
+                                s[n][1] = fmaf(s0, d[1], s[n][1]);
+                                s[n][2] = fmaf(s1, d[2], s[n][2]);
+                                s[n][3] = fmaf(s1, d[3], s[n][3]);
+                            }
+                        } else {
+                            const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
+                            const unsigned a0 = codes8<0x4140>(magic, lo), a1 = codes8<0x4140>(magic, hi);
+                            const unsigned a2 = codes8<0x4342>(magic, lo), a3 = codes8<0x4342>(magic, hi);
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                mma(s[n], a0, a1, a2, a3, qr[n][j][0], qr[n][j][1]);
+                            }
                         }
+                    }
+                }
+                {
+                    const float s0 = BITS == 8 ? scaleAt(ks[0], 0) : 1.f, s1 = BITS == 8 ? scaleAt(ks[1], 0) : 1.f;
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            acc[pair][i] = 0.f;
-                        }
-                    }
-#pragma unroll
-                    for (int c = 0; c < CPR; c += 2) {
-                        unsigned w[4];
-                        loadMatrices(w, k_addr + (((c + m_chunk) ^ m_swz) << 4));
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) { // the two chunks
-                            const int j = c + x;
-#pragma unroll
-                            for (int pair = 0; pair < 2; ++pair) {
-                                const unsigned word = w[2 * x + pair];
-                                if constexpr (BITS == 4) {
-                                    unsigned b[4];
-                                    codes4(magic, word, b);
-                                    float d[4];
-                                    mmaFirst(d, qr[0][2 * j][0], NH == 2 ? qr[NH - 1][2 * j][0] : 0u, qr[0][2 * j][1], NH == 2 ? qr[NH - 1][2 * j][1] : 0u,
-                                        b[0], b[1]);
-                                    mma(d, qr[0][2 * j + 1][0], NH == 2 ? qr[NH - 1][2 * j + 1][0] : 0u, qr[0][2 * j + 1][1],
-                                        NH == 2 ? qr[NH - 1][2 * j + 1][1] : 0u, b[2], b[3]);
-                                    const float s0 = scaleAt(ks[pair], 0, j), s1 = scaleAt(ks[pair], 1, j);
-#pragma unroll
-                                    for (int n = 0; n < NH; ++n) {
-                                        s[pair][n][0] = fmaf(s0, d[2 * n], s[pair][n][0]);
-                                        s[pair][n][1] = fmaf(s1, d[2 * n + 1], s[pair][n][1]);
-                                    }
-                                } else {
-                                    const unsigned f = word ^ 0x80808080u;
-                                    mma(acc[pair], qr[0][j][0], NH == 2 ? qr[NH - 1][j][0] : 0u, qr[0][j][1], NH == 2 ? qr[NH - 1][j][1] : 0u,
-                                        codes8<0x4140>(magic, f), codes8<0x4342>(magic, f));
-                                }
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int pair = 0; pair < 2; ++pair) {
-#pragma unroll
-                        for (int n = 0; n < NH; ++n) {
-                            if constexpr (BITS == 8) {
-                                s[pair][n][0] = acc[pair][2 * n] * scaleAt(ks[pair], 0, 0);
-                                s[pair][n][1] = acc[pair][2 * n + 1] * scaleAt(ks[pair], 1, 0);
-                            }
-                            s[pair][n][0] *= factor[n];
-                            s[pair][n][1] *= factor[n];
+                            s[n][i] *= BITS == 8 ? factor[n][i & 1] * (i < 2 ? s0 : s1) : factor[n][i & 1];
                         }
                     }
                 }
                 if (token0 >= special) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int pair = i >> 1, x = i & 1, token = token0 + 8 * pair + 2 * t + x;
+                    for (int r = 0; r < 2; ++r) {
+                        const int token = token0 + 8 * r + g;
+                        const float far = static_cast<float>(token - (len - 1));
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
-                            s[pair][n][x] += slope[n] * static_cast<float>(token - (len - 1));
+                            s[n][2 * r] += slope[n][0] * far;
+                            s[n][2 * r + 1] += slope[n][1] * far;
                         }
                         if (token >= len) { // no weight, whatever the scales are
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
-                                s[pair][n][x] = -INFINITY;
+                                s[n][2 * r] = s[n][2 * r + 1] = -INFINITY;
                             }
-                            if constexpr (NG == 1) {
-                                vs[pair][0] &= x ? 0x0000ffffu : 0xffff0000u;
-                            } else {
 #pragma unroll
-                                for (int k = 0; k < NG / 2; ++k) {
-                                    vs[pair][x * (NG / 2) + k] = 0u;
-                                }
+                            for (int k = 0; k < kWords; ++k) {
+                                vs[r][k] = 0u;
                             }
                         }
                     }
@@ -679,104 +676,66 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 
                 // How far a token's weights can reach above its p: log2 of its largest V scale is at most bits / 128 - 126.9 for a
                 // bf16 with these bits (log2(1 + f) <= f + 0.0861).  The constant stays out; it is taken off with the maximum.
-                float high[NH];
-                {
-                    float bits[2][2];
+                float reach[2]; // 2^23 + bits
 #pragma unroll
-                    for (int pair = 0; pair < 2; ++pair) {
-                        unsigned both = vs[pair][0]; // tokens 0 | 1, their largest
-                        if constexpr (NG > 1) {
-                            unsigned m0 = vs[pair][0], m1 = vs[pair][NG / 2];
+                for (int r = 0; r < 2; ++r) {
+                    unsigned m = vs[r][0];
 #pragma unroll
-                            for (int k = 1; k < NG / 2; ++k) {
-                                m0 = __vmaxu2(m0, vs[pair][k]);
-                                m1 = __vmaxu2(m1, vs[pair][NG / 2 + k]);
-                            }
-                            both = __vmaxu2(__byte_perm(m0, m1, 0x5410), __byte_perm(m0, m1, 0x7632));
-                        }
-                        both = __vmaxu2(both, kLeastScale | (kLeastScale << 16));
-                        bits[pair][0] = __uint_as_float(__byte_perm(both, 0x4b000000u, 0x7610)); // 2^23 + bits
-                        bits[pair][1] = __uint_as_float(__byte_perm(both, 0x4b000000u, 0x7632));
+                    for (int k = 1; k < kWords; ++k) {
+                        m = __vmaxu2(m, vs[r][k]);
                     }
-#pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-                        high[n] = kLowest;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            high[n] = fmaxf(high[n], fmaf(bits[i >> 1][i & 1], 0.0078125f, s[i >> 1][n][i & 1]));
-                        }
-                    }
+                    reach[r] = __uint_as_float(max(max(m & 0xffffu, m >> 16), kLeastScale) | 0x4b000000u);
                 }
                 constexpr float kBias = 65536.f + 126.9f; // 2^23 / 128 and the constant
-                // the maximum moves rarely
-                bool move = false;
+                float high[NH][2];
+                bool move = false; // the maximum does rarely
 #pragma unroll
                 for (int n = 0; n < NH; ++n) {
-                    high[n] -= kBias;
-                    move |= high[n] > top[n] + kSlack;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        high[n][x] = fmaxf(fmaf(reach[0], 0.0078125f, s[n][x]), fmaf(reach[1], 0.0078125f, s[n][2 + x]));
+                        move |= high[n][x] > top[n][x] + (kSlack + kBias);
+                    }
                 }
                 if (__any_sync(0xffffffffu, move)) {
-                    // a NaN scale would count as 2^129: such tokens count without theirs
-                    bool nan_scale = false;
+                    // a NaN scale would count as 2^129: such a token counts without it
 #pragma unroll
-                    for (int pair = 0; pair < 2; ++pair) {
+                    for (int r = 0; r < 2; ++r) {
+                        unsigned most = kLeastScale;
 #pragma unroll
                         for (int k = 0; k < kWords; ++k) {
-                            nan_scale |= (vs[pair][k] & 0xffffu) >= 0x7f80u || (vs[pair][k] >> 16) >= 0x7f80u;
+                            const unsigned lo = vs[r][k] & 0xffffu, hi = vs[r][k] >> 16;
+                            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
                         }
+                        reach[r] = static_cast<float>(most) * 0.0078125f - 126.9f;
                     }
-                    if (nan_scale) {
-#pragma unroll
-                        for (int n = 0; n < NH; ++n) {
-                            high[n] = kLowest;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            unsigned most = kLeastScale;
-#pragma unroll
-                            for (int k = 0; k < (NG == 1 ? 1 : NG / 2); ++k) {
-                                const unsigned w = vs[i >> 1][NG == 1 ? 0 : (i & 1) * (NG / 2) + k], lo = w & 0xffffu, hi = w >> 16;
-                                if (NG > 1 || (i & 1) == 0) {
-                                    most = max(most, lo < 0x7f80u ? lo : 0u);
-                                }
-                                if (NG > 1 || (i & 1) == 1) {
-                                    most = max(most, hi < 0x7f80u ? hi : 0u);
-                                }
-                            }
-#pragma unroll
-                            for (int n = 0; n < NH; ++n) {
-                                high[n] = fmaxf(high[n], s[i >> 1][n][i & 1] + (static_cast<float>(most) * 0.0078125f - 126.9f));
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-                        high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 1));
-                        high[n] = fmaxf(high[n], __shfl_xor_sync(0xffffffffu, high[n], 2));
-                        const float now = fmaxf(top[n], high[n]);
-                        const float alpha = exp2Fast(top[n] - now); // the first time: 0
-                        top[n] = now;
-                        sum[n] *= alpha;
-                        const float alpha0 = __shfl_sync(0xffffffffu, alpha, 8 * t), alpha1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
-#pragma unroll
-                        for (int j = 0; j < HD / 16; ++j) {
-                            o[n][j][0] *= alpha0;
-                            o[n][j][1] *= alpha1;
-                            o[n][j][2] *= alpha0;
-                            o[n][j][3] *= alpha1;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int pair = 0; pair < 2; ++pair) {
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            s[pair][n][x] = exp2Fast(s[pair][n][x] - top[n]);
+                            float now = fmaxf(top[n][x], fmaxf(s[n][x] + reach[0], s[n][2 + x] + reach[1]));
+                            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
+                            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
+                            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
+                            const float alpha = exp2Fast(top[n][x] - now); // the first time: 0
+                            top[n][x] = now;
+                            sum[n][x] *= alpha;
+#pragma unroll
+                            for (int j = 0; j < HD / 16; ++j) {
+                                o[n][j][x] *= alpha;
+                                o[n][j][2 + x] *= alpha;
+                            }
                         }
-                        sum[n] += s[pair][n][0] + s[pair][n][1];
                     }
+                }
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[n][i] = exp2Fast(s[n][i] - top[n][i & 1]);
+                    }
+                    sum[n][0] += s[n][0] + s[n][2];
+                    sum[n][1] += s[n][1] + s[n][3];
                 }
 
                 // outputs
@@ -789,13 +748,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     for (int x = 0; x < 2; ++x) {
                         const int j = c + x;
                         if (BITS == 4 || j == 0) { // the weights of this group
+                            const float v0 = scaleAt(vs[0], BITS == 4 ? j : 0), v1 = scaleAt(vs[1], BITS == 4 ? j : 0);
 #pragma unroll
-                            for (int pair = 0; pair < 2; ++pair) {
-                                const float v0 = scaleAt(vs[pair], 0, BITS == 4 ? j : 0), v1 = scaleAt(vs[pair], 1, BITS == 4 ? j : 0);
-#pragma unroll
-                                for (int n = 0; n < NH; ++n) {
-                                    weight[n][pair] = packHalves(s[pair][n][0] * v0, s[pair][n][1] * v1);
-                                }
+                            for (int n = 0; n < NH; ++n) {
+                                weight[n][0] = transposed(packHalves(s[n][0] * v0, s[n][1] * v0));
+                                weight[n][1] = transposed(packHalves(s[n][2] * v1, s[n][3] * v1));
                             }
                         }
                         if constexpr (BITS == 4) {
@@ -809,7 +766,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                             }
                         } else {
                             const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
-                            const unsigned a0 = codes8<0x4240>(magic, lo), a1 = codes8<0x4341>(magic, lo), a2 = codes8<0x4240>(magic, hi), a3 = codes8<0x4341>(magic, hi);
+                            const unsigned a0 = codes8<0x4240>(magic, lo), a1 = codes8<0x4341>(magic, lo);
+                            const unsigned a2 = codes8<0x4240>(magic, hi), a3 = codes8<0x4341>(magic, hi);
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
                                 mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
@@ -834,12 +792,16 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             }
             place = unit_first + done.tiles + kUnitCost; // if the range goes on, it does with the next unit
             tile = 0;
-            float inv[NH];
+            float inv[NH][2];
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
-                sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
-                sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
-                inv[n] = 1.f / sum[n];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    sum[n][x] += __shfl_xor_sync(0xffffffffu, sum[n][x], 4);
+                    sum[n][x] += __shfl_xor_sync(0xffffffffu, sum[n][x], 8);
+                    sum[n][x] += __shfl_xor_sync(0xffffffffu, sum[n][x], 16);
+                    inv[n][x] = 1.f / sum[n][x];
+                }
             }
             if (!(first && last) && lane == 0) {
                 pieces[2 * warp + first] = {unit_first, done.seq, done.sub, done.tiles, 1};
@@ -852,13 +814,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 constexpr int kPer = BITS == 4 ? 4 : 2; // neighbouring elements of a row that a lane has
                 constexpr int kRuns = HD / (8 * kPer);
                 if (first && last) {
-                    const float inv0 = __shfl_sync(0xffffffffu, inv[n], 8 * t), inv1 = __shfl_sync(0xffffffffu, inv[n], 8 * t + 4);
                     const long long row = done.seq * a.o_seq + (head_at + 8 * n + 2 * t) * a.o_head;
 #pragma unroll
                     for (int j = 0; j < kRuns; ++j) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const float f = x ? inv1 : inv0;
+                            const float f = inv[n][x];
                             float v[kPer];
                             v[0] = o[n][BITS == 4 ? 2 * j : j][x] * f;
                             v[1] = o[n][BITS == 4 ? 2 * j : j][2 + x] * (BITS == 4 ? f * 0.0625f : f);
@@ -872,8 +833,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         }
                     }
                 } else {
-                    if (t == 0) {
-                        sums[(2 * warp + first) * HT + 8 * n + g] = make_float2(top[n], sum[n]);
+                    if (g == 0) {
+                        sums[(2 * warp + first) * HT + 8 * n + 2 * t] = make_float2(top[n][0], sum[n][0]);
+                        sums[(2 * warp + first) * HT + 8 * n + 2 * t + 1] = make_float2(top[n][1], sum[n][1]);
                     }
                     float *row0 = mine_o + (8 * n + 2 * t) * C::kStride, *row1 = row0 + C::kStride;
 #pragma unroll
