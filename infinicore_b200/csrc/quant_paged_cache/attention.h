@@ -81,6 +81,8 @@ struct TilesPlan {
     unsigned half_magic = 0, half_self = 0; // division by block_size / 8
     int half_shift = 0;
     bool out_words = false;
+    bool task_of_unit = false; // how the combine kernel's tasks are numbered
+    int tasks = 0, combine_heads = 0, combine_parts = 0;
     size_t tasks_bytes = 0;
     size_t workspace_bytes = 0;
 };

@@ -1,6 +1,6 @@
-// The fast kernel of infiniopQuantPagedAttention: tiles of 16 tokens, matrix instructions on the codes.
+// The fast kernel of infiniopQuantPagedAttention: tiles of 16 or 32 tokens, matrix instructions on the codes.
 //
-// Work.  A unit is (sequence, kv head, tile of 8 or 16 q heads of its group), ceil(length / 16) token tiles long.
+// Work.  A unit is (sequence, kv head, tile of 8 or 16 q heads of its group), as many token tiles long as cover the sequence.
 // All units lie end to end in one line, each with kUnitCost tiles in front for what a unit costs by itself (q, results),
 // and the line is cut into equal ranges, one for each warp of a persistent grid, so that ragged batches, many short and
 // few long sequences load the machine alike.  A warp that has a unit to itself stores its rows; pieces of a unit in one
@@ -37,14 +37,14 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 16;
 constexpr int kUnitCost = 1;       // tiles' worth of time that a unit costs beside its tiles
 constexpr int kMinRange = 3;       // of a warp: at least two tiles of a unit's first range
 constexpr float kSlack = 8.f;      // in the log2 domain; 2^8 is far inside fp16
 constexpr unsigned kLeastScale = 27u << 7; // V scales count as at least 2^-100 for the maximum: an all-zero row stays finite
 
+// What the combine kernel has to do for a unit: nothing, or to add this many pieces from this CTA's on.
 struct Task {
-    int seq, sub, pieces, pad;
+    int seq, sub, pieces, cta;
 };
 
 // A part of a unit that one warp has done: first tile's position on the line, tiles of the whole unit.
@@ -60,13 +60,17 @@ struct Cfg {
     static constexpr int kRowBytes = HD * BITS / 8;
     static constexpr int kChunks = kRowBytes / 16;            // 16-byte chunks of a row
     static constexpr int kGroups = BITS == 4 ? HD / 32 : 1;   // scales of a row
+    // A tile is one or two times 16 tokens: the loop around the matrix instructions costs as many issue slots as 8 tokens' arithmetic,
+    // which is what bounds the 4-bit form.
+    static constexpr int kSubs = BITS == 4 && HD * HT <= 1024 ? 2 : 1;
+    static constexpr int kTile = 16 * kSubs;
     static constexpr int kStage = 2 * kTile * kRowBytes + 2 * kTile * kGroups * 2;
     static constexpr int kHeadTiles = HT / 8;
     static constexpr int kStride = HD + 4;                    // floats: rows of two heads apart hit other banks
     static constexpr int kResult = HT * kStride * 4;
     static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes) + kThreads * 4 + 256;
     // resident CTAs: what the registers of q, outputs and scales leave room for
-    static constexpr int kCtas = HD * HT <= 1024 ? 4 : HD * HT <= 1536 ? 3 : 2;
+    static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
     static constexpr int kStages = kFit > 6 ? 6 : kFit;
     static_assert(kStages >= 2, "a ring of two tiles at least");
@@ -184,8 +188,10 @@ __device__ __forceinline__ unsigned codes8(const Magic &m, unsigned flipped) {
 // ---- the line of tiles -------------------------------------------------------------------------------------
 
 struct TilesArgs {
-    unsigned char *workspace; // Task[ctas] | records
+    unsigned char *workspace; // Task[] | records
     long long tasks_bytes;
+    int task_of_unit;         // tasks are numbered by unit, where there are no more units than CTAs; otherwise by CTA
+    int combine_heads;        // of a CTA of the combine kernel
     int subs;                 // kv heads * head tiles of a group
     int head_tiles;
     unsigned halves;          // block_size / 8
@@ -206,8 +212,14 @@ struct Lens { // lengths of the sequences a CTA meets first, in shared memory
     }
 };
 
-__device__ __forceinline__ int tilesOf(int len) { return len > 0 ? (len + kTile - 1) / kTile : 0; }
-__device__ __forceinline__ long long costOf(int len) { return len > 0 ? tilesOf(len) + kUnitCost : 0; }
+template <int TILE>
+__device__ __forceinline__ int tilesOf(int len) {
+    return len > 0 ? (len + TILE - 1) / TILE : 0;
+}
+template <int TILE>
+__device__ __forceinline__ long long costOf(int len) {
+    return len > 0 ? tilesOf<TILE>(len) + kUnitCost : 0;
+}
 
 // Where a walk over a warp's range is: the unit, how much of the range lies behind what it takes of that unit.  Kept in
 // shared memory, read and written by all lanes alike: the loop over a unit's tiles has no use for it.
@@ -215,6 +227,7 @@ struct Walk {
     int seq, sub, tiles, len, budget, pad;
 
     // To the next unit: how many of its tiles are in the range (0: the range has ended).
+    template <int TILE>
     __device__ __forceinline__ int step(int subs, const Lens &lens) {
         budget -= kUnitCost; // at or below 0: the range ends in front of the unit's first tile
         if (budget <= 0) {
@@ -225,7 +238,7 @@ struct Walk {
             do {
                 len = lens(++seq);
             } while (len <= 0);
-            tiles = tilesOf(len);
+            tiles = tilesOf<TILE>(len);
         }
         const int n = min(tiles, budget);
         budget -= n;
@@ -268,7 +281,7 @@ __device__ __forceinline__ void storeOut(const AttentionArgs &a, const TilesArgs
 template <int BITS, int HD, int HT, bool P16>
 __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAttentionTilesKernel(const AttentionArgs a, const TilesArgs p) {
     using C = Cfg<BITS, HD, HT>;
-    constexpr int NG = C::kGroups, NH = C::kHeadTiles, CPR = C::kChunks, S = C::kStages;
+    constexpr int NG = C::kGroups, NH = C::kHeadTiles, CPR = C::kChunks, S = C::kStages, TILE = C::kTile, SUBS = C::kSubs;
     extern __shared__ __align__(128) unsigned char smem[];
     float *results = reinterpret_cast<float *>(smem + kWarps * C::kRing);                                     // [warp][head][kStride]
     float2 *sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(results) + kWarps * C::kResult); // [warp][2][head]
@@ -288,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     for (int i = 0; i < per; ++i) {
         const int s = tid * per + i;
         const int len = s < a.num_seqs ? lengthOf(a, s) : 0;
-        mine += costOf(len);
+        mine += costOf<TILE>(len);
         if (per == 1) {
             lens_s[tid] = len;
         }
@@ -319,10 +332,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     long long range = (total + workers - 1) / workers;
     range = range > kMinRange ? range : kMinRange;
     const long long cta_range = range * kWarps, cta_start = cta_range * blockIdx.x;
-    Task *task = reinterpret_cast<Task *>(p.workspace) + blockIdx.x;
+    Task *tasks = reinterpret_cast<Task *>(p.workspace);
     if (cta_start >= total) {
-        if (tid == 0) {
-            task->pieces = 0;
+        if (tid == 0 && !p.task_of_unit) {
+            tasks[blockIdx.x].pieces = 0;
         }
         return;
     }
@@ -332,10 +345,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             long long pos = cta_start + w * range - (upto - mine) * p.subs;
             if (pos >= 0 && pos < mine * p.subs) { // one thread for each start
                 int s = tid * per;
-                long long cost = costOf(lengthOf(a, s)) * p.subs;
+                long long cost = costOf<TILE>(lengthOf(a, s)) * p.subs;
                 while (pos >= cost) {
                     pos -= cost;
-                    cost = costOf(lengthOf(a, ++s)) * p.subs;
+                    cost = costOf<TILE>(lengthOf(a, ++s)) * p.subs;
                 }
                 plan_s[4 + 2 * w] = s;
                 plan_s[5 + 2 * w] = pos;
@@ -360,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             Walk w;
             w.seq = static_cast<int>(plan_s[4 + 2 * warp]);
             w.len = lens(w.seq);
-            w.tiles = tilesOf(w.len);
+            w.tiles = tilesOf<TILE>(w.len);
             const long long pos = plan_s[5 + 2 * warp], cost = w.tiles + kUnitCost;
             w.sub = static_cast<int>(pos / cost);
             const int in = static_cast<int>(pos - w.sub * cost) - kUnitCost; // below 0: in front of the unit's first tile
@@ -374,20 +387,21 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         }
 
         // ---- copies: the next tile's block is already looked up
-        unsigned f_half = 2u * static_cast<unsigned>(tile); // first half (8 tokens) of the next tile, within its unit
+        unsigned f_half = TILE / 8 * static_cast<unsigned>(tile); // first half (8 tokens) of the next tile, within its unit
         int f_left = left;
         const unsigned char *table_row = nullptr;
-        // this lane's first 16 bytes of K and V codes and of scales in block 0 of the unit's kv head
-        const unsigned char *k_lane = nullptr, *v_lane = nullptr, *s_lane = nullptr;
-        unsigned block0 = 0, block1 = 0, slot0 = 0, slot1 = 0; // blocks of the halves, their first slots there
+        // block 0 of the unit's kv head: K and V codes, and this lane's 16 bytes of scales in a run of 8 tokens
+        const unsigned char *k_unit = nullptr, *v_unit = nullptr, *s_lane = nullptr;
+        constexpr int kRuns = P16 ? SUBS : 2 * SUBS; // runs of 16 or 8 tokens, each in one block
+        unsigned block[kRuns] = {}, first_slot[kRuns] = {}; // of the next tile's runs: the block, the first slot there
         const unsigned code_block = static_cast<unsigned>(a.k_block), code_slot = static_cast<unsigned>(a.k_slot);
         const unsigned scale_block = 2u * static_cast<unsigned>(a.ks_block);
         auto unit = [&]() {
             const int kv = copies.sub / p.head_tiles;
             table_row = static_cast<const unsigned char *>(a.block_tables) + ((copies.seq * a.table_seq) << p.index_shift);
-            k_lane = a.k_codes + kv * a.k_head;
-            v_lane = a.v_codes + kv * a.k_head;
-            const bool v = lane >= 2 * NG;
+            k_unit = a.k_codes + kv * a.k_head;
+            v_unit = a.v_codes + kv * a.k_head;
+            const bool v = lane >= TILE / 8 * NG;
             s_lane = reinterpret_cast<const unsigned char *>((v ? a.v_scales : a.k_scales) + kv * a.ks_head) + (lane % NG) * 16;
         };
         auto entry = [&](unsigned page) { // the low word of a 64-bit entry says all that a block in the pool can be
@@ -404,47 +418,57 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         };
         auto look = [&]() {
             const unsigned page = (__umulhi(f_half, p.half_magic) + (f_half & p.half_self)) >> p.half_shift;
-            slot0 = 8u * (f_half - page * p.halves);
-            block0 = entry(page);
-            if constexpr (!P16) {
-                block1 = block0;
-                slot1 = slot0 + 8u;
-                if (slot1 == static_cast<unsigned>(a.block_size)) {
-                    // the second half is the next block's; behind the sequence's end it is read where the first is
-                    if (8 * static_cast<int>(f_half + 1) < copies.len) {
-                        block1 = entry(page + 1);
-                        slot1 = 0;
-                    } else {
-                        slot1 = slot0;
-                    }
-                }
+            first_slot[0] = 8u * (f_half - page * p.halves);
+            unsigned at = page;
+            block[0] = entry(at);
+#pragma unroll
+            for (int r = 1; r < kRuns; ++r) {
+                // a run behind the sequence's end, whose table entry may say anything, is read where the one before is; entries are
+                // only loaded here (the same one twice, if it must be): the next fetch is the first to wait for them
+                constexpr unsigned kTokens = P16 ? 16u : 8u;
+                const unsigned slot = first_slot[r - 1] + kTokens;
+                const bool live = 8 * static_cast<int>(f_half) + r * static_cast<int>(kTokens) < copies.len;
+                const bool turn = slot >= static_cast<unsigned>(a.block_size);
+                at += live && turn ? 1u : 0u;
+                first_slot[r] = !live ? first_slot[r - 1] : turn ? 0u : slot;
+                block[r] = entry(at);
             }
         };
         auto fetch = [&](unsigned dst) { // the next tile into a slot of the ring
             if (f_left > 0) {
-                const unsigned long long c0 = static_cast<unsigned long long>(block0) * code_block + static_cast<unsigned long long>(slot0) * code_slot;
-                const unsigned long long c1 = P16 ? c0 + 8ull * code_slot
-                                                  : static_cast<unsigned long long>(block1) * code_block + static_cast<unsigned long long>(slot1) * code_slot;
+                unsigned long long from[kRuns];
 #pragma unroll
-                for (int j = 0; j < CPR / 2; ++j) {
+                for (int r = 0; r < kRuns; ++r) {
+                    from[r] = static_cast<unsigned long long>(block[r]) * code_block + static_cast<unsigned long long>(first_slot[r]) * code_slot;
+                }
+                constexpr int kCopies = CPR * TILE / 32; // of a lane, for K as for V
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j) {
                     const int i = lane + 32 * j, r = i / CPR, c = i % CPR;
                     const int swz = CPR % 8 == 0 ? (r & 7) : CPR % 4 == 0 ? ((r >> 1) & 3) : ((r >> 2) & 1);
                     const unsigned to = dst + r * C::kRowBytes + ((c ^ swz) << 4);
-                    const unsigned in = static_cast<unsigned>(r & 7) * code_slot + c * 16;
-                    const unsigned long long from = (r < 8 ? c0 : c1) + in;
-                    copy16(to, k_lane + from);
-                    copy16(to + kTile * C::kRowBytes, v_lane + from);
+                    const int sub = SUBS == 1 ? 0 : 32 * j / CPR / 16; // where there are two, 16 rows are whole rounds of the warp
+                    const unsigned long long run = P16 ? from[sub] : (r & 8) ? from[kRuns == 1 ? 0 : 2 * sub + 1] : from[P16 ? 0 : 2 * sub];
+                    const unsigned in = static_cast<unsigned>(P16 ? r & 15 : r & 7) * code_slot + c * 16;
+                    copy16(to, k_unit + (run + in));
+                    copy16(to + TILE * C::kRowBytes, v_unit + (run + in));
                 }
-                // scales: a half's 8 rows are one run of NG chunks
-                if (lane < 4 * NG) {
-                    const bool h = (lane / NG) & 1;
-                    const unsigned b = P16 || !h ? block0 : block1, at = h ? (P16 ? slot0 + 8u : slot1) : slot0;
-                    copy16(dst + 2 * kTile * C::kRowBytes + lane * 16, s_lane + static_cast<unsigned long long>(b) * scale_block + at * (2u * NG));
+                // scales: 8 rows are one run of NG chunks
+                if (lane < TILE / 4 * NG) {
+                    const int h = (lane / NG) & (TILE / 8 - 1), r = P16 ? h >> 1 : h;
+                    unsigned b = block[0], at = first_slot[0];
+#pragma unroll
+                    for (int k = 1; k < kRuns; ++k) {
+                        b = r == k ? block[k] : b;
+                        at = r == k ? first_slot[k] : at;
+                    }
+                    at += P16 ? 8u * (h & 1) : 0u;
+                    copy16(dst + 2 * TILE * C::kRowBytes + lane * 16, s_lane + static_cast<unsigned long long>(b) * scale_block + at * (2u * NG));
                 }
-                f_half += 2u;
+                f_half += TILE / 8;
                 if (--f_left == 0) {
                     Walk w = copies;
-                    f_left = w.step(p.subs, lens);
+                    f_left = w.step<TILE>(p.subs, lens);
                     __syncwarp();
                     copies = w;
                     __syncwarp();
@@ -558,117 +582,118 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 }
             }
 
-            int token0 = tile * kTile;
+            int token0 = tile * TILE;
             // from this token on a tile needs more than the plain arithmetic: a distance bias, tokens behind the end
-            const int special = a.alibi != nullptr ? 0 : len - kTile + 1;
+            const int special = a.alibi != nullptr ? 0 : len - TILE + 1;
             do {
                 waitCopies<S - 2>();
                 __syncwarp();
                 fetch(spare);
-                const unsigned k_addr = stage + m_row * C::kRowBytes, v_addr = k_addr + kTile * C::kRowBytes;
+                const unsigned k_addr = stage + m_row * C::kRowBytes, v_addr = k_addr + TILE * C::kRowBytes;
 
-                // scales of the lane's tokens g and g + 8, two groups a word (one scale: the low half)
+                // scales of the lane's tokens g and g + 8 of each 16, two groups a word (one scale: the low half)
                 constexpr int kWords = NG == 1 ? 1 : NG / 2;
-                unsigned ks[2][kWords], vs[2][kWords];
-                {
-                    const unsigned char *sc = ring + (stage - ring_addr) + 2 * kTile * C::kRowBytes + g * (2 * NG);
+                const unsigned char *scales = ring + (stage - ring_addr) + 2 * TILE * C::kRowBytes + g * (2 * NG);
+                auto loadScales = [](unsigned (&w)[kWords], const unsigned char *from) {
+                    if constexpr (NG == 1) {
+                        w[0] = *reinterpret_cast<const unsigned short *>(from);
+                    } else if constexpr (kWords == 4) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(from);
+                        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+                    } else if constexpr (kWords == 2) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(from);
+                        w[0] = x.x, w[1] = x.y;
+                    } else {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const unsigned char *kp = sc + r * (16 * NG), *vp = kp + 32 * NG;
-                        if constexpr (NG == 1) {
-                            ks[r][0] = *reinterpret_cast<const unsigned short *>(kp);
-                            vs[r][0] = *reinterpret_cast<const unsigned short *>(vp);
-                        } else if constexpr (kWords % 4 == 0) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(kp), y = *reinterpret_cast<const uint4 *>(vp);
-                            ks[r][0] = x.x, ks[r][1] = x.y, ks[r][2] = x.z, ks[r][3] = x.w;
-                            vs[r][0] = y.x, vs[r][1] = y.y, vs[r][2] = y.z, vs[r][3] = y.w;
-                        } else if constexpr (kWords == 2) {
-                            const uint2 x = *reinterpret_cast<const uint2 *>(kp), y = *reinterpret_cast<const uint2 *>(vp);
-                            ks[r][0] = x.x, ks[r][1] = x.y;
-                            vs[r][0] = y.x, vs[r][1] = y.y;
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < kWords; ++i) {
-                                ks[r][i] = reinterpret_cast<const unsigned *>(kp)[i];
-                                vs[r][i] = reinterpret_cast<const unsigned *>(vp)[i];
-                            }
+                        for (int i = 0; i < kWords; ++i) {
+                            w[i] = reinterpret_cast<const unsigned *>(from)[i];
                         }
                     }
-                }
+                };
                 auto scaleAt = [](const unsigned (&w)[kWords], int j) {
                     return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
                 };
 
                 // scores
-                float s[NH][4]; // [.][tokens g, heads 2t and 2t + 1 | tokens g + 8]
+                float s[SUBS][NH][4]; // [.][.][token g, heads 2t and 2t + 1 | token g + 8]
 #pragma unroll
-                for (int n = 0; n < NH; ++n) {
+                for (int u = 0; u < SUBS; ++u) {
+                    unsigned ks[2][kWords];
+                    loadScales(ks[0], scales + u * (32 * NG));
+                    loadScales(ks[1], scales + u * (32 * NG) + 16 * NG);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[n][i] = 0.f;
+                    for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            s[u][n][i] = 0.f;
+                        }
                     }
-                }
 #pragma unroll
-                for (int c = 0; c < CPR; c += 2) {
-                    unsigned w[4];
-                    loadMatrices(w, k_addr + (((c + m_chunk) ^ m_swz) << 4));
+                    for (int c = 0; c < CPR; c += 2) {
+                        unsigned w[4];
+                        loadMatrices(w, k_addr + u * (16 * C::kRowBytes) + (((c + m_chunk) ^ m_swz) << 4));
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) { // the two chunks
-                        const int j = c + x;
-                        if constexpr (BITS == 4) {
-                            unsigned lo[4], hi[4];
-                            codes4(magic, w[2 * x], lo);
-                            codes4(magic, w[2 * x + 1], hi);
-                            const float s0 = scaleAt(ks[0], j), s1 = scaleAt(ks[1], j);
+                        for (int x = 0; x < 2; ++x) { // the two chunks
+                            const int j = c + x;
+                            if constexpr (BITS == 4) {
+                                unsigned lo[4], hi[4];
+                                codes4(magic, w[2 * x], lo);
+                                codes4(magic, w[2 * x + 1], hi);
+                                const float s0 = scaleAt(ks[0], j), s1 = scaleAt(ks[1], j);
 #pragma unroll
-                            for (int n = 0; n < NH; ++n) {
-                                float d[4];
-                                mmaFirst(d, lo[0], hi[0], lo[1], hi[1], qr[n][2 * j][0], qr[n][2 * j][1]);
-                                mma(d, lo[2], hi[2], lo[3], hi[3], qr[n][2 * j + 1][0], qr[n][2 * j + 1][1]);
-                                s[n][0] = fmaf(s0, d[0], s[n][0]);
-                                s[n][1] = fmaf(s0, d[1], s[n][1]);
-                                s[n][2] = fmaf(s1, d[2], s[n][2]);
-                                s[n][3] = fmaf(s1, d[3], s[n][3]);
-                            }
-                        } else {
-                            const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
-                            const unsigned a0 = codes8<0x4140>(magic, lo), a1 = codes8<0x4140>(magic, hi);
-                            const unsigned a2 = codes8<0x4342>(magic, lo), a3 = codes8<0x4342>(magic, hi);
+                                for (int n = 0; n < NH; ++n) {
+                                    float d[4];
+                                    mmaFirst(d, lo[0], hi[0], lo[1], hi[1], qr[n][2 * j][0], qr[n][2 * j][1]);
+                                    mma(d, lo[2], hi[2], lo[3], hi[3], qr[n][2 * j + 1][0], qr[n][2 * j + 1][1]);
+                                    s[u][n][0] = fmaf(s0, d[0], s[u][n][0]);
+                                    s[u][n][1] = fmaf(s0, d[1], s[u][n][1]);
+                                    s[u][n][2] = fmaf(s1, d[2], s[u][n][2]);
+                                    s[u][n][3] = fmaf(s1, d[3], s[u][n][3]);
+                                }
+                            } else {
+                                const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
+                                const unsigned a0 = codes8<0x4140>(magic, lo), a1 = codes8<0x4140>(magic, hi);
+                                const unsigned a2 = codes8<0x4342>(magic, lo), a3 = codes8<0x4342>(magic, hi);
 #pragma unroll
-                            for (int n = 0; n < NH; ++n) {
-                                mma(s[n], a0, a1, a2, a3, qr[n][j][0], qr[n][j][1]);
+                                for (int n = 0; n < NH; ++n) {
+                                    mma(s[u][n], a0, a1, a2, a3, qr[n][j][0], qr[n][j][1]);
+                                }
                             }
                         }
                     }
-                }
-                {
                     const float s0 = BITS == 8 ? scaleAt(ks[0], 0) : 1.f, s1 = BITS == 8 ? scaleAt(ks[1], 0) : 1.f;
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            s[n][i] *= BITS == 8 ? factor[n][i & 1] * (i < 2 ? s0 : s1) : factor[n][i & 1];
+                            s[u][n][i] *= BITS == 8 ? factor[n][i & 1] * (i < 2 ? s0 : s1) : factor[n][i & 1];
                         }
                     }
                 }
+                unsigned vs[SUBS][2][kWords];
+#pragma unroll
+                for (int u = 0; u < SUBS; ++u) {
+                    loadScales(vs[u][0], scales + 2 * TILE * NG + u * (32 * NG));
+                    loadScales(vs[u][1], scales + 2 * TILE * NG + u * (32 * NG) + 16 * NG);
+                }
                 if (token0 >= special) {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const int token = token0 + 8 * r + g;
+                    for (int r = 0; r < 2 * SUBS; ++r) {
+                        const int u = r >> 1, i = 2 * (r & 1), token = token0 + 8 * r + g;
                         const float far = static_cast<float>(token - (len - 1));
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
-                            s[n][2 * r] += slope[n][0] * far;
-                            s[n][2 * r + 1] += slope[n][1] * far;
+                            s[u][n][i] += slope[n][0] * far;
+                            s[u][n][i + 1] += slope[n][1] * far;
                         }
                         if (token >= len) { // no weight, whatever the scales are
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
-                                s[n][2 * r] = s[n][2 * r + 1] = -INFINITY;
+                                s[u][n][i] = s[u][n][i + 1] = -INFINITY;
                             }
 #pragma unroll
                             for (int k = 0; k < kWords; ++k) {
-                                vs[r][k] = 0u;
+                                vs[u][r & 1][k] = 0u;
                             }
                         }
                     }
@@ -676,35 +701,38 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 
                 // How far a token's weights can reach above its p: log2 of its largest V scale is at most bits / 128 - 126.9 for a
                 // bf16 with these bits (log2(1 + f) <= f + 0.0861).  The constant stays out; it is taken off with the maximum.
-                float reach[2]; // 2^23 + bits
+                float reach[2 * SUBS]; // 2^23 + bits
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    unsigned m = vs[r][0];
+                for (int r = 0; r < 2 * SUBS; ++r) {
+                    unsigned m = vs[r >> 1][r & 1][0];
 #pragma unroll
                     for (int k = 1; k < kWords; ++k) {
-                        m = __vmaxu2(m, vs[r][k]);
+                        m = __vmaxu2(m, vs[r >> 1][r & 1][k]);
                     }
                     reach[r] = __uint_as_float(max(max(m & 0xffffu, m >> 16), kLeastScale) | 0x4b000000u);
                 }
                 constexpr float kBias = 65536.f + 126.9f; // 2^23 / 128 and the constant
-                float high[NH][2];
                 bool move = false; // the maximum does rarely
 #pragma unroll
                 for (int n = 0; n < NH; ++n) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        high[n][x] = fmaxf(fmaf(reach[0], 0.0078125f, s[n][x]), fmaf(reach[1], 0.0078125f, s[n][2 + x]));
-                        move |= high[n][x] > top[n][x] + (kSlack + kBias);
+                        float high = fmaf(reach[0], 0.0078125f, s[0][n][x]);
+#pragma unroll
+                        for (int r = 1; r < 2 * SUBS; ++r) {
+                            high = fmaxf(high, fmaf(reach[r], 0.0078125f, s[r >> 1][n][2 * (r & 1) + x]));
+                        }
+                        move |= high > top[n][x] + (kSlack + kBias);
                     }
                 }
                 if (__any_sync(0xffffffffu, move)) {
                     // a NaN scale would count as 2^129: such a token counts without it
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+                    for (int r = 0; r < 2 * SUBS; ++r) {
                         unsigned most = kLeastScale;
 #pragma unroll
                         for (int k = 0; k < kWords; ++k) {
-                            const unsigned lo = vs[r][k] & 0xffffu, hi = vs[r][k] >> 16;
+                            const unsigned lo = vs[r >> 1][r & 1][k] & 0xffffu, hi = vs[r >> 1][r & 1][k] >> 16;
                             most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
                         }
                         reach[r] = static_cast<float>(most) * 0.0078125f - 126.9f;
@@ -713,7 +741,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     for (int n = 0; n < NH; ++n) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            float now = fmaxf(top[n][x], fmaxf(s[n][x] + reach[0], s[n][2 + x] + reach[1]));
+                            float now = top[n][x];
+#pragma unroll
+                            for (int r = 0; r < 2 * SUBS; ++r) {
+                                now = fmaxf(now, s[r >> 1][n][2 * (r & 1) + x] + reach[r]);
+                            }
                             now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
                             now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
                             now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
@@ -729,53 +761,59 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < NH; ++n) {
+                for (int u = 0; u < SUBS; ++u) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[n][i] = exp2Fast(s[n][i] - top[n][i & 1]);
+                    for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            s[u][n][i] = exp2Fast(s[u][n][i] - top[n][i & 1]);
+                        }
+                        sum[n][0] += s[u][n][0] + s[u][n][2];
+                        sum[n][1] += s[u][n][1] + s[u][n][3];
                     }
-                    sum[n][0] += s[n][0] + s[n][2];
-                    sum[n][1] += s[n][1] + s[n][3];
                 }
 
                 // outputs
-                unsigned weight[NH][2];
 #pragma unroll
-                for (int c = 0; c < CPR; c += 2) {
-                    unsigned w[4];
-                    loadMatricesTransposed(w, v_addr + (((c + m_chunk) ^ m_swz) << 4));
+                for (int u = 0; u < SUBS; ++u) {
+                    unsigned weight[NH][2];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int j = c + x;
-                        if (BITS == 4 || j == 0) { // the weights of this group
-                            const float v0 = scaleAt(vs[0], BITS == 4 ? j : 0), v1 = scaleAt(vs[1], BITS == 4 ? j : 0);
+                    for (int c = 0; c < CPR; c += 2) {
+                        unsigned w[4];
+                        loadMatricesTransposed(w, v_addr + u * (16 * C::kRowBytes) + (((c + m_chunk) ^ m_swz) << 4));
 #pragma unroll
-                            for (int n = 0; n < NH; ++n) {
-                                weight[n][0] = transposed(packHalves(s[n][0] * v0, s[n][1] * v0));
-                                weight[n][1] = transposed(packHalves(s[n][2] * v1, s[n][3] * v1));
+                        for (int x = 0; x < 2; ++x) {
+                            const int j = c + x;
+                            if (BITS == 4 || j == 0) { // the weights of this group
+                                const float v0 = scaleAt(vs[u][0], BITS == 4 ? j : 0), v1 = scaleAt(vs[u][1], BITS == 4 ? j : 0);
+#pragma unroll
+                                for (int n = 0; n < NH; ++n) {
+                                    weight[n][0] = transposed(packHalves(s[u][n][0] * v0, s[u][n][1] * v0));
+                                    weight[n][1] = transposed(packHalves(s[u][n][2] * v1, s[u][n][3] * v1));
+                                }
                             }
-                        }
-                        if constexpr (BITS == 4) {
-                            unsigned lo[4], hi[4];
-                            codes4Odd16(magic, w[2 * x], lo);
-                            codes4Odd16(magic, w[2 * x + 1], hi);
+                            if constexpr (BITS == 4) {
+                                unsigned lo[4], hi[4];
+                                codes4Odd16(magic, w[2 * x], lo);
+                                codes4Odd16(magic, w[2 * x + 1], hi);
 #pragma unroll
-                            for (int n = 0; n < NH; ++n) {
-                                mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], weight[n][0], weight[n][1]);
-                                mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], weight[n][0], weight[n][1]);
-                            }
-                        } else {
-                            const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
-                            const unsigned a0 = codes8<0x4240>(magic, lo), a1 = codes8<0x4341>(magic, lo);
-                            const unsigned a2 = codes8<0x4240>(magic, hi), a3 = codes8<0x4341>(magic, hi);
+                                for (int n = 0; n < NH; ++n) {
+                                    mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], weight[n][0], weight[n][1]);
+                                    mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], weight[n][0], weight[n][1]);
+                                }
+                            } else {
+                                const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
+                                const unsigned a0 = codes8<0x4240>(magic, lo), a1 = codes8<0x4341>(magic, lo);
+                                const unsigned a2 = codes8<0x4240>(magic, hi), a3 = codes8<0x4341>(magic, hi);
 #pragma unroll
-                            for (int n = 0; n < NH; ++n) {
-                                mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
+                                for (int n = 0; n < NH; ++n) {
+                                    mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
+                                }
                             }
                         }
                     }
                 }
-                token0 += kTile;
+                token0 += TILE;
                 spare = stage;
                 stage = stage == ring_addr + (S - 1) * C::kStage ? ring_addr : stage + C::kStage;
             } while (--left > 0);
@@ -786,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             const bool first = unit_first >= start, last = unit_first + done.tiles <= end;
             {
                 Walk w = done;
-                left = last ? w.step(p.subs, lens) : 0;
+                left = last ? w.step<TILE>(p.subs, lens) : 0;
                 __syncwarp();
                 work = w;
             }
@@ -802,6 +840,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     sum[n][x] += __shfl_xor_sync(0xffffffffu, sum[n][x], 16);
                     inv[n][x] = 1.f / sum[n][x];
                 }
+            }
+            if (first && last && lane == 0 && p.task_of_unit) {
+                tasks[done.seq * p.subs + done.sub].pieces = 0;
             }
             if (!(first && last) && lane == 0) {
                 pieces[2 * warp + first] = {unit_first, done.seq, done.sub, done.tiles, 1};
@@ -856,7 +897,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 
     // ---- the pieces that this CTA's warps left: those of one unit are neighbours
     __syncthreads();
-    Task cut = {0, 0, 0, 0};
+    int cut = 0; // the pieces of the CTA's last unit, where that goes on in other CTAs
 #pragma unroll 1
     for (int k = 0; k < 2 * kWarps;) {
         const Piece piece = pieces[k];
@@ -908,57 +949,90 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 }
             }
         }
-        if (first && !last) { // the CTA's last unit: it names the pieces for the combine kernel
-            cut.seq = piece.seq;
-            cut.sub = piece.sub;
-            cut.pieces = static_cast<int>((piece.first + piece.tiles - 1) / cta_range - blockIdx.x) + 1;
+        if (first) {
+            cut = last ? 0 : static_cast<int>((piece.first + piece.tiles - 1) / cta_range - blockIdx.x) + 1;
+            if (tid == 0 && (cut > 0 || p.task_of_unit)) {
+                tasks[p.task_of_unit ? piece.seq * p.subs + piece.sub : static_cast<int>(blockIdx.x)] = {piece.seq, piece.sub, cut,
+                                                                                                        static_cast<int>(blockIdx.x)};
+            }
         }
         k = upto_k;
     }
-    if (tid == 0) {
-        *task = cut;
+    if (tid == 0 && cut == 0 && !p.task_of_unit) {
+        tasks[blockIdx.x].pieces = 0;
     }
 }
 
-// Adds the pieces of the unit that CTA x of the tiles kernel began and did not end.
+// Adds the pieces of a cut unit: CTA (task, part of its heads).  A thread has four columns of a head and every kSides-th
+// piece, which it adds as they come (maximum, sum, output); the sides meet in shared memory.  Several sides read at a
+// time, since a long sequence alone may lie in pieces over the whole grid.
+constexpr int kCombineThreads = 256;
+
 template <int HD, int HT>
-__global__ void __launch_bounds__(256) quantAttentionCombineKernel(const AttentionArgs a, const TilesArgs p) {
+__global__ void __launch_bounds__(kCombineThreads) quantAttentionCombineKernel(const AttentionArgs a, const TilesArgs p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    constexpr int kRecord = HT * HD + 2 * HT;
+    constexpr int kRecord = HT * HD + 2 * HT, kColumns = HD / 4;
+    __shared__ float4 part[kCombineThreads];
+    __shared__ float2 part_ml[kCombineThreads];
     const Task task = reinterpret_cast<const Task *>(p.workspace)[blockIdx.x];
-    if (task.pieces == 0) {
+    if (p.task_of_unit && lengthOf(a, static_cast<int>(blockIdx.x) / p.subs) <= 0) {
+        return; // no one wrote this task
+    }
+    const int kv = task.sub / p.head_tiles, head0 = (task.sub - kv * p.head_tiles) * HT; // within the group
+    const int h0 = static_cast<int>(blockIdx.y) * p.combine_heads;
+    const int heads = min(p.combine_heads, min(HT, a.group - head0) - h0);
+    if (task.pieces == 0 || heads <= 0) {
         return;
     }
     const float *records = reinterpret_cast<const float *>(p.workspace + p.tasks_bytes);
-    // piece 0 is this CTA's second record, piece i the first one of CTA x + i
-    auto recordOf = [&](int i) { return records + (2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kRecord; };
-    const int kv = task.sub / p.head_tiles;
-    const int head0 = (task.sub - kv * p.head_tiles) * HT;
-    const int heads = min(HT, a.group - head0);
-    for (int i = threadIdx.x; i < heads * (HD / 4); i += blockDim.x) {
-        const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
-        float m = kLowest;
-        for (int k = 0; k < task.pieces; ++k) {
-            m = fmaxf(m, recordOf(k)[HT * HD + h]);
-        }
-        float l = 0.f;
+    const int items = p.combine_heads * kColumns; // a multiple or a part of the threads
+    const int sides = items < kCombineThreads ? kCombineThreads / items : 1;
+    const int side = static_cast<int>(threadIdx.x) / items;
+    for (int item = sides > 1 ? static_cast<int>(threadIdx.x) % items : static_cast<int>(threadIdx.x); item < items; item += sides > 1 ? items : kCombineThreads) {
+        const int h = h0 + item / kColumns, column = item % kColumns;
+        const bool live = item / kColumns < heads;
+        float m = kLowest, l = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live && side < sides) {
 #pragma unroll 4
-        for (int k = 0; k < task.pieces; ++k) {
-            const float *r = recordOf(k);
-            const float mk = r[HT * HD + h], lk = r[HT * HD + HT + h];
-            const float f = exp2Fast(mk - m);
-            const float4 x = *reinterpret_cast<const float4 *>(r + h * HD + d);
-            l = fmaf(f, lk, l);
-            v.x = fmaf(f, x.x, v.x);
-            v.y = fmaf(f, x.y, v.y);
-            v.z = fmaf(f, x.z, v.z);
-            v.w = fmaf(f, x.w, v.w);
+            for (int k = side; k < task.pieces; k += sides) {
+                // piece 0 is the second record of the CTA that began the unit, piece k the first one of the k-th CTA behind it
+                const float *r = records + (2ll * (task.cta + k) + (k == 0 ? 1 : 0)) * kRecord;
+                const float mk = r[HT * HD + h], lk = r[HT * HD + HT + h];
+                const float4 x = *reinterpret_cast<const float4 *>(r + h * HD + 4 * column);
+                const float now = fmaxf(m, mk), f = exp2Fast(m - now), fk = exp2Fast(mk - now);
+                m = now;
+                l = fmaf(f, l, fk * lk);
+                v.x = fmaf(f, v.x, fk * x.x);
+                v.y = fmaf(f, v.y, fk * x.y);
+                v.z = fmaf(f, v.z, fk * x.z);
+                v.w = fmaf(f, v.w, fk * x.w);
+            }
         }
-        const float inv = 1.f / l;
-        const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-        storeOut(a, p, task.seq * a.o_seq + (static_cast<long long>(kv) * a.group + head0 + h) * a.o_head + d, y);
+        if (sides > 1) {
+            part[threadIdx.x] = v;
+            part_ml[threadIdx.x] = make_float2(m, l);
+            __syncthreads();
+            if (side == 0) {
+                for (int k = 1; k < sides && k < task.pieces; ++k) {
+                    const float2 ml = part_ml[k * items + item];
+                    const float4 x = part[k * items + item];
+                    const float now = fmaxf(m, ml.x), f = exp2Fast(m - now), fk = exp2Fast(ml.x - now);
+                    m = now;
+                    l = fmaf(f, l, fk * ml.y);
+                    v.x = fmaf(f, v.x, fk * x.x);
+                    v.y = fmaf(f, v.y, fk * x.y);
+                    v.z = fmaf(f, v.z, fk * x.z);
+                    v.w = fmaf(f, v.w, fk * x.w);
+                }
+            }
+        }
+        if (live && side == 0) {
+            const float inv = 1.f / l;
+            const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+            storeOut(a, p, task.seq * a.o_seq + (static_cast<long long>(kv) * a.group + head0 + h) * a.o_head + 4 * column, y);
+        }
     }
 }
 
@@ -966,13 +1040,13 @@ using TilesKernel = void (*)(AttentionArgs, TilesArgs);
 
 struct Variant {
     TilesKernel tiles[2], combine; // blocks of 8 | 16 tokens
-    int ctas, smem, record, heads;
+    int ctas, smem, record, heads, tile;
 };
 
 template <int BITS, int HD, int HT>
 Variant variant() {
     using C = Cfg<BITS, HD, HT>;
-    return {{quantAttentionTilesKernel<BITS, HD, HT, false>, quantAttentionTilesKernel<BITS, HD, HT, true>}, quantAttentionCombineKernel<HD, HT>, C::kCtas, C::kSmem, C::kRecord, HT};
+    return {{quantAttentionTilesKernel<BITS, HD, HT, false>, quantAttentionTilesKernel<BITS, HD, HT, true>}, quantAttentionCombineKernel<HD, HT>, C::kCtas, C::kSmem, C::kRecord, HT, C::kTile};
 }
 
 template <int BITS>
@@ -1017,7 +1091,7 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     const Variant var = variantFor(I);
     const unsigned long long group = I.num_heads / P.num_kv_heads;
     const unsigned long long head_tiles = (group + var.heads - 1) / var.heads;
-    const unsigned long long tiles = (static_cast<unsigned long long>(I.max_blocks) * P.block_size + kTile - 1) / kTile;
+    const unsigned long long tiles = (static_cast<unsigned long long>(I.max_blocks) * P.block_size + var.tile - 1) / var.tile;
     const unsigned long long subs = head_tiles * P.num_kv_heads;
     const long double line = static_cast<long double>(tiles + kUnitCost) * subs * I.num_seqs;
     const unsigned long long at_most = static_cast<unsigned long long>(props.sm_count) * var.ctas;
@@ -1029,7 +1103,14 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     plan.grid = static_cast<int>(useful < at_most ? useful : at_most);
     plan.head_tiles = static_cast<int>(head_tiles);
     plan.subs = static_cast<int>(subs);
-    plan.tasks_bytes = (sizeof(Task) * plan.grid + 255) / 256 * 256;
+    const unsigned long long units = subs * I.num_seqs; // below 2^64: the line is longer
+    plan.task_of_unit = units <= static_cast<unsigned long long>(plan.grid);
+    plan.tasks = plan.task_of_unit ? static_cast<int>(units) : plan.grid;
+    // all heads of a unit in one CTA of the combine kernel, or each in its own: with few units each has many pieces
+    const int heads = static_cast<int>(group < static_cast<unsigned long long>(var.heads) ? group : var.heads);
+    plan.combine_heads = static_cast<long long>(plan.tasks) * heads > 8ll * props.sm_count ? heads : 1;
+    plan.combine_parts = heads / plan.combine_heads;
+    plan.tasks_bytes = (sizeof(Task) * plan.tasks + 255) / 256 * 256;
     plan.workspace_bytes = plan.tasks_bytes + sizeof(float) * 2 * plan.grid * static_cast<size_t>(var.record);
     // n / halves for n < 2^31 as mulhi(n, magic) >> shift: magic = floor(2^(32 + shift) / halves) + 1 with 2^shift < halves, which is
     // below 2^32 and off by at most halves, and n * halves < 2^(32 + shift); 2^(31) and one shift less for a power of two
@@ -1061,6 +1142,8 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     TilesArgs p;
     p.workspace = static_cast<unsigned char *>(workspace);
     p.tasks_bytes = static_cast<long long>(plan.tasks_bytes);
+    p.combine_heads = plan.combine_heads;
+    p.task_of_unit = plan.task_of_unit ? 1 : 0;
     p.subs = plan.subs;
     p.head_tiles = plan.head_tiles;
     p.half_magic = plan.half_magic;
@@ -1087,7 +1170,8 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     (void)cudaLaunchKernelEx(&cfg, kernel, a, p);
     const infiniStatus_t st = checkLaunch("quantAttentionTilesKernel");
     B200_RETURN_IF(st != INFINI_STATUS_SUCCESS, st);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(static_cast<unsigned>(plan.tasks), static_cast<unsigned>(plan.combine_parts));
+    cfg.blockDim = dim3(kCombineThreads);
     cfg.dynamicSmemBytes = 0;
     (void)cudaLaunchKernelEx(&cfg, var.combine, a, p);
     return checkLaunch("quantAttentionCombineKernel");
