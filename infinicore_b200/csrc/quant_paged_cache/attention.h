@@ -81,10 +81,12 @@ struct TilesPlan {
     unsigned half_magic = 0, half_self = 0; // division by block_size / 8
     int half_shift = 0;
     bool out_words = false;
+    bool unit_of_cta = false;  // no unit is cut between CTAs
     bool task_of_unit = false; // how the combine kernel's tasks are numbered
     int tasks = 0, combine_heads = 0, combine_parts = 0;
     size_t tasks_bytes = 0;
     size_t workspace_bytes = 0;
+    mutable int ready = 0; // the kernel may use its shared memory
 };
 TilesPlan planTiles(const AttentionInfo &info, const DeviceProps &props);
 bool tilesTakePointers(const TilesPlan &plan, const AttentionArgs &a, const void *workspace);

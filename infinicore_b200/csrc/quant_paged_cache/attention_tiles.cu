@@ -68,7 +68,7 @@ struct Cfg {
     static constexpr int kHeadTiles = HT / 8;
     static constexpr int kStride = HD + 4;                    // floats: rows of two heads apart hit other banks
     static constexpr int kResult = HT * kStride * 4;
-    static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes) + kThreads * 4 + 256;
+    static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes);
     // resident CTAs: what the registers of q, outputs and scales leave room for
     static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
@@ -190,6 +190,7 @@ __device__ __forceinline__ unsigned codes8(const Magic &m, unsigned flipped) {
 struct TilesArgs {
     unsigned char *workspace; // Task[] | records
     long long tasks_bytes;
+    int unit_of_cta;          // every CTA has one unit to itself: nothing to combine
     int task_of_unit;         // tasks are numbered by unit, where there are no more units than CTAs; otherwise by CTA
     int combine_heads;        // of a CTA of the combine kernel
     int subs;                 // kv heads * head tiles of a group
@@ -200,16 +201,6 @@ struct TilesArgs {
     int half_shift;
     int index_shift;          // log2 of the bytes of a table entry
     int out_words;            // rows of out can be stored 8 bytes at a time
-};
-
-struct Lens { // lengths of the sequences a CTA meets first, in shared memory
-    const AttentionArgs &a;
-    const int *cached;
-    int base;
-    __device__ __forceinline__ int operator()(int seq) const {
-        const unsigned d = static_cast<unsigned>(seq - base);
-        return d < static_cast<unsigned>(kThreads) ? cached[d] : lengthOf(a, seq);
-    }
 };
 
 template <int TILE>
@@ -228,7 +219,7 @@ struct Walk {
 
     // To the next unit: how many of its tiles are in the range (0: the range has ended).
     template <int TILE>
-    __device__ __forceinline__ int step(int subs, const Lens &lens) {
+    __device__ __forceinline__ int step(const AttentionArgs &a, int subs) {
         budget -= kUnitCost; // at or below 0: the range ends in front of the unit's first tile
         if (budget <= 0) {
             return 0;
@@ -236,7 +227,7 @@ struct Walk {
         if (++sub == subs) {
             sub = 0;
             do {
-                len = lens(++seq);
+                len = lengthOf(a, ++seq);
             } while (len <= 0);
             tiles = tilesOf<TILE>(len);
         }
@@ -287,80 +278,81 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     float2 *sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(results) + kWarps * C::kResult); // [warp][2][head]
     Piece *pieces = reinterpret_cast<Piece *>(sums + kWarps * 2 * HT);                                        // [warp][2]
     Walk *walks = reinterpret_cast<Walk *>(pieces + kWarps * 2);                                              // [warp][copies | arithmetic]
-    int *lens_s = reinterpret_cast<int *>(walks + kWarps * 2);
-    long long *plan_s = reinterpret_cast<long long *>(lens_s + kThreads); // sums of warps; then seq and position of each start
     const int tid = static_cast<int>(pinned(threadIdx.x)), warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // the ranges of this CTA's warps
-    const int per = (a.num_seqs + kThreads - 1) / kThreads;
-    long long mine = 0;
-    for (int i = 0; i < per; ++i) {
-        const int s = tid * per + i;
-        const int len = s < a.num_seqs ? lengthOf(a, s) : 0;
-        mine += costOf<TILE>(len);
-        if (per == 1) {
-            lens_s[tid] = len;
-        }
+    if (lane < 2) {
+        pieces[2 * warp + lane].used = 0;
     }
-    if (tid < kWarps * 2) {
-        pieces[tid].used = 0;
-    }
-    long long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) {
-            upto += x;
-        }
-    }
-    if (lane == 31) {
-        plan_s[warp] = upto;
-    }
-    __syncthreads();
-    long long all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        all += plan_s[w];
-        upto += w < warp ? plan_s[w] : 0;
-    }
-    const long long total = all * p.subs;
-    const int workers = static_cast<int>(gridDim.x) * kWarps;
-    long long range = (total + workers - 1) / workers;
-    range = range > kMinRange ? range : kMinRange;
-    const long long cta_range = range * kWarps, cta_start = cta_range * blockIdx.x;
+    // this warp's range
     Task *tasks = reinterpret_cast<Task *>(p.workspace);
-    if (cta_start >= total) {
-        if (tid == 0 && !p.task_of_unit) {
-            tasks[blockIdx.x].pieces = 0;
+    long long total, range; // of the line; of a warp
+    long long cta_start;
+    Walk first_walk = {};   // unit of the range's start; its position there in `budget`
+    if (p.unit_of_cta) {
+        // the line is one unit
+        first_walk.seq = static_cast<int>(blockIdx.x) / p.subs;
+        first_walk.sub = static_cast<int>(blockIdx.x) - first_walk.seq * p.subs;
+        first_walk.len = lengthOf(a, first_walk.seq);
+        total = costOf<TILE>(first_walk.len);
+        if (total == 0) {
+            return;
         }
-        return;
-    }
-    if (mine > 0) {
-#pragma unroll 1
-        for (int w = 0; w < kWarps; ++w) {
-            long long pos = cta_start + w * range - (upto - mine) * p.subs;
-            if (pos >= 0 && pos < mine * p.subs) { // one thread for each start
-                int s = tid * per;
-                long long cost = costOf<TILE>(lengthOf(a, s)) * p.subs;
-                while (pos >= cost) {
-                    pos -= cost;
-                    cost = costOf<TILE>(lengthOf(a, ++s)) * p.subs;
-                }
-                plan_s[4 + 2 * w] = s;
-                plan_s[5 + 2 * w] = pos;
+        range = (total + kWarps - 1) / kWarps;
+        range = range > kMinRange ? range : kMinRange;
+        cta_start = 0;
+        first_walk.budget = static_cast<int>(range * warp);
+    } else {
+        // every warp adds up the batch for itself: lane i has sequences i * per to (i + 1) * per - 1
+        const int per = (a.num_seqs + 31) / 32;
+        long long mine = 0;
+#pragma unroll 4
+        for (int i = 0; i < per; ++i) {
+            const int s = lane * per + i;
+            mine += s < a.num_seqs ? costOf<TILE>(lengthOf(a, s)) : 0;
+        }
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            upto += lane >= o ? x : 0;
+        }
+        total = __shfl_sync(0xffffffffu, upto, 31) * p.subs;
+        const int workers = static_cast<int>(gridDim.x) * kWarps;
+        range = (total + workers - 1) / workers;
+        range = range > kMinRange ? range : kMinRange;
+        cta_start = range * kWarps * blockIdx.x;
+        if (cta_start >= total) {
+            if (tid == 0 && !p.task_of_unit) {
+                tasks[blockIdx.x].pieces = 0;
+            }
+            return;
+        }
+        long long pos = cta_start + range * warp - (upto - mine) * p.subs; // within this lane's sequences, if not negative and before
+        const bool here = pos >= 0 && pos < mine * p.subs;                 // their end, which is so for one lane at most
+        int s = lane * per;
+        if (here) {
+            long long cost = costOf<TILE>(lengthOf(a, s)) * p.subs;
+            while (pos >= cost) {
+                pos -= cost;
+                cost = costOf<TILE>(lengthOf(a, ++s)) * p.subs;
             }
         }
+        const unsigned who = __ballot_sync(0xffffffffu, here);
+        if (who != 0) {
+            const int from = __ffs(who) - 1;
+            first_walk.seq = __shfl_sync(0xffffffffu, s, from);
+            pos = __shfl_sync(0xffffffffu, pos, from);
+            first_walk.len = lengthOf(a, first_walk.seq);
+            const long long cost = costOf<TILE>(first_walk.len);
+            first_walk.sub = static_cast<int>(pos / cost);
+            first_walk.budget = static_cast<int>(pos - first_walk.sub * cost);
+        }
     }
-    __syncthreads();
-    const Lens lens{a, lens_s, per == 1 ? 0 : static_cast<int>(plan_s[4])};
-    if (per != 1) {
-        lens_s[tid] = lens.base + tid < a.num_seqs ? lengthOf(a, lens.base + tid) : 0;
-        __syncthreads();
-    }
+    const long long cta_range = range * kWarps;
     const long long start = cta_start + warp * range, end = start + range < total ? start + range : total;
 
     unsigned char *ring = smem + warp * C::kRing;
@@ -370,13 +362,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         int tile, left;  // of the unit in work: present tile, tiles from there on in the range
         long long place; // of the present tile on the line
         {
-            Walk w;
-            w.seq = static_cast<int>(plan_s[4 + 2 * warp]);
-            w.len = lens(w.seq);
+            Walk w = first_walk;
             w.tiles = tilesOf<TILE>(w.len);
-            const long long pos = plan_s[5 + 2 * warp], cost = w.tiles + kUnitCost;
-            w.sub = static_cast<int>(pos / cost);
-            const int in = static_cast<int>(pos - w.sub * cost) - kUnitCost; // below 0: in front of the unit's first tile
+            const int in = w.budget - kUnitCost; // below 0: in front of the unit's first tile
             tile = in > 0 ? in : 0;
             place = start + (tile - in);
             const int budget = static_cast<int>(end - place);
@@ -468,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 f_half += TILE / 8;
                 if (--f_left == 0) {
                     Walk w = copies;
-                    f_left = w.step<TILE>(p.subs, lens);
+                    f_left = w.step<TILE>(a, p.subs);
                     __syncwarp();
                     copies = w;
                     __syncwarp();
@@ -824,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             const bool first = unit_first >= start, last = unit_first + done.tiles <= end;
             {
                 Walk w = done;
-                left = last ? w.step<TILE>(p.subs, lens) : 0;
+                left = last ? w.step<TILE>(a, p.subs) : 0;
                 __syncwarp();
                 work = w;
             }
@@ -841,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     inv[n][x] = 1.f / sum[n][x];
                 }
             }
-            if (first && last && lane == 0 && p.task_of_unit) {
+            if (first && last && lane == 0 && p.task_of_unit && !p.unit_of_cta) {
                 tasks[done.seq * p.subs + done.sub].pieces = 0;
             }
             if (!(first && last) && lane == 0) {
@@ -951,14 +939,14 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         }
         if (first) {
             cut = last ? 0 : static_cast<int>((piece.first + piece.tiles - 1) / cta_range - blockIdx.x) + 1;
-            if (tid == 0 && (cut > 0 || p.task_of_unit)) {
+            if (tid == 0 && !p.unit_of_cta && (cut > 0 || p.task_of_unit)) {
                 tasks[p.task_of_unit ? piece.seq * p.subs + piece.sub : static_cast<int>(blockIdx.x)] = {piece.seq, piece.sub, cut,
                                                                                                         static_cast<int>(blockIdx.x)};
             }
         }
         k = upto_k;
     }
-    if (tid == 0 && cut == 0 && !p.task_of_unit) {
+    if (tid == 0 && cut == 0 && !p.task_of_unit && !p.unit_of_cta) {
         tasks[blockIdx.x].pieces = 0;
     }
 }
@@ -1104,14 +1092,25 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     plan.head_tiles = static_cast<int>(head_tiles);
     plan.subs = static_cast<int>(subs);
     const unsigned long long units = subs * I.num_seqs; // below 2^64: the line is longer
+    // A unit to each CTA saves the combine kernel, but lets the longest unit set the time; it is for units that are known to be short
+    // and few enough to run at once.  Measured at 32/8 heads of 128 (us, a unit to each CTA | the line): 4 sequences of 256 tokens
+    // 7.6 | 11.5 at 4 bits, 8.0 | 11.5 at 8; of 1024 13.1 | 12.0, 15.4 | 12.5; 16 of 1024 13.4 | 16.4, 15.6 | 17.6; 64 of 1024
+    // at 8 bits 29 | 35; 256 of 256 (more units than fit) 48 | 35, 43 | 38.
+    const size_t longest = P.block_size * I.max_blocks;
+    plan.unit_of_cta = units <= at_most && longest <= (units >= 64 ? 1024u : 512u);
+    if (plan.unit_of_cta) {
+        plan.grid = static_cast<int>(units);
+    }
     plan.task_of_unit = units <= static_cast<unsigned long long>(plan.grid);
     plan.tasks = plan.task_of_unit ? static_cast<int>(units) : plan.grid;
     // all heads of a unit in one CTA of the combine kernel, or each in its own: with few units each has many pieces
     const int heads = static_cast<int>(group < static_cast<unsigned long long>(var.heads) ? group : var.heads);
     plan.combine_heads = static_cast<long long>(plan.tasks) * heads > 8ll * props.sm_count ? heads : 1;
     plan.combine_parts = heads / plan.combine_heads;
+    if (!plan.unit_of_cta) {
     plan.tasks_bytes = (sizeof(Task) * plan.tasks + 255) / 256 * 256;
     plan.workspace_bytes = plan.tasks_bytes + sizeof(float) * 2 * plan.grid * static_cast<size_t>(var.record);
+    }
     // n / halves for n < 2^31 as mulhi(n, magic) >> shift: magic = floor(2^(32 + shift) / halves) + 1 with 2^shift < halves, which is
     // below 2^32 and off by at most halves, and n * halves < 2^(32 + shift); 2^(31) and one shift less for a power of two
     const unsigned halves = static_cast<unsigned>(P.block_size / 8);
@@ -1143,6 +1142,7 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     p.workspace = static_cast<unsigned char *>(workspace);
     p.tasks_bytes = static_cast<long long>(plan.tasks_bytes);
     p.combine_heads = plan.combine_heads;
+    p.unit_of_cta = plan.unit_of_cta ? 1 : 0;
     p.task_of_unit = plan.task_of_unit ? 1 : 0;
     p.subs = plan.subs;
     p.head_tiles = plan.head_tiles;
@@ -1152,10 +1152,13 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     p.index_shift = a.index_is_64 ? 3 : 2;
     p.halves = static_cast<unsigned>(a.block_size / 8);
     p.out_words = plan.out_words && alignedTo(a.out, 8) ? 1 : 0;
-    // an attribute of the current device's function, so it is set for each launch
     const TilesKernel kernel = var.tiles[a.block_size % 16 == 0];
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem) != cudaSuccess) {
-        return checkLaunch("quantAttentionTilesKernel: shared memory");
+    // an attribute of the device's function: set by the descriptor's first launch
+    if (__atomic_load_n(&plan.ready, __ATOMIC_RELAXED) == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem) != cudaSuccess) {
+            return checkLaunch("quantAttentionTilesKernel: shared memory");
+        }
+        __atomic_store_n(&plan.ready, 1, __ATOMIC_RELAXED);
     }
     cudaLaunchAttribute pdl;
     pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1169,7 +1172,9 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     cfg.numAttrs = 1;
     (void)cudaLaunchKernelEx(&cfg, kernel, a, p);
     const infiniStatus_t st = checkLaunch("quantAttentionTilesKernel");
-    B200_RETURN_IF(st != INFINI_STATUS_SUCCESS, st);
+    if (st != INFINI_STATUS_SUCCESS || plan.unit_of_cta) {
+        return st;
+    }
     cfg.gridDim = dim3(static_cast<unsigned>(plan.tasks), static_cast<unsigned>(plan.combine_parts));
     cfg.blockDim = dim3(kCombineThreads);
     cfg.dynamicSmemBytes = 0;

@@ -1,11 +1,10 @@
 // infiniopQuantPagedCaching and infiniopQuantPagedCacheRead: rows of K and V into pools of 8- or 4-bit codes
 // and back.
 //
-// Both kernels give a lane eight neighbouring elements of a row (16 bytes of a 16-bit row; 8 or 4 bytes of
-// codes), a row a power of two of lanes, and let one lane move its eight elements of the K row and of the V
-// row of one (token, kv head), so that both loads are in flight before the first is used.  Consecutive lanes
-// take consecutive words, so every access of a warp covers whole rows.  A step's rows are a launch's latency;
-// a prefill's are bound by HBM.
+// Both kernels give a lane 16 neighbouring elements of a row (32 bytes of a 16-bit row in one access; 16 or 8 bytes of
+// codes), a row a power of two of lanes, and let one lane move its elements of the K row and of the V row of kTokens
+// tokens, so that all loads are in flight before the first is used.  Consecutive lanes take consecutive words, so every
+// access of a warp covers whole rows.  A step's rows are a launch's latency; a prefill's are bound by HBM.
 //
 // Quantising without a division per element: with s the group's scale, code = x / s to the nearest, halves
 // away from zero, is the nearest integer to x * r for r = (1 + 2^-21) / s rounded to fp32.  x has at most 11
@@ -42,13 +41,13 @@ struct Side { // K or V; strides of codes in bytes, of scales and rows in elemen
     long long s_block, s_head, s_slot;
     long long r_token, r_head;
     int width;  // elements of a row
-    int groups; // scales of a row
+
 };
 
 struct CachingArgs {
     Side k, v;
     const int64_t *slot_mapping;
-    long long num_pairs; // tokens * kv heads
+    long long num_tokens;
     int num_kv_heads;
     int block_size;
     int lanes_log2; // lanes of a row
@@ -64,14 +63,14 @@ __device__ __forceinline__ void gridDependency() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// The (token, kv head) of this thread's lanes, and the slot; false for nothing to do.
-__device__ __forceinline__ bool locate(const CachingArgs &a, long long &token, int &head, int &lane, long long &slot) {
+constexpr int kElems = 16; // of a lane
+
+// The first token, the kv head and the lane's place in a row; false behind the last pair.
+template <int TOKENS>
+__device__ __forceinline__ bool locate(const CachingArgs &a, long long &token, int &head, int &lane) {
     const long long thread = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-    const long long pair = thread >> a.lanes_log2;
+    const long long pair = thread >> a.lanes_log2; // (TOKENS tokens, kv head)
     lane = static_cast<int>(thread) & ((1 << a.lanes_log2) - 1);
-    if (pair >= a.num_pairs) {
-        return false;
-    }
     if (pair <= 0xffffffffLL) {
         const unsigned p = static_cast<unsigned>(pair);
         const unsigned t = p / static_cast<unsigned>(a.num_kv_heads);
@@ -81,14 +80,20 @@ __device__ __forceinline__ bool locate(const CachingArgs &a, long long &token, i
         token = pair / a.num_kv_heads;
         head = static_cast<int>(pair - token * a.num_kv_heads);
     }
-    slot = a.slot_mapping[token];
+    token *= TOKENS;
+    return token < a.num_tokens;
+}
+
+// A token's slot, negative for padding; in checked mode one outside the pool raises a flag and counts as padding.
+__device__ __forceinline__ long long slotOf(const CachingArgs &a, long long token, bool report) {
+    long long slot = a.slot_mapping[token];
     if (a.check_indices && slot >= a.num_slots) {
-        if (lane == 0 && head == 0) {
+        if (report) {
             atomicOr(a.kernel_flags, INFINIOP_KERNEL_FLAG_SLOT_OUT_OF_RANGE);
         }
         slot = -1;
     }
-    return true;
+    return slot;
 }
 
 __device__ __forceinline__ void splitSlot(const CachingArgs &a, long long slot, long long &block, long long &off) {
@@ -113,65 +118,83 @@ __device__ __forceinline__ float bitsToFloat<__nv_bfloat16>(unsigned h) {
     return __uint_as_float(h << 16);
 }
 
+struct Words { // 32 bytes
+    unsigned w[8];
+};
+
+__device__ __forceinline__ Words load32(const void *p) {
+    Words x;
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]), "=r"(x.w[4]), "=r"(x.w[5]), "=r"(x.w[6]), "=r"(x.w[7])
+                 : "l"(p));
+    return x;
+}
+
+__device__ __forceinline__ void store32(void *p, const Words &x) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(x.w[0]), "r"(x.w[1]), "r"(x.w[2]), "r"(x.w[3]), "r"(x.w[4]),
+                 "r"(x.w[5]), "r"(x.w[6]), "r"(x.w[7])
+                 : "memory");
+}
+
+// 16 elements of 16 bits
 template <bool VEC>
-__device__ __forceinline__ uint4 loadEight(const unsigned short *p) {
+__device__ __forceinline__ Words loadRow(const unsigned short *p) {
     if constexpr (VEC) {
-        return *reinterpret_cast<const uint4 *>(p);
+        return load32(p);
     } else {
-        uint4 w;
-        w.x = p[0] | (static_cast<unsigned>(p[1]) << 16);
-        w.y = p[2] | (static_cast<unsigned>(p[3]) << 16);
-        w.z = p[4] | (static_cast<unsigned>(p[5]) << 16);
-        w.w = p[6] | (static_cast<unsigned>(p[7]) << 16);
-        return w;
+        Words x;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x.w[i] = p[2 * i] | (static_cast<unsigned>(p[2 * i + 1]) << 16);
+        }
+        return x;
     }
 }
 
-// Largest magnitude among the 16-bit values of the lanes that share a scale, as the bits of a magnitude
-// (which order like the values, infinities and NaN last).
-__device__ __forceinline__ unsigned largestOf(const uint4 &w) {
+// Largest magnitude among 16-bit values, as the bits of a magnitude (which order like the values, infinities and NaN last).
+__device__ __forceinline__ unsigned largestOf(const Words &x) {
     const unsigned m = 0x7fff7fffu;
-    const unsigned a = __vmaxu2(__vmaxu2(w.x & m, w.y & m), __vmaxu2(w.z & m, w.w & m));
+    unsigned a = x.w[0] & m;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        a = __vmaxu2(a, x.w[i] & m);
+    }
     return max(a & 0xffffu, a >> 16);
 }
 
 template <int BITS, typename T, bool VEC>
-__device__ __forceinline__ void storeCodes(unsigned char *dst, const uint4 &w, float r, bool zero) {
-    const unsigned in[4] = {w.x, w.y, w.z, w.w};
-    unsigned c[8];
+__device__ __forceinline__ void storeCodes(unsigned char *dst, const Words &x, float r, bool zero) {
+    constexpr int kWords = BITS / 2; // 16 codes
+    unsigned out[kWords];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        c[2 * i] = __float_as_uint(fmaf(bitsToFloat<T>(in[i] & 0xffffu), r, 12582912.f));
-        c[2 * i + 1] = __float_as_uint(fmaf(bitsToFloat<T>(in[i] >> 16), r, 12582912.f));
+    for (int k = 0; k < kWords; ++k) {
+        constexpr int kPer = 32 / BITS;
+        unsigned c[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int e = k * kPer + i;
+            const unsigned half = e & 1 ? x.w[e / 2] >> 16 : x.w[e / 2] & 0xffffu;
+            c[i] = __float_as_uint(fmaf(bitsToFloat<T>(half), r, 12582912.f));
+        }
+        if constexpr (BITS == 8) {
+            out[k] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        } else {
+            out[k] = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                out[k] |= (c[i] & 15u) << (4 * i);
+            }
+        }
+        out[k] = zero ? 0u : out[k];
     }
-    if constexpr (BITS == 8) {
-        unsigned lo = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-        unsigned hi = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-        lo = zero ? 0u : lo;
-        hi = zero ? 0u : hi;
-        if constexpr (VEC) {
-            *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                dst[i] = static_cast<unsigned char>(lo >> (8 * i));
-                dst[4 + i] = static_cast<unsigned char>(hi >> (8 * i));
-            }
-        }
+    if constexpr (VEC && BITS == 8) {
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+    } else if constexpr (VEC) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(out[0], out[1]);
     } else {
-        unsigned word = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            word |= (c[i] & 15u) << (4 * i);
-        }
-        word = zero ? 0u : word;
-        if constexpr (VEC) {
-            *reinterpret_cast<unsigned *>(dst) = word;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                dst[i] = static_cast<unsigned char>(word >> (8 * i));
-            }
+        for (int i = 0; i < 4 * kWords; ++i) {
+            dst[i] = static_cast<unsigned char>(out[i / 4] >> (8 * (i % 4)));
         }
     }
 }
@@ -192,190 +215,216 @@ __device__ __forceinline__ unsigned short scaleOf(unsigned largest, float &r, bo
     return bits;
 }
 
-// NV: vectors of eight elements a lane has of a row (1 up to 256 elements, 4 up to 1024).
+// NV: vectors of 16 elements a lane has of a row (1 up to 512 elements, 2 up to 1024).  All lanes of a warp come here;
+// `live`: whether this row is written.
 template <int BITS, typename T, int NV, bool VEC>
-__device__ __forceinline__ void writeRow(const Side &s, const uint4 (&w)[NV], long long block, int head, long long off, int lane, int lanes,
-                                         unsigned mask) {
+__device__ __forceinline__ void writeRow(const Side &s, const Words (&x)[NV], bool live, long long block, int head, long long off, int lane, int lanes) {
     unsigned char *codes = static_cast<unsigned char *>(s.codes) + block * s.block + head * s.head + off * s.slot;
     unsigned short *scales = static_cast<unsigned short *>(s.scales) + block * s.s_block + head * s.s_head + off * s.s_slot;
-    constexpr int kBytes = BITS; // codes of eight elements
+    unsigned whole = 0;
     if constexpr (BITS == 8) {
-        unsigned m = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            m = max(m, largestOf(w[i])); // vectors beyond the row hold zeros
+            whole = max(whole, largestOf(x[i])); // vectors beyond the row hold zeros
         }
         for (int o = 1; o < lanes; o <<= 1) {
-            m = max(m, __shfl_xor_sync(mask, m, o));
+            whole = max(whole, __shfl_xor_sync(0xffffffffu, whole, o));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        unsigned m = whole;
+        if constexpr (BITS == 4) {
+            m = largestOf(x[i]);
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1)); // a group is two lanes
         }
         float r;
         bool zero;
         const unsigned short bits = scaleOf<BITS, T>(m, r, zero);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = 8 * (lane + i * lanes);
-            if (e < s.width) {
-                storeCodes<BITS, T, VEC>(codes + (lane + i * lanes) * kBytes, w[i], r, zero);
-            }
-        }
-        if (lane == 0) {
-            scales[0] = bits;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            unsigned m = largestOf(w[i]);
-            m = max(m, __shfl_xor_sync(mask, m, 1));
-            m = max(m, __shfl_xor_sync(mask, m, 2));
-            float r;
-            bool zero;
-            const unsigned short bits = scaleOf<BITS, T>(m, r, zero);
-            const int vec = lane + i * lanes;
-            if (8 * vec < s.width) {
-                storeCodes<BITS, T, VEC>(codes + vec * kBytes, w[i], r, zero);
-                if ((vec & 3) == 0) {
-                    scales[vec >> 2] = bits;
-                }
+        const int vec = lane + i * lanes;
+        if (live && kElems * vec < s.width) {
+            storeCodes<BITS, T, VEC>(codes + vec * (2 * BITS), x[i], r, zero);
+            if (BITS == 8 ? vec == 0 : (vec & 1) == 0) {
+                scales[BITS == 8 ? 0 : vec >> 1] = bits;
             }
         }
     }
 }
 
-template <int BITS, typename T, int NV, bool VEC>
+template <int BITS, typename T, int NV, bool VEC, int TOKENS>
 __global__ void __launch_bounds__(kThreads) quantPagedCachingKernel(const CachingArgs a) {
     gridDependency();
-    long long token, slot;
+    long long token0;
     int head, lane;
-    const bool mine = locate(a, token, head, lane, slot) && slot >= 0;
-    // whole rows leave together: the lanes of a row are neighbours in one warp and agree on `mine`
-    const unsigned mask = __ballot_sync(0xffffffffu, mine);
-    if (!mine) {
-        return;
-    }
+    const bool any = locate<TOKENS>(a, token0, head, lane);
     const int lanes = 1 << a.lanes_log2;
-    const unsigned short *k = static_cast<const unsigned short *>(a.k.rows) + token * a.k.r_token + head * a.k.r_head;
-    const unsigned short *v = static_cast<const unsigned short *>(a.v.rows) + token * a.v.r_token + head * a.v.r_head;
-    uint4 kw[NV], vw[NV];
+    long long slot[TOKENS];
+    Words k[TOKENS][NV], v[TOKENS][NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int e = 8 * (lane + i * lanes);
-        kw[i] = e < a.k.width ? loadEight<VEC>(k + e) : make_uint4(0, 0, 0, 0);
-        vw[i] = e < a.v.width ? loadEight<VEC>(v + e) : make_uint4(0, 0, 0, 0);
+    for (int u = 0; u < TOKENS; ++u) {
+        const long long token = token0 + u;
+        const bool here = any && token < a.num_tokens;
+        slot[u] = here ? slotOf(a, token, lane == 0 && head == 0) : -1;
+        const unsigned short *kr = static_cast<const unsigned short *>(a.k.rows) + token * a.k.r_token + head * a.k.r_head;
+        const unsigned short *vr = static_cast<const unsigned short *>(a.v.rows) + token * a.v.r_token + head * a.v.r_head;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) { // rows of padding too: the slot need not have come
+            const int e = kElems * (lane + i * lanes);
+            k[u][i] = v[u][i] = Words{};
+            if (here && e < a.k.width) {
+                k[u][i] = loadRow<VEC>(kr + e);
+            }
+            if (here && e < a.v.width) {
+                v[u][i] = loadRow<VEC>(vr + e);
+            }
+        }
     }
-    long long block, off;
-    splitSlot(a, slot, block, off);
-    writeRow<BITS, T, NV, VEC>(a.k, kw, block, head, off, lane, lanes, mask);
-    writeRow<BITS, T, NV, VEC>(a.v, vw, block, head, off, lane, lanes, mask);
+#pragma unroll
+    for (int u = 0; u < TOKENS; ++u) {
+        long long block = 0, off = 0;
+        if (slot[u] >= 0) {
+            splitSlot(a, slot[u], block, off);
+        }
+        writeRow<BITS, T, NV, VEC>(a.k, k[u], slot[u] >= 0, block, head, off, lane, lanes);
+        writeRow<BITS, T, NV, VEC>(a.v, v[u], slot[u] >= 0, block, head, off, lane, lanes);
+    }
 }
 
 // ---- reading back ------------------------------------------------------------------------------------------
 
 template <typename T>
-__device__ __forceinline__ T roundTo(float v);
+__device__ __forceinline__ unsigned roundPair(float lo, float hi);
 template <>
-__device__ __forceinline__ float roundTo<float>(float v) { return v; }
+__device__ __forceinline__ unsigned roundPair<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
 template <>
-__device__ __forceinline__ __half roundTo<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 roundTo<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ unsigned roundPair<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
 
-// Eight codes: one or two words.
+// 16 codes: two or four words.
 template <int BITS, bool VEC>
-__device__ __forceinline__ uint2 loadCodes(const unsigned char *p) {
-    uint2 w = make_uint2(0, 0);
-    if constexpr (BITS == 8) {
-        if constexpr (VEC) {
-            w = *reinterpret_cast<const uint2 *>(p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w.x |= static_cast<unsigned>(p[i]) << (8 * i);
-                w.y |= static_cast<unsigned>(p[4 + i]) << (8 * i);
-            }
-        }
+__device__ __forceinline__ void loadCodes(unsigned (&w)[BITS / 2], const unsigned char *p) {
+    if constexpr (VEC && BITS == 8) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(p);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (VEC) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p);
+        w[0] = x.x, w[1] = x.y;
     } else {
-        if constexpr (VEC) {
-            w.x = *reinterpret_cast<const unsigned *>(p);
-        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w.x |= static_cast<unsigned>(p[i]) << (8 * i);
-            }
+        for (int i = 0; i < BITS / 2; ++i) {
+            w[i] = p[4 * i] | (static_cast<unsigned>(p[4 * i + 1]) << 8) | (static_cast<unsigned>(p[4 * i + 2]) << 16)
+                 | (static_cast<unsigned>(p[4 * i + 3]) << 24);
         }
     }
-    return w;
 }
 
 template <int BITS, typename T, bool VEC>
-__device__ __forceinline__ void storeValues(T *dst, uint2 codes, float s) {
-    T out[8];
+__device__ __forceinline__ void storeValues(T *dst, const unsigned (&codes)[BITS / 2], float s) {
+    float v[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        int c;
-        if constexpr (BITS == 8) {
-            c = static_cast<int>((i < 4 ? codes.x : codes.y) << (24 - 8 * (i & 3))) >> 24;
-        } else {
-            c = static_cast<int>(codes.x << (28 - 4 * i)) >> 28;
-        }
-        out[i] = roundTo<T>(static_cast<float>(c) * s); // the product has at most 15 bits: one rounding
+    for (int e = 0; e < 16; ++e) {
+        constexpr int kPer = 32 / BITS;
+        const int c = static_cast<int>(codes[e / kPer] << (32 - BITS - BITS * (e % kPer))) >> (32 - BITS);
+        v[e] = static_cast<float>(c) * s; // at most 15 bits: rounded once, below
     }
-    if constexpr (VEC) {
-        constexpr int kWords = 8 * sizeof(T) / 16;
-        uint4 w[kWords];
-        memcpy(w, out, sizeof(out));
+    if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            reinterpret_cast<uint4 *>(dst)[i] = w[i];
+        for (int h = 0; h < 2; ++h) {
+            Words x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x.w[i] = __float_as_uint(v[8 * h + i]);
+            }
+            if constexpr (VEC) {
+                store32(dst + 8 * h, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    dst[8 * h + i] = v[8 * h + i];
+                }
+            }
         }
     } else {
+        Words x;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            dst[i] = out[i];
+            x.w[i] = roundPair<T>(v[2 * i], v[2 * i + 1]);
+        }
+        if constexpr (VEC) {
+            store32(dst, x);
+        } else {
+            unsigned short *p = reinterpret_cast<unsigned short *>(dst);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p[i] = static_cast<unsigned short>(x.w[i / 2] >> (16 * (i & 1)));
+            }
         }
     }
 }
 
-template <int BITS, typename T, int NV, bool VEC>
+template <int BITS, typename T, int NV, bool VEC, int TOKENS>
 __global__ void __launch_bounds__(kThreads) quantPagedCacheReadKernel(const CachingArgs a) {
     gridDependency();
-    long long token, slot;
+    long long token0;
     int head, lane;
-    if (!locate(a, token, head, lane, slot)) {
+    if (!locate<TOKENS>(a, token0, head, lane)) {
         return;
     }
     const int lanes = 1 << a.lanes_log2;
-    long long block = 0, off = 0;
-    if (slot >= 0) {
-        splitSlot(a, slot, block, off);
+    long long slot[TOKENS];
+#pragma unroll
+    for (int u = 0; u < TOKENS; ++u) {
+        slot[u] = token0 + u < a.num_tokens ? slotOf(a, token0 + u, lane == 0 && head == 0) : -1;
     }
     const Side *const sides[2] = {&a.k, &a.v};
-    uint2 codes[2][NV];
-    float scale[2][NV];
+    unsigned codes[TOKENS][2][NV][BITS / 2];
+    unsigned scale[TOKENS][2][NV];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const Side &s = *sides[x];
-        const unsigned char *c = static_cast<const unsigned char *>(s.codes) + block * s.block + head * s.head + off * s.slot;
-        const unsigned short *f = static_cast<const unsigned short *>(s.scales) + block * s.s_block + head * s.s_head + off * s.s_slot;
+    for (int u = 0; u < TOKENS; ++u) {
+        long long block = 0, off = 0;
+        if (slot[u] >= 0) {
+            splitSlot(a, slot[u], block, off);
+        }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int vec = lane + i * lanes;
-            codes[x][i] = make_uint2(0, 0);
-            scale[x][i] = 0.f;
-            if (slot >= 0 && 8 * vec < s.width) {
-                codes[x][i] = loadCodes<BITS, VEC>(c + vec * BITS);
-                scale[x][i] = bitsToFloat<__nv_bfloat16>(f[BITS == 8 ? 0 : vec >> 2]);
+        for (int x = 0; x < 2; ++x) {
+            const Side &s = *sides[x];
+            const unsigned char *c = static_cast<const unsigned char *>(s.codes) + block * s.block + head * s.head + off * s.slot;
+            const unsigned short *f = static_cast<const unsigned short *>(s.scales) + block * s.s_block + head * s.s_head + off * s.s_slot;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int vec = lane + i * lanes;
+#pragma unroll
+                for (int k = 0; k < BITS / 2; ++k) {
+                    codes[u][x][i][k] = 0;
+                }
+                scale[u][x][i] = 0;
+                if (slot[u] >= 0 && kElems * vec < s.width) {
+                    loadCodes<BITS, VEC>(codes[u][x][i], c + vec * (2 * BITS));
+                    scale[u][x][i] = f[BITS == 8 ? 0 : vec >> 1];
+                }
             }
         }
     }
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const Side &s = *sides[x];
-        T *rows = static_cast<T *>(s.rows) + token * s.r_token + head * s.r_head;
+    for (int u = 0; u < TOKENS; ++u) {
+        if (token0 + u >= a.num_tokens) {
+            break;
+        }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int vec = lane + i * lanes;
-            if (8 * vec < s.width) {
-                storeValues<BITS, T, VEC>(rows + 8 * vec, codes[x][i], scale[x][i]);
+        for (int x = 0; x < 2; ++x) {
+            const Side &s = *sides[x];
+            T *rows = static_cast<T *>(s.rows) + (token0 + u) * s.r_token + head * s.r_head;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int vec = lane + i * lanes;
+                if (kElems * vec < s.width) {
+                    storeValues<BITS, T, VEC>(rows + kElems * vec, codes[u][x][i], bitsToFloat<__nv_bfloat16>(scale[u][x][i]));
+                }
             }
         }
     }
@@ -410,38 +459,46 @@ static infiniStatus_t create(CachingDescriptor **out, b200::Handle *h, OpKind ki
     return INFINI_STATUS_SUCCESS;
 }
 
-// Whether codes, scales and rows of one side can be moved in whole vectors of eight elements.
+// Whether codes and rows of one side can be moved in whole vectors of 16 elements.
 static bool vectors(const Side &s, int bits, size_t row_elem) {
     auto ok = [](long long stride, long long bytes, long long unit) { return (stride * bytes) % unit == 0; };
     const long long e = static_cast<long long>(row_elem);
-    return alignedTo(s.codes, bits) && ok(s.block, 1, bits) && ok(s.head, 1, bits) && ok(s.slot, 1, bits)
-        && alignedTo(s.rows, 16) && ok(s.r_token, e, 16) && ok(s.r_head, e, 16);
+    const int codes = 2 * bits;
+    return alignedTo(s.codes, codes) && ok(s.block, 1, codes) && ok(s.head, 1, codes) && ok(s.slot, 1, codes)
+        && alignedTo(s.rows, 32) && ok(s.r_token, e, 32) && ok(s.r_head, e, 32);
 }
 
 using Kernel = void (*)(CachingArgs);
 
-template <int BITS, typename T>
-static Kernel pick(bool read, int nv, bool vec) {
-    if (read) {
-        return nv == 1 ? (vec ? quantPagedCacheReadKernel<BITS, T, 1, true> : quantPagedCacheReadKernel<BITS, T, 1, false>)
-                       : (vec ? quantPagedCacheReadKernel<BITS, T, 4, true> : quantPagedCacheReadKernel<BITS, T, 4, false>);
-    }
-    if constexpr (!std::is_same<T, float>::value) {
-        return nv == 1 ? (vec ? quantPagedCachingKernel<BITS, T, 1, true> : quantPagedCachingKernel<BITS, T, 1, false>)
-                       : (vec ? quantPagedCachingKernel<BITS, T, 4, true> : quantPagedCachingKernel<BITS, T, 4, false>);
+// Several tokens a lane where there are enough to fill the machine and rows are one vector a lane.
+constexpr int kTokens = 2;
+
+template <int BITS, typename T, bool READ>
+static Kernel pick(int nv, bool vec, bool many) {
+    if constexpr (READ) {
+        return nv > 1 ? (vec ? quantPagedCacheReadKernel<BITS, T, 2, true, 1> : quantPagedCacheReadKernel<BITS, T, 2, false, 1>)
+             : !vec   ? quantPagedCacheReadKernel<BITS, T, 1, false, 1>
+                      : (many ? quantPagedCacheReadKernel<BITS, T, 1, true, kTokens> : quantPagedCacheReadKernel<BITS, T, 1, true, 1>);
     } else {
-        return nullptr;
+        return nv > 1 ? (vec ? quantPagedCachingKernel<BITS, T, 2, true, 1> : quantPagedCachingKernel<BITS, T, 2, false, 1>)
+             : !vec   ? quantPagedCachingKernel<BITS, T, 1, false, 1>
+                      : (many ? quantPagedCachingKernel<BITS, T, 1, true, kTokens> : quantPagedCachingKernel<BITS, T, 1, true, 1>);
     }
 }
 
-template <typename T>
-static Kernel pick(bool read, int bits, int nv, bool vec) {
-    return bits == 4 ? pick<4, T>(read, nv, vec) : pick<8, T>(read, nv, vec);
+template <int BITS>
+static Kernel pick(infiniDtype_t dtype, bool read, int nv, bool vec, bool many) {
+    if (dtype == INFINI_DTYPE_F32) { // reading only
+        return pick<BITS, float, true>(nv, vec, many);
+    }
+    if (dtype == INFINI_DTYPE_F16) {
+        return read ? pick<BITS, __half, true>(nv, vec, many) : pick<BITS, __half, false>(nv, vec, many);
+    }
+    return read ? pick<BITS, __nv_bfloat16, true>(nv, vec, many) : pick<BITS, __nv_bfloat16, false>(nv, vec, many);
 }
 
 static Side side(const Pool &p, void *codes, void *scales, void *rows, ptrdiff_t token, ptrdiff_t head) {
-    return {codes,  scales, rows, p.block, p.kv_head, p.slot, p.s_block, p.s_head, p.s_slot, token, head, static_cast<int>(p.head),
-            static_cast<int>(p.groups)};
+    return {codes,  scales, rows, p.block, p.kv_head, p.slot, p.s_block, p.s_head, p.s_slot, token, head, static_cast<int>(p.head)};
 }
 
 static infiniStatus_t launch(const CachingDescriptor &d, void *k_cache, void *v_cache, void *k_scales, void *v_scales, void *k, void *v,
@@ -452,7 +509,7 @@ static infiniStatus_t launch(const CachingDescriptor &d, void *k_cache, void *v_
     a.k = side(P.k, k_cache, k_scales, k, d.k_token, d.k_head);
     a.v = side(P.v, v_cache, v_scales, v, d.v_token, d.v_head);
     a.slot_mapping = static_cast<const int64_t *>(slots);
-    a.num_pairs = static_cast<long long>(d.num_tokens) * static_cast<long long>(P.num_kv_heads);
+    a.num_tokens = static_cast<long long>(d.num_tokens);
     a.num_kv_heads = static_cast<int>(P.num_kv_heads);
     a.block_size = static_cast<int>(P.block_size);
     a.kernel_flags = d.base.props->kernel_flags;
@@ -460,19 +517,21 @@ static infiniStatus_t launch(const CachingDescriptor &d, void *k_cache, void *v_
     a.check_indices = (d.check_indices && a.kernel_flags != nullptr) ? 1 : 0;
 
     const int widest = a.k.width > a.v.width ? a.k.width : a.v.width;
-    a.lanes_log2 = 2; // a group of 32 elements is four lanes
-    while (a.lanes_log2 < 5 && (8 << a.lanes_log2) < widest) {
+    a.lanes_log2 = 1; // a group of 32 elements is two lanes
+    while (a.lanes_log2 < 5 && (kElems << a.lanes_log2) < widest) {
         ++a.lanes_log2;
     }
-    const int nv = widest <= 256 ? 1 : 4;
+    const int nv = widest <= 32 * kElems ? 1 : 2;
     const size_t elem = dtypeSize(d.dtype);
     const bool vec = vectors(a.k, P.bits, elem) && vectors(a.v, P.bits, elem);
-    const long long blocks = ((a.num_pairs << a.lanes_log2) + kThreads - 1) / kThreads;
+    const long long pairs = a.num_tokens * static_cast<long long>(P.num_kv_heads);
+    const bool many = nv == 1 && vec && (pairs << a.lanes_log2) >= 2048ll * d.base.props->sm_count;
+    const int tokens = many ? kTokens : 1;
+    const long long threads = ((a.num_tokens + tokens - 1) / tokens * static_cast<long long>(P.num_kv_heads)) << a.lanes_log2;
+    const long long blocks = (threads + kThreads - 1) / kThreads;
     B200_RETURN_IF(blocks > 0x7fffffffLL, INFINI_STATUS_BAD_TENSOR_SHAPE);
 
-    const Kernel kernel = d.dtype == INFINI_DTYPE_F16    ? pick<__half>(read, P.bits, nv, vec)
-                        : d.dtype == INFINI_DTYPE_BF16 ? pick<__nv_bfloat16>(read, P.bits, nv, vec)
-                                                       : pick<float>(read, P.bits, nv, vec);
+    const Kernel kernel = P.bits == 4 ? pick<4>(d.dtype, read, nv, vec, many) : pick<8>(d.dtype, read, nv, vec, many);
     cudaLaunchAttribute pdl;
     pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl.val.programmaticStreamSerializationAllowed = d.use_pdl ? 1 : 0;

@@ -398,25 +398,15 @@ def paged_caching(k_cache, v_cache, k, v, slot_mapping):
 # These calls are a decode step's smallest, so their way to the library is short: the cache key is made of the
 # tensors' own metadata objects, and the device is switched only where it is not the current one.
 
-def _one_device(*tensors):
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _one_device(tensors):
     dev = tensors[0].get_device()
     for t in tensors:
-        if t.get_device() != dev or dev < 0:
+        if t is not None and (t.get_device() != dev or dev < 0):
             return _require_cuda(*tensors)  # says what is wrong
     return dev
-
-
-def _quant_entry(dev, op, tensors, extra=()):
-    """The cached descriptor of `op` for these tensors (None where an optional one is left out)."""
-    key = (op, extra, *[(t.dtype, t.shape, t.stride()) if t is not None else None for t in tensors])
-    per_dev = getattr(_tls, "per_dev", None)
-    st = per_dev.get(dev) if per_dev is not None else None
-    entry = st["cache"].get(key) if st is not None else None
-    if entry is not None:
-        st["cache"].move_to_end(key)
-        return st, entry
-    st = _state(dev)
-    return st, _lookup(st, key, lambda: _make_quant(st, op, tensors, extra))
 
 
 def _make_quant(st, op, tensors, extra):
@@ -435,19 +425,43 @@ def _make_quant(st, op, tensors, extra):
             "destroy": getattr(LIBINFINIOP, f"infiniopDestroy{op}Descriptor")}
 
 
-def _run_quant(dev, op, tensors, extra=()):
-    st, entry = _quant_entry(dev, op, tensors, extra)
+def _run_quant(op, tensors, extra=()):
+    """Runs `op` on these tensors (None where an optional one is left out), its descriptor from the cache."""
+    dev = _one_device(tensors)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _run_quant(dev, op, tensors, extra)
-    need, ws = entry["workspace"], None
+            return _run_quant(op, tensors, extra)
+    key = [op, extra]
+    pointers = []
+    for t in tensors:
+        if t is None:
+            key.append(None)
+            pointers.append(None)
+        else:
+            key += (t.dtype, t.shape, t.stride())
+            pointers.append(t.data_ptr())
+    key = tuple(key)
+    per_dev = getattr(_tls, "per_dev", None)
+    st = per_dev.get(dev) if per_dev is not None else None
+    entry = st["cache"].get(key) if st is not None else None
+    if entry is not None:
+        st["cache"].move_to_end(key)
+    else:
+        st = _state(dev)
+        entry = _lookup(st, key, lambda: _make_quant(st, op, tensors, extra))
+    need, ws, stream = entry["workspace"], None, _raw_stream(dev)
     if need:
         # a captured call gets scratch of its own graph's memory: two graphs may be replayed at the same time
-        buf = (torch.empty(need, dtype=torch.uint8, device=f"cuda:{dev}") if torch.cuda.is_current_stream_capturing()
-               else _workspace(st, need, dev))
+        if torch.cuda.is_current_stream_capturing():
+            buf = torch.empty(need, dtype=torch.uint8, device=f"cuda:{dev}")
+        else:
+            buf = st["workspace"].get(stream)
+            if buf is None or buf.numel() < need:
+                buf = _workspace(st, need, dev)
         ws = buf.data_ptr()
-    check_error(entry["run"](entry["desc"], ws, need, *[t.data_ptr() if t is not None else None for t in tensors],
-                             torch.cuda.current_stream(dev).cuda_stream))
+    status = entry["run"](entry["desc"], ws, need, *pointers, stream)
+    if status:
+        check_error(status)
 
 
 def quant_paged_caching(k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping):
@@ -459,7 +473,7 @@ def quant_paged_caching(k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping
     bfloat16 and the codes x / scale, to the nearest, halves away from zero; one with an infinity or NaN reads back
     as NaN.  Returns (k_cache, v_cache, k_scales, v_scales)."""
     tensors = (k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping)
-    _run_quant(_one_device(*tensors), "QuantPagedCaching", tensors)
+    _run_quant("QuantPagedCaching", tensors)
     return (k_cache, v_cache, k_scales, v_scales)
 
 
@@ -468,12 +482,12 @@ def quant_paged_cache_read(k_cache, v_cache, k_scales, v_scales, slot_mapping, d
     allowed; zeros where negative) of pools that quant_paged_caching wrote, as dense rows k [num_tokens, num_kv_heads,
     k head size] and v.  `out`: a pair of tensors to write instead of new ones (their dtype counts).  Returns (k, v)."""
     if out is None:
-        packed = 2 if k_cache.dtype == torch.uint8 else 1
-        out = tuple(torch.empty((slot_mapping.shape[0], c.shape[1], c.shape[3] * packed), dtype=dtype, device=c.device)
-                    for c in (k_cache, v_cache))
+        tokens, heads, packed = slot_mapping.shape[0], k_cache.shape[1], 2 if k_cache.dtype == torch.uint8 else 1
+        out = (k_cache.new_empty((tokens, heads, k_cache.shape[3] * packed), dtype=dtype),
+               v_cache.new_empty((tokens, heads, v_cache.shape[3] * packed), dtype=dtype))
     k, v = out
     tensors = (k, v, k_cache, v_cache, k_scales, v_scales, slot_mapping)
-    _run_quant(_one_device(*tensors), "QuantPagedCacheRead", tensors)
+    _run_quant("QuantPagedCacheRead", tensors)
     return (k, v)
 
 
@@ -486,6 +500,5 @@ def quant_paged_attention(q, k_cache, v_cache, k_scales, v_scales, block_tables,
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     tensors = (out, q, k_cache, v_cache, k_scales, v_scales, block_tables, cache_lens, alibi_slopes)
-    dev = _one_device(*(tensors if alibi_slopes is not None else tensors[:-1]))
-    _run_quant(dev, "QuantPagedAttention", tensors, (float(scale),))
+    _run_quant("QuantPagedAttention", tensors, (float(scale),))
     return out
