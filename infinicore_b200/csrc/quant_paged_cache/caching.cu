@@ -6,13 +6,12 @@
 // tokens, so that all loads are in flight before the first is used.  Consecutive lanes take consecutive words, so every
 // access of a warp covers whole rows.  A step's rows are a launch's latency; a prefill's are bound by HBM.
 //
-// Quantising without a division per element: with s the group's scale, code = x / s to the nearest, halves
-// away from zero, is the nearest integer to x * r for r = (1 + 2^-21) / s rounded to fp32.  x has at most 11
-// significant bits and s 8, so x / s is either exactly k + 1/2 or at least 2^-16 (relative) away from it: with
-// 2x = X 2^a and (2k + 1) s = Y 2^b, X < 2^12, Y < 2^16, the difference is a multiple of the smaller power.
-// x * r is above x / s in magnitude by a relative 2^-21 +- 2^-22, which moves an exact half up and carries
-// nothing else across a half.  The sum fma(x, r, 1.5 * 2^23) then rounds once, to the nearest integer, and
-// leaves it in the low bits of the float.
+// Quantising without a division per element: with s the group's scale, code = x / s to the nearest, halves away from
+// zero, is the nearest integer to x * r for r = (1 + 2^-21) / s to 1.5 ulp.  x has at most 11 significant bits and s 8, so
+// x / s is either exactly k + 1/2 or at least 2^-16 (relative) away from it: with 2x = X 2^a and (2k + 1) s = Y 2^b,
+// X < 2^11, Y < 2^16, the difference is a multiple of the smaller power.  x * r is above x / s in magnitude by a relative
+// 2^-21 +- 2^-22, which moves an exact half up and carries nothing else across a half.  The sum fma(x, r, 1.5 * 2^23) then
+// rounds once, to the nearest integer, and leaves it in the low bits of the float.
 #include "quant_pool.h"
 
 #include <cuda_bf16.h>
@@ -164,28 +163,23 @@ __device__ __forceinline__ unsigned largestOf(const Words &x) {
 
 template <int BITS, typename T, bool VEC>
 __device__ __forceinline__ void storeCodes(unsigned char *dst, const Words &x, float r, bool zero) {
-    constexpr int kWords = BITS / 2; // 16 codes
+    constexpr int kWords = BITS / 2, kPer = 32 / BITS; // 16 codes
+    constexpr unsigned kOne = 1u << BITS;
+    // a word is sum_i (code_i + half a field) * field^i, which has no borrows, and every field's top bit flipped; the codes come as
+    // the bits of 1.5 * 2^23 + code
+    constexpr unsigned kOnes = 0xffffffffu / (kOne - 1), kTops = kOnes << (BITS - 1);
+    constexpr unsigned kAdd = kTops - 0x4b400000u * kOnes;
     unsigned out[kWords];
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
-        constexpr int kPer = 32 / BITS;
-        unsigned c[kPer];
+        unsigned word = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
+        for (int i = kPer - 1; i >= 0; --i) {
             const int e = k * kPer + i;
             const unsigned half = e & 1 ? x.w[e / 2] >> 16 : x.w[e / 2] & 0xffffu;
-            c[i] = __float_as_uint(fmaf(bitsToFloat<T>(half), r, 12582912.f));
+            word = word * kOne + __float_as_uint(fmaf(bitsToFloat<T>(half), r, 12582912.f));
         }
-        if constexpr (BITS == 8) {
-            out[k] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-        } else {
-            out[k] = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                out[k] |= (c[i] & 15u) << (4 * i);
-            }
-        }
-        out[k] = zero ? 0u : out[k];
+        out[k] = zero ? 0u : (word + kAdd) ^ kTops;
     }
     if constexpr (VEC && BITS == 8) {
         *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
@@ -203,7 +197,11 @@ __device__ __forceinline__ void storeCodes(unsigned char *dst, const Words &x, f
 template <int BITS, typename T>
 __device__ __forceinline__ unsigned short scaleOf(unsigned largest, float &r, bool &zero) {
     constexpr unsigned kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    const float s = __fdiv_rn(bitsToFloat<T>(largest), BITS == 8 ? 127.f : 7.f);
+    // A / Q to bf16.  A has at most 11 bits, so A / Q is a relative 2^-12 or more away from the middle of two neighbouring bf16, or on
+    // it (Q = 7 and fp16 only); the residual makes a quotient that fits fp32 exact.
+    constexpr float kQ = BITS == 8 ? 127.f : 7.f, kInverse = 1.f / kQ;
+    const float largest_f = bitsToFloat<T>(largest), about = largest_f * kInverse;
+    const float s = fmaf(fmaf(-about, kQ, largest_f), kInverse, about);
     unsigned short bits = __bfloat16_as_ushort(__float2bfloat16_rn(s));
     if (largest >= kInf) {
         bits = 0x7fffu; // NaN
@@ -211,7 +209,9 @@ __device__ __forceinline__ unsigned short scaleOf(unsigned largest, float &r, bo
         bits = 0; // below 2^-126
     }
     zero = bits == 0 || largest >= kInf;
-    r = zero ? 0.f : __frcp_rn(__uint_as_float(static_cast<unsigned>(bits) << 16)) * (1.f + 4.76837158203125e-7f);
+    float inverse; // to 1 ulp
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(__uint_as_float(static_cast<unsigned>(bits) << 16)));
+    r = inverse * (1.f + 4.76837158203125e-7f); // not used where the codes are 0
     return bits;
 }
 

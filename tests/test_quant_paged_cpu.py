@@ -230,19 +230,34 @@ def test_a_value_is_half_a_step_from_what_it_stands_for(bits, dtype):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+def test_the_scale_by_a_product_is_the_definition(bits):
+    """The kernel's scale is bf16(fma(fma(-t, Q, A), i, t)) with t = A i, i = fp32(1 / Q): the same bf16 as A / Q for every 11-bit A."""
+    q = torch.tensor(float(qh.limits(bits)))
+    i = (1.0 / q.double()).float()
+    a = torch.arange(1024, 2048).float()
+    t = a * i
+    residual = (a.double() - t.double() * q.double()).float()     # exact in 53 bits, and one rounding as an fma has
+    s = (residual.double() * i.double() + t.double()).float()
+    assert torch.equal(s.to(torch.bfloat16), (a / q).to(torch.bfloat16))
+    assert torch.equal((a.double() / q.double()).float().to(torch.bfloat16), (a / q).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 def test_the_rounding_by_a_reciprocal_is_the_definition(bits):
-    """The kernel rounds fma(x, r, 1.5 * 2^23) with r = fp32(fp32(1 / s) (1 + 2^-21)) instead of dividing.  Here the same
-    arithmetic in fp32 on every bf16 scale mantissa and every fp16 mantissa below the limit gives the codes of the
-    definition, exact halves included."""
+    """The kernel rounds fma(x, r, 1.5 * 2^23) with r = fp32(i (1 + 2^-21)), i = 1 / s to 1 ulp, instead of dividing.  Here the
+    same arithmetic in fp32 on every bf16 scale significand and every fp16 significand below the limit gives the codes of the
+    definition, exact halves included, with i rounded either way."""
     q = qh.limits(bits)
     s = (torch.arange(128, 256).double() / 128).float()                      # every bf16 significand
-    r = ((1.0 / s.double()).float() * torch.tensor(1 + 2.0 ** -21)).float()
     x = torch.cat([torch.arange(1024, 2048).double() * 2.0 ** e for e in range(-14, 1)])   # every fp16 significand
     x = x[None].expand(128, -1)
     keep = x <= (q + 0.4) * s[:, None].double()
     exact = torch.floor(x / s[:, None].double() + 0.5)
-    prod = x * r[:, None].double()              # 11 + 24 bits: exact in 53
-    rounded = torch.round(prod)                 # one rounding of the exact product, to the nearest integer
-    assert bool((rounded == exact)[keep].all())
+    nearest = (1.0 / s.double()).float()
+    for i in (nearest, torch.nextafter(nearest, torch.zeros(())), torch.nextafter(nearest, torch.full((), 2.0))):
+        r = i * torch.tensor(1 + 2.0 ** -21)
+        prod = x * r[:, None].double()          # 11 + 24 bits: exact in 53
+        rounded = torch.round(prod)             # one rounding of the exact product, to the nearest integer
+        assert bool((rounded == exact)[keep].all())
     halves = (2 * x / s[:, None].double()) % 2 == 1
     assert int((halves & keep).sum()) > 100     # there are exact halves among them
