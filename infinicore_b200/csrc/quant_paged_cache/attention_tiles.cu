@@ -282,7 +282,6 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     const int g = lane >> 2, t = lane & 3;
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (lane < 2) {
         pieces[2 * warp + lane].used = 0;
@@ -883,6 +882,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         }
     }
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // ---- the pieces that this CTA's warps left: those of one unit are neighbours
     __syncthreads();
     int cut = 0; // the pieces of the CTA's last unit, where that goes on in other CTAs
@@ -954,12 +954,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 // Adds the pieces of a cut unit: CTA (task, part of its heads).  A thread has four columns of a head and every kSides-th
 // piece, which it adds as they come (maximum, sum, output); the sides meet in shared memory.  Several sides read at a
 // time, since a long sequence alone may lie in pieces over the whole grid.
-constexpr int kCombineThreads = 256;
+constexpr int kCombineThreads = 512;
 
 template <int HD, int HT>
 __global__ void __launch_bounds__(kCombineThreads) quantAttentionCombineKernel(const AttentionArgs a, const TilesArgs p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int kRecord = HT * HD + 2 * HT, kColumns = HD / 4;
     __shared__ float4 part[kCombineThreads];
     __shared__ float2 part_ml[kCombineThreads];
