@@ -75,6 +75,7 @@ __device__ __forceinline__ float maxNan(float a, float b) {
 // The tiles kernel (attention_tiles.cu): whether a layout suits it, and what a launch needs.
 struct TilesPlan {
     bool eligible = false;
+    bool dense = false; // 16 tokens of a head are one run of memory
     int grid = 0;
     int subs = 0;       // kv heads * head tiles of a group
     int head_tiles = 0;

@@ -268,8 +268,9 @@ __device__ __forceinline__ void storeOut(const AttentionArgs &a, const TilesArgs
     }
 }
 
-// P16: blocks are multiples of 16 tokens, so a tile lies in one; otherwise of 8, and a half of a tile does.
-template <int BITS, int HD, int HT, bool P16>
+// DENSE: blocks are multiples of 16 tokens and the rows of a head follow one another in a block, so 16 tokens are one run of
+// memory; otherwise blocks are multiples of 8 tokens, rows lie anywhere, and 8 tokens' scales are one run.
+template <int BITS, int HD, int HT, bool DENSE>
 __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAttentionTilesKernel(const AttentionArgs a, const TilesArgs p) {
     using C = Cfg<BITS, HD, HT>;
     constexpr int NG = C::kGroups, NH = C::kHeadTiles, CPR = C::kChunks, S = C::kStages, TILE = C::kTile, SUBS = C::kSubs;
@@ -377,19 +378,21 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         unsigned f_half = TILE / 8 * static_cast<unsigned>(tile); // first half (8 tokens) of the next tile, within its unit
         int f_left = left;
         const unsigned char *table_row = nullptr;
-        // block 0 of the unit's kv head: K and V codes, and this lane's 16 bytes of scales in a run of 8 tokens
-        const unsigned char *k_unit = nullptr, *v_unit = nullptr, *s_lane = nullptr;
-        constexpr int kRuns = P16 ? SUBS : 2 * SUBS; // runs of 16 or 8 tokens, each in one block
+        // this lane's first 16 bytes of codes (where runs are dense; otherwise the kv head's first) and of scales in block 0
+        const unsigned char *k_lane = nullptr, *v_lane = nullptr, *s_lane = nullptr;
+        constexpr int kRuns = DENSE ? SUBS : 2 * SUBS; // runs of 16 or 8 tokens, each in one block
         unsigned block[kRuns] = {}, first_slot[kRuns] = {}; // of the next tile's runs: the block, the first slot there
         const unsigned code_block = static_cast<unsigned>(a.k_block), code_slot = static_cast<unsigned>(a.k_slot);
         const unsigned scale_block = 2u * static_cast<unsigned>(a.ks_block);
         auto unit = [&]() {
             const int kv = copies.sub / p.head_tiles;
             table_row = static_cast<const unsigned char *>(a.block_tables) + ((copies.seq * a.table_seq) << p.index_shift);
-            k_unit = a.k_codes + kv * a.k_head;
-            v_unit = a.v_codes + kv * a.k_head;
+            const long long codes = kv * a.k_head + (DENSE ? lane * 16 : 0);
+            k_lane = a.k_codes + codes;
+            v_lane = a.v_codes + codes;
             const bool v = lane >= TILE / 8 * NG;
-            s_lane = reinterpret_cast<const unsigned char *>((v ? a.v_scales : a.k_scales) + kv * a.ks_head) + (lane % NG) * 16;
+            const int chunk = lane % NG + (DENSE ? (lane / NG & 1) * NG : 0);
+            s_lane = reinterpret_cast<const unsigned char *>((v ? a.v_scales : a.k_scales) + kv * a.ks_head) + chunk * 16;
         };
         auto entry = [&](unsigned page) { // the low word of a 64-bit entry says all that a block in the pool can be
             const unsigned char *at = table_row + (static_cast<unsigned long long>(page) << p.index_shift);
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             for (int r = 1; r < kRuns; ++r) {
                 // a run behind the sequence's end, whose table entry may say anything, is read where the one before is; entries are
                 // only loaded here (the same one twice, if it must be): the next fetch is the first to wait for them
-                constexpr unsigned kTokens = P16 ? 16u : 8u;
+                constexpr unsigned kTokens = DENSE ? 16u : 8u;
                 const unsigned slot = first_slot[r - 1] + kTokens;
                 const bool live = 8 * static_cast<int>(f_half) + r * static_cast<int>(kTokens) < copies.len;
                 const bool turn = slot >= static_cast<unsigned>(a.block_size);
@@ -423,33 +426,39 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         };
         auto fetch = [&](unsigned dst) { // the next tile into a slot of the ring
             if (f_left > 0) {
-                unsigned long long from[kRuns];
+                constexpr int kCopies = CPR * TILE / 32; // of a lane, for K as for V
+                const unsigned char *k_run[kRuns], *v_run[kRuns];
 #pragma unroll
                 for (int r = 0; r < kRuns; ++r) {
-                    from[r] = static_cast<unsigned long long>(block[r]) * code_block + static_cast<unsigned long long>(first_slot[r]) * code_slot;
+                    const unsigned row = DENSE ? C::kRowBytes : code_slot;
+                    k_run[r] = k_lane + static_cast<unsigned long long>(block[r]) * code_block + static_cast<unsigned long long>(first_slot[r]) * row;
+                    v_run[r] = v_lane + static_cast<unsigned long long>(block[r]) * code_block + static_cast<unsigned long long>(first_slot[r]) * row;
                 }
-                constexpr int kCopies = CPR * TILE / 32; // of a lane, for K as for V
 #pragma unroll
                 for (int j = 0; j < kCopies; ++j) {
                     const int i = lane + 32 * j, r = i / CPR, c = i % CPR;
                     const int swz = CPR % 8 == 0 ? (r & 7) : CPR % 4 == 0 ? ((r >> 1) & 3) : ((r >> 2) & 1);
                     const unsigned to = dst + r * C::kRowBytes + ((c ^ swz) << 4);
-                    const int sub = SUBS == 1 ? 0 : 32 * j / CPR / 16; // where there are two, 16 rows are whole rounds of the warp
-                    const unsigned long long run = P16 ? from[sub] : (r & 8) ? from[kRuns == 1 ? 0 : 2 * sub + 1] : from[P16 ? 0 : 2 * sub];
-                    const unsigned in = static_cast<unsigned>(P16 ? r & 15 : r & 7) * code_slot + c * 16;
-                    copy16(to, k_unit + (run + in));
-                    copy16(to + TILE * C::kRowBytes, v_unit + (run + in));
+                    if constexpr (DENSE) {
+                        constexpr int kOfRun = kCopies / kRuns; // copies of a run are 512 bytes apart
+                        copy16(to, k_run[j / kOfRun] + j % kOfRun * 512);
+                        copy16(to + TILE * C::kRowBytes, v_run[j / kOfRun] + j % kOfRun * 512);
+                    } else {
+                        const int sub = SUBS == 1 ? 0 : 32 * j / CPR / 16; // where there are two, 16 rows are whole rounds of the warp
+                        const unsigned in = static_cast<unsigned>(r & 7) * code_slot + c * 16;
+                        copy16(to, ((r & 8) ? k_run[kRuns == 1 ? 0 : 2 * sub + 1] : k_run[kRuns == 1 ? 0 : 2 * sub]) + in);
+                        copy16(to + TILE * C::kRowBytes, ((r & 8) ? v_run[kRuns == 1 ? 0 : 2 * sub + 1] : v_run[kRuns == 1 ? 0 : 2 * sub]) + in);
+                    }
                 }
                 // scales: 8 rows are one run of NG chunks
                 if (lane < TILE / 4 * NG) {
-                    const int h = (lane / NG) & (TILE / 8 - 1), r = P16 ? h >> 1 : h;
+                    const int h = (lane / NG) & (TILE / 8 - 1), r = DENSE ? h >> 1 : h;
                     unsigned b = block[0], at = first_slot[0];
 #pragma unroll
                     for (int k = 1; k < kRuns; ++k) {
                         b = r == k ? block[k] : b;
                         at = r == k ? first_slot[k] : at;
                     }
-                    at += P16 ? 8u * (h & 1) : 0u;
                     copy16(dst + 2 * TILE * C::kRowBytes + lane * 16, s_lane + static_cast<unsigned long long>(b) * scale_block + at * (2u * NG));
                 }
                 f_half += TILE / 8;
@@ -648,12 +657,14 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                             }
                         }
                     }
-                    const float s0 = BITS == 8 ? scaleAt(ks[0], 0) : 1.f, s1 = BITS == 8 ? scaleAt(ks[1], 0) : 1.f;
+                    if constexpr (BITS == 8) {
+                        const float s0 = scaleAt(ks[0], 0), s1 = scaleAt(ks[1], 0);
 #pragma unroll
-                    for (int n = 0; n < NH; ++n) {
+                        for (int n = 0; n < NH; ++n) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[u][n][i] *= BITS == 8 ? factor[n][i & 1] * (i < 2 ? s0 : s1) : factor[n][i & 1];
+                            for (int i = 0; i < 4; ++i) {
+                                s[u][n][i] *= i < 2 ? s0 : s1;
+                            }
                         }
                     }
                 }
@@ -663,15 +674,26 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     loadScales(vs[u][0], scales + 2 * TILE * NG + u * (32 * NG));
                     loadScales(vs[u][1], scales + 2 * TILE * NG + u * (32 * NG) + 16 * NG);
                 }
+                // scores in the log2 domain are s * f from here on
+                float f[NH][2];
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+                    f[n][0] = factor[n][0];
+                    f[n][1] = factor[n][1];
+                }
                 if (token0 >= special) {
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        f[n][0] = f[n][1] = 1.f;
+                    }
 #pragma unroll
                     for (int r = 0; r < 2 * SUBS; ++r) {
                         const int u = r >> 1, i = 2 * (r & 1), token = token0 + 8 * r + g;
                         const float far = static_cast<float>(token - (len - 1));
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
-                            s[u][n][i] += slope[n][0] * far;
-                            s[u][n][i + 1] += slope[n][1] * far;
+                            s[u][n][i] = fmaf(slope[n][0], far, s[u][n][i] * factor[n][0]);
+                            s[u][n][i + 1] = fmaf(slope[n][1], far, s[u][n][i + 1] * factor[n][1]);
                         }
                         if (token >= len) { // no weight, whatever the scales are
 #pragma unroll
@@ -688,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 
                 // How far a token's weights can reach above its p: log2 of its largest V scale is at most bits / 128 - 126.9 for a
                 // bf16 with these bits (log2(1 + f) <= f + 0.0861).  The constant stays out; it is taken off with the maximum.
-                float reach[2 * SUBS]; // 2^23 + bits
+                float reach[2 * SUBS]; // 65536 + bits / 128
 #pragma unroll
                 for (int r = 0; r < 2 * SUBS; ++r) {
                     unsigned m = vs[r >> 1][r & 1][0];
@@ -696,18 +718,18 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     for (int k = 1; k < kWords; ++k) {
                         m = __vmaxu2(m, vs[r >> 1][r & 1][k]);
                     }
-                    reach[r] = __uint_as_float(max(max(m & 0xffffu, m >> 16), kLeastScale) | 0x4b000000u);
+                    reach[r] = __uint_as_float(max(max(m & 0xffffu, m >> 16), kLeastScale) | 0x47800000u); // 2^16 (1 + bits / 2^23)
                 }
-                constexpr float kBias = 65536.f + 126.9f; // 2^23 / 128 and the constant
+                constexpr float kBias = 65536.f + 126.9f;
                 bool move = false; // the maximum does rarely
 #pragma unroll
                 for (int n = 0; n < NH; ++n) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float high = fmaf(reach[0], 0.0078125f, s[0][n][x]);
+                        float high = fmaf(s[0][n][x], f[n][x], reach[0]);
 #pragma unroll
                         for (int r = 1; r < 2 * SUBS; ++r) {
-                            high = fmaxf(high, fmaf(reach[r], 0.0078125f, s[r >> 1][n][2 * (r & 1) + x]));
+                            high = fmaxf(high, fmaf(s[r >> 1][n][2 * (r & 1) + x], f[n][x], reach[r]));
                         }
                         move |= high > top[n][x] + (kSlack + kBias);
                     }
@@ -731,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                             float now = top[n][x];
 #pragma unroll
                             for (int r = 0; r < 2 * SUBS; ++r) {
-                                now = fmaxf(now, s[r >> 1][n][2 * (r & 1) + x] + reach[r]);
+                                now = fmaxf(now, fmaf(s[r >> 1][n][2 * (r & 1) + x], f[n][x], reach[r]));
                             }
                             now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
                             now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
@@ -753,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     for (int n = 0; n < NH; ++n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            s[u][n][i] = exp2Fast(s[u][n][i] - top[n][i & 1]);
+                            s[u][n][i] = exp2Fast(fmaf(s[u][n][i], f[n][i & 1], -top[n][i & 1]));
                         }
                         sum[n][0] += s[u][n][0] + s[u][n][2];
                         sum[n][1] += s[u][n][1] + s[u][n][3];
@@ -1026,7 +1048,7 @@ __global__ void __launch_bounds__(kCombineThreads) quantAttentionCombineKernel(c
 using TilesKernel = void (*)(AttentionArgs, TilesArgs);
 
 struct Variant {
-    TilesKernel tiles[2], combine; // blocks of 8 | 16 tokens
+    TilesKernel tiles[2], combine; // any | dense
     int ctas, smem, record, heads, tile;
 };
 
@@ -1113,6 +1135,7 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     // n / halves for n < 2^31 as mulhi(n, magic) >> shift: magic = floor(2^(32 + shift) / halves) + 1 with 2^shift < halves, which is
     // below 2^32 and off by at most halves, and n * halves < 2^(32 + shift); 2^(31) and one shift less for a power of two
     const unsigned halves = static_cast<unsigned>(P.block_size / 8);
+    plan.dense = P.block_size % 16 == 0 && k.slot == static_cast<ptrdiff_t>(I.head_size * P.bits / 8);
     plan.half_self = halves == 1 ? 0xffffffffu : 0u;
     if (halves > 1) {
         while ((2u << plan.half_shift) <= halves) {
@@ -1151,7 +1174,7 @@ infiniStatus_t launchTiles(const AttentionInfo &info, const TilesPlan &plan, con
     p.index_shift = a.index_is_64 ? 3 : 2;
     p.halves = static_cast<unsigned>(a.block_size / 8);
     p.out_words = plan.out_words && alignedTo(a.out, 8) ? 1 : 0;
-    const TilesKernel kernel = var.tiles[a.block_size % 16 == 0];
+    const TilesKernel kernel = var.tiles[plan.dense];
     // an attribute of the device's function: set by the descriptor's first launch
     if (__atomic_load_n(&plan.ready, __ATOMIC_RELAXED) == 0) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem) != cudaSuccess) {
