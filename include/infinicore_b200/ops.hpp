@@ -459,6 +459,76 @@ inline void paged_decode_step_(const Tensor &out, const Tensor &q, const Tensor 
     }
 }
 
+// Pools held in 8 or 4 bits (include/infiniop/ops/quant_paged_caching.h; no reference counterpart): codes (I8 or U8) and BF16 scales.
+struct QuantPools {
+    Tensor k_cache, v_cache, k_scales, v_scales;
+};
+
+// Rows k / v [tokens, kv_heads, head] quantised into the pools at slot_mapping.
+inline void quant_paged_caching_(const QuantPools &pools, const Tensor &k, const Tensor &v, const Tensor &slot_mapping,
+                                 infinirtStream_t stream = nullptr) {
+    using namespace detail;
+    DeviceState &st = state();
+    Key key("quant_paged_caching");
+    key.add(&pools.k_cache).add(&pools.v_cache).add(&pools.k_scales).add(&pools.v_scales).add(&k).add(&v).add(&slot_mapping);
+    const Entry &e = lookup(
+        st, key,
+        [&](infiniopHandle_t h, InfiniopDescriptor **d) {
+            TensorDesc kc(&pools.k_cache), vc(&pools.v_cache), ks(&pools.k_scales), vs(&pools.v_scales), tk(&k), tv(&v), sm(&slot_mapping);
+            return infiniopCreateQuantPagedCachingDescriptor(h, d, kc.get(), vc.get(), ks.get(), vs.get(), tk.get(), tv.get(), sm.get());
+        },
+        infiniopGetQuantPagedCachingWorkspaceSize, infiniopDestroyQuantPagedCachingDescriptor, "infiniopCreateQuantPagedCachingDescriptor");
+    check(infiniopQuantPagedCaching(e.desc, st.workspace(e.workspace_bytes, stream), e.workspace_bytes, pools.k_cache.data, pools.v_cache.data,
+                                    pools.k_scales.data, pools.v_scales.data, k.data, v.data, slot_mapping.data, stream),
+          "infiniopQuantPagedCaching");
+}
+
+// The values at slot_mapping as rows k / v [tokens, kv_heads, head] of F16, BF16 or F32.
+inline void quant_paged_cache_read_(const Tensor &k, const Tensor &v, const QuantPools &pools, const Tensor &slot_mapping,
+                                    infinirtStream_t stream = nullptr) {
+    using namespace detail;
+    DeviceState &st = state();
+    Key key("quant_paged_cache_read");
+    key.add(&k).add(&v).add(&pools.k_cache).add(&pools.v_cache).add(&pools.k_scales).add(&pools.v_scales).add(&slot_mapping);
+    const Entry &e = lookup(
+        st, key,
+        [&](infiniopHandle_t h, InfiniopDescriptor **d) {
+            TensorDesc tk(&k), tv(&v), kc(&pools.k_cache), vc(&pools.v_cache), ks(&pools.k_scales), vs(&pools.v_scales), sm(&slot_mapping);
+            return infiniopCreateQuantPagedCacheReadDescriptor(h, d, tk.get(), tv.get(), kc.get(), vc.get(), ks.get(), vs.get(), sm.get());
+        },
+        infiniopGetQuantPagedCacheReadWorkspaceSize, infiniopDestroyQuantPagedCacheReadDescriptor,
+        "infiniopCreateQuantPagedCacheReadDescriptor");
+    check(infiniopQuantPagedCacheRead(e.desc, st.workspace(e.workspace_bytes, stream), e.workspace_bytes, k.data, v.data, pools.k_cache.data,
+                                      pools.v_cache.data, pools.k_scales.data, pools.v_scales.data, slot_mapping.data, stream),
+          "infiniopQuantPagedCacheRead");
+}
+
+// out [seqs, heads, head] = decode attention of q [seqs, heads, head] over the pools.
+inline void quant_paged_attention_(const Tensor &out, const Tensor &q, const QuantPools &pools, const Tensor &block_tables,
+                                   const Tensor &kv_lens, const std::optional<Tensor> &alibi_slopes, float scale,
+                                   infinirtStream_t stream = nullptr) {
+    using namespace detail;
+    DeviceState &st = state();
+    const Tensor *alibi = detail_op::ptr(alibi_slopes);
+    Key key("quant_paged_attention");
+    key.add(&out).add(&q).add(&pools.k_cache).add(&pools.v_cache).add(&pools.k_scales).add(&pools.v_scales).add(&block_tables).add(&kv_lens);
+    key.add(alibi).raw(scale);
+    const Entry &e = lookup(
+        st, key,
+        [&](infiniopHandle_t h, InfiniopDescriptor **d) {
+            TensorDesc o(&out), tq(&q), kc(&pools.k_cache), vc(&pools.v_cache), ks(&pools.k_scales), vs(&pools.v_scales), bt(&block_tables),
+                sl(&kv_lens), al(alibi);
+            return infiniopCreateQuantPagedAttentionDescriptor(h, d, o.get(), tq.get(), kc.get(), vc.get(), ks.get(), vs.get(), bt.get(),
+                                                               sl.get(), al.get(), scale);
+        },
+        infiniopGetQuantPagedAttentionWorkspaceSize, infiniopDestroyQuantPagedAttentionDescriptor,
+        "infiniopCreateQuantPagedAttentionDescriptor");
+    check(infiniopQuantPagedAttention(e.desc, st.workspace(e.workspace_bytes, stream), e.workspace_bytes, out.data, q.data, pools.k_cache.data,
+                                      pools.v_cache.data, pools.k_scales.data, pools.v_scales.data, block_tables.data, kv_lens.data,
+                                      detail_op::data(alibi_slopes), stream),
+          "infiniopQuantPagedAttention");
+}
+
 } // namespace op
 } // namespace infinicore_b200
 

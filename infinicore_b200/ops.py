@@ -396,17 +396,10 @@ def paged_caching(k_cache, v_cache, k, v, slot_mapping):
 # ---- pools held in 8 or 4 bits ----------------------------------------------------------------
 #
 # These calls are a decode step's smallest, so their way to the library is short: the cache key is made of the
-# tensors' own metadata objects, and the device is switched only where it is not the current one.
+# tensors' own metadata objects (without the optional tensor where that is left out: the number of entries tells), and the
+# device is switched only where it is not the current one.
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
-
-
-def _one_device(tensors):
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and (t.get_device() != dev or dev < 0):
-            return _require_cuda(*tensors)  # says what is wrong
-    return dev
 
 
 def _make_quant(st, op, tensors, extra):
@@ -426,21 +419,15 @@ def _make_quant(st, op, tensors, extra):
 
 
 def _run_quant(op, tensors, extra=()):
-    """Runs `op` on these tensors (None where an optional one is left out), its descriptor from the cache."""
-    dev = _one_device(tensors)
+    """Runs `op` on these tensors, its descriptor from the cache.  The last one may be None: an optional one left out."""
+    given = tensors if tensors[-1] is not None else tensors[:-1]
+    dev = given[0].get_device()
+    key = (op, extra, *[t.dtype for t in given], *[t.shape for t in given], *[t.stride() for t in given])
+    if any([t.get_device() != dev for t in given]) or dev < 0:
+        _require_cuda(*given)  # says what is wrong
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _run_quant(op, tensors, extra)
-    key = [op, extra]
-    pointers = []
-    for t in tensors:
-        if t is None:
-            key.append(None)
-            pointers.append(None)
-        else:
-            key += (t.dtype, t.shape, t.stride())
-            pointers.append(t.data_ptr())
-    key = tuple(key)
     per_dev = getattr(_tls, "per_dev", None)
     st = per_dev.get(dev) if per_dev is not None else None
     entry = st["cache"].get(key) if st is not None else None
@@ -459,6 +446,9 @@ def _run_quant(op, tensors, extra=()):
             if buf is None or buf.numel() < need:
                 buf = _workspace(st, need, dev)
         ws = buf.data_ptr()
+    pointers = [t.data_ptr() for t in given]
+    if given is not tensors:
+        pointers.append(None)
     status = entry["run"](entry["desc"], ws, need, *pointers, stream)
     if status:
         check_error(status)
