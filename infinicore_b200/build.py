@@ -115,7 +115,8 @@ def _link(objs, out: Path, extra, verbose: bool) -> None:
 
 
 def build(force: bool = False, verbose: bool = False) -> dict:
-    """Compiles what is stale and returns {"infinirt": path, "infiniop": path, "infiniccl": path, "pybind": path}."""
+    """Compiles what is stale and returns {"infinirt": path, "infiniop": path, "infiniccl": path, "pybind": path,
+    "torch_ops": path}."""
     LIB.mkdir(exist_ok=True)
     OBJ.mkdir(exist_ok=True)
     if force:
@@ -135,7 +136,8 @@ def build(force: bool = False, verbose: bool = False) -> dict:
         _link(op_objs, libop, [f"-L{LIB}", "-linfinirt", "-Xlinker", "-rpath=$ORIGIN"], verbose)
     if force or not libccl.exists() or libccl.stat().st_mtime < newest_obj:
         _link(ccl_objs, libccl, [f"-L{LIB}", "-linfinirt", "-lnccl", "-Xlinker", "-rpath=$ORIGIN"], verbose)
-    return {"infinirt": librt, "infiniop": libop, "infiniccl": libccl, "pybind": build_pybind(force, verbose)}
+    return {"infinirt": librt, "infiniop": libop, "infiniccl": libccl, "pybind": build_pybind(force, verbose),
+            "torch_ops": build_torch_ops(force, verbose)}
 
 
 def build_pybind(force: bool = False, verbose: bool = False) -> Path:
@@ -165,6 +167,40 @@ def build_pybind(force: bool = False, verbose: bool = False) -> Path:
         sys.stderr.write(res.stdout + res.stderr)
     if res.returncode != 0:
         raise RuntimeError("g++ failed on pybind/module.cpp")
+    stamp.write_text(want)
+    return out
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles the operators on torch tensors (csrc/pybind/torch_ops.cpp) with g++ against torch's own headers, in-tree, linked
+    to the libraries in lib/ (found again at run time through $ORIGIN/lib) and to torch's (loaded by `import torch`)."""
+    import sysconfig
+
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    src = CSRC / "pybind" / "torch_ops.cpp"
+    out = PKG / ("_torch_ops" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+    stamp = OBJ / "torch_ops.sha"
+    want = _digest([src, INCLUDE / "infinicore_b200" / "ops.hpp"] + list(INCLUDE.rglob("*.h"))) + torch.__version__
+    if not force and out.exists() and stamp.exists() and stamp.read_text() == want:
+        return out
+    gxx = shutil.which("g++")
+    if gxx is None:
+        raise RuntimeError("g++ not found")
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = [gxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f"-I{INCLUDE}", "-isystem", str(base / "include"), "-isystem", str(base / "include/torch/csrc/api/include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"), "-Wall", "-Wextra", str(src), "-o", str(out),
+           f"-L{LIB}", "-linfiniop", "-linfinirt", f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN/lib"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed on pybind/torch_ops.cpp")
     stamp.write_text(want)
     return out
 

@@ -395,63 +395,18 @@ def paged_caching(k_cache, v_cache, k, v, slot_mapping):
 
 # ---- pools held in 8 or 4 bits ----------------------------------------------------------------
 #
-# These calls are a decode step's smallest, so their way to the library is short: the cache key is made of the
-# tensors' own metadata objects (without the optional tensor where that is left out: the number of entries tells), and the
-# device is switched only where it is not the current one.
+# These calls are a decode step's smallest: checks, descriptor cache and call are in C++ (csrc/pybind/torch_ops.cpp).
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_torch_ops = None
 
 
-def _make_quant(st, op, tensors, extra):
-    descs = [_desc(t) if t is not None else None for t in tensors]
-    desc = infiniopOperatorDescriptor_t()
-    try:
-        check_error(getattr(LIBINFINIOP, f"infiniopCreate{op}Descriptor")(
-            st["handle"], ctypes.byref(desc), *[t.descriptor if t is not None else None for t in descs], *extra))
-    finally:
-        for t in descs:
-            if t is not None:
-                t.destroy_desc()
-    size = ctypes.c_size_t(0)
-    check_error(getattr(LIBINFINIOP, f"infiniopGet{op}WorkspaceSize")(desc, ctypes.byref(size)))
-    return {"desc": desc, "workspace": size.value, "run": getattr(LIBINFINIOP, f"infiniop{op}"),
-            "destroy": getattr(LIBINFINIOP, f"infiniopDestroy{op}Descriptor")}
+def _quant():
+    global _torch_ops
+    if _torch_ops is None:
+        from . import _torch_ops as module
 
-
-def _run_quant(op, tensors, extra=()):
-    """Runs `op` on these tensors, its descriptor from the cache.  The last one may be None: an optional one left out."""
-    given = tensors if tensors[-1] is not None else tensors[:-1]
-    dev = given[0].get_device()
-    key = (op, extra, *[t.dtype for t in given], *[t.shape for t in given], *[t.stride() for t in given])
-    if any([t.get_device() != dev for t in given]) or dev < 0:
-        _require_cuda(*given)  # says what is wrong
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _run_quant(op, tensors, extra)
-    per_dev = getattr(_tls, "per_dev", None)
-    st = per_dev.get(dev) if per_dev is not None else None
-    entry = st["cache"].get(key) if st is not None else None
-    if entry is not None:
-        st["cache"].move_to_end(key)
-    else:
-        st = _state(dev)
-        entry = _lookup(st, key, lambda: _make_quant(st, op, tensors, extra))
-    need, ws, stream = entry["workspace"], None, _raw_stream(dev)
-    if need:
-        # a captured call gets scratch of its own graph's memory: two graphs may be replayed at the same time
-        if torch.cuda.is_current_stream_capturing():
-            buf = torch.empty(need, dtype=torch.uint8, device=f"cuda:{dev}")
-        else:
-            buf = st["workspace"].get(stream)
-            if buf is None or buf.numel() < need:
-                buf = _workspace(st, need, dev)
-        ws = buf.data_ptr()
-    pointers = [t.data_ptr() for t in given]
-    if given is not tensors:
-        pointers.append(None)
-    status = entry["run"](entry["desc"], ws, need, *pointers, stream)
-    if status:
-        check_error(status)
+        _torch_ops = module
+    return _torch_ops
 
 
 def quant_paged_caching(k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping):
@@ -462,8 +417,7 @@ def quant_paged_caching(k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping
     (8 bits) or head_size / 32 (4 bits).  A group with largest magnitude A gets the scale A / 127 or A / 7 rounded to
     bfloat16 and the codes x / scale, to the nearest, halves away from zero; one with an infinity or NaN reads back
     as NaN.  Returns (k_cache, v_cache, k_scales, v_scales)."""
-    tensors = (k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping)
-    _run_quant("QuantPagedCaching", tensors)
+    _quant().quant_paged_caching(k_cache, v_cache, k_scales, v_scales, k, v, slot_mapping)
     return (k_cache, v_cache, k_scales, v_scales)
 
 
@@ -472,12 +426,9 @@ def quant_paged_cache_read(k_cache, v_cache, k_scales, v_scales, slot_mapping, d
     allowed; zeros where negative) of pools that quant_paged_caching wrote, as dense rows k [num_tokens, num_kv_heads,
     k head size] and v.  `out`: a pair of tensors to write instead of new ones (their dtype counts).  Returns (k, v)."""
     if out is None:
-        tokens, heads, packed = slot_mapping.shape[0], k_cache.shape[1], 2 if k_cache.dtype == torch.uint8 else 1
-        out = (k_cache.new_empty((tokens, heads, k_cache.shape[3] * packed), dtype=dtype),
-               v_cache.new_empty((tokens, heads, v_cache.shape[3] * packed), dtype=dtype))
+        return _quant().quant_paged_cache_read_new(k_cache, v_cache, k_scales, v_scales, slot_mapping, dtype)
     k, v = out
-    tensors = (k, v, k_cache, v_cache, k_scales, v_scales, slot_mapping)
-    _run_quant("QuantPagedCacheRead", tensors)
+    _quant().quant_paged_cache_read(k, v, k_cache, v_cache, k_scales, v_scales, slot_mapping)
     return (k, v)
 
 
@@ -489,6 +440,5 @@ def quant_paged_attention(q, k_cache, v_cache, k_scales, v_scales, block_tables,
     `out` is allocated here).  Captured into a CUDA graph, each call has scratch of its own.  Returns `out`."""
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    tensors = (out, q, k_cache, v_cache, k_scales, v_scales, block_tables, cache_lens, alibi_slopes)
-    _run_quant("QuantPagedAttention", tensors, (float(scale),))
+    _quant().quant_paged_attention(out, q, k_cache, v_cache, k_scales, v_scales, block_tables, cache_lens, alibi_slopes, scale)
     return out

@@ -215,19 +215,16 @@ def test_reading_is_the_rounded_product(ib, shape, bits, dtype):
 @contextlib.contextmanager
 def rows_path():
     """Descriptors made here use the kernel for any layout; none of them is kept."""
-    from infinicore_b200 import ops
-
     with environment(INFINIOP_QUANT_ATTENTION_PATH="rows"):
-        forget(ops)
+        forget()
         yield
-    forget(ops)
+    forget()
 
 
-def forget(ops):
-    cache = ops._tls.per_dev[0]["cache"]
-    for key in [k for k in cache if k[0] == "QuantPagedAttention"]:
-        entry = cache.pop(key)
-        entry["destroy"](entry["desc"])
+def forget():
+    from infinicore_b200 import _torch_ops
+
+    _torch_ops.clear_cache()
 
 
 def check_attention(ib, gen, lens, heads, kvh, hd, bs, bits, dtype, scale=None, alibi=False, ix=torch.int64, std=1.0, qstd=1.0, what=""):
@@ -601,6 +598,7 @@ def test_checked_indices_raise_flags_and_touch_nothing_foreign(ib):
     row is skipped (zeros when read), a bad block is read as block 0."""
     g = torch.Generator().manual_seed(61)
     ib.kernel_status()
+    forget()
     with environment(INFINIOP_PAGED_CHECK_INDICES=1):
         pools = qh.random_pools(g, 6, 2, 16, 64, 64, 8)
         before = [t.clone() for t in pools]
@@ -622,13 +620,7 @@ def test_checked_indices_raise_flags_and_touch_nothing_foreign(ib):
         # an entry behind the last page is not read
         ib.quant_paged_attention(q, *pools, bad, torch.tensor([16, 20], device="cuda"), None, 0.125)
         assert ib.kernel_status() == 0
-        # descriptors made here must not serve later tests
-        from infinicore_b200 import ops
-
-        cache = ops._tls.per_dev[0]["cache"]
-        for key in [k for k in cache if str(k[0]).startswith("QuantPaged")]:
-            entry = cache.pop(key)
-            entry["destroy"](entry["desc"])
+    forget()  # descriptors made here must not serve later tests
 
 
 def test_refusals_reach_python(ib):
