@@ -1,7 +1,7 @@
 // The fast kernel of infiniopQuantPagedAttention: tiles of 16 or 32 tokens, matrix instructions on the codes.
 //
 // Work.  A unit is (sequence, kv head, tile of 8 or 16 q heads of its group), as many token tiles long as cover the sequence.
-// All units lie end to end in one line, each with kUnitCost tiles in front for what a unit costs by itself (q, results),
+// All units lie end to end in one line, each with unitCost() tiles in front for what a unit costs by itself (q, results),
 // and the line is cut into equal ranges, one for each warp of a persistent grid, so that ragged batches, many short and
 // few long sequences load the machine alike.  A warp that has a unit to itself stores its rows; pieces of a unit in one
 // CTA meet in shared memory at the CTA's end; a unit that is cut between CTAs leaves partial results (maximum, sum,
@@ -37,8 +37,10 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kUnitCost = 1;       // tiles' worth of time that a unit costs beside its tiles
-constexpr int kMinRange = 3;       // of a warp: at least two tiles of a unit's first range
+// What a unit costs beside its tiles, in tiles: the time of 64 tokens.  Measured at 40 ragged sequences (64/8 heads of 128, 4 bits): 0
+// tokens 64 us, 32 43.5, 64 41.0, 128 40.7; at 62 sequences of 200 to 2000 32.1, 31.2, 30.2, 31.0.
+constexpr int unitCost(int tile) { return 64 / tile; }
+constexpr int minRange(int tile) { return unitCost(tile) + 2; } // of a warp: at least two tiles of a unit's first range
 constexpr float kSlack = 8.f;      // in the log2 domain; 2^8 is far inside fp16
 constexpr unsigned kLeastScale = 27u << 7; // V scales count as at least 2^-100 for the maximum: an all-zero row stays finite
 
@@ -70,7 +72,7 @@ struct Cfg {
     static constexpr int kResult = HT * kStride * 4;
     static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes);
     // resident CTAs: what the registers of q, outputs and scales leave room for
-    static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
+    static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 || HT == 16 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
     static constexpr int kStages = kFit > 6 ? 6 : kFit;
     static_assert(kStages >= 2, "a ring of two tiles at least");
@@ -209,7 +211,7 @@ __device__ __forceinline__ int tilesOf(int len) {
 }
 template <int TILE>
 __device__ __forceinline__ long long costOf(int len) {
-    return len > 0 ? tilesOf<TILE>(len) + kUnitCost : 0;
+    return len > 0 ? tilesOf<TILE>(len) + unitCost(TILE) : 0;
 }
 
 // Where a walk over a warp's range is: the unit, how much of the range lies behind what it takes of that unit.  Kept in
@@ -220,7 +222,7 @@ struct Walk {
     // To the next unit: how many of its tiles are in the range (0: the range has ended).
     template <int TILE>
     __device__ __forceinline__ int step(const AttentionArgs &a, int subs) {
-        budget -= kUnitCost; // at or below 0: the range ends in front of the unit's first tile
+        budget -= unitCost(TILE); // at or below 0: the range ends in front of the unit's first tile
         if (budget <= 0) {
             return 0;
         }
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     long long cta_start;
     Walk first_walk = {};   // unit of the range's start; its position there in `budget`
     if (p.unit_of_cta) {
-        // the line is one unit
+        // the line is one unit, and a warp's range a fourth of its tiles
         first_walk.seq = static_cast<int>(blockIdx.x) / p.subs;
         first_walk.sub = static_cast<int>(blockIdx.x) - first_walk.seq * p.subs;
         first_walk.len = lengthOf(a, first_walk.seq);
@@ -301,10 +303,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         if (total == 0) {
             return;
         }
-        range = (total + kWarps - 1) / kWarps;
-        range = range > kMinRange ? range : kMinRange;
-        cta_start = 0;
-        first_walk.budget = static_cast<int>(range * warp);
+        range = (tilesOf<TILE>(first_walk.len) + kWarps - 1) / kWarps;
+        cta_start = unitCost(TILE);
+        first_walk.budget = static_cast<int>(cta_start + range * warp);
     } else {
         // every warp adds up the batch for itself: lane i has sequences i * per to (i + 1) * per - 1
         const int per = (a.num_seqs + 31) / 32;
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         total = __shfl_sync(0xffffffffu, upto, 31) * p.subs;
         const int workers = static_cast<int>(gridDim.x) * kWarps;
         range = (total + workers - 1) / workers;
-        range = range > kMinRange ? range : kMinRange;
+        range = range > minRange(TILE) ? range : minRange(TILE);
         cta_start = range * kWarps * blockIdx.x;
         if (cta_start >= total) {
             if (tid == 0 && !p.task_of_unit) {
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         {
             Walk w = first_walk;
             w.tiles = tilesOf<TILE>(w.len);
-            const int in = w.budget - kUnitCost; // below 0: in front of the unit's first tile
+            const int in = w.budget - unitCost(TILE); // below 0: in front of the unit's first tile
             tile = in > 0 ? in : 0;
             place = start + (tile - in);
             const int budget = static_cast<int>(end - place);
@@ -477,6 +478,32 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             }
             commitCopies();
         };
+        // q of a unit as it lies in memory: heads g and g + 8, at 4 bits 8 elements from 32 j + 8 t, at 8 bits 4 from 32 j + 4 t and 4 from
+        // 16 behind; loaded a unit ahead
+        uint4 q_raw[NH][HD / 32];
+        auto loadQ = [&]() {
+            const int kv = work.sub / p.head_tiles, head0 = (work.sub - kv * p.head_tiles) * HT;
+            const unsigned short *q = static_cast<const unsigned short *>(a.q) + work.seq * a.q_seq
+                                    + (static_cast<long long>(kv) * a.group + head0 + g) * a.q_head;
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) {
+                    q_raw[n][j] = make_uint4(0, 0, 0, 0);
+                    if (head0 + g + 8 * n < a.group) {
+                        const unsigned short *from = q + 8 * n * a.q_head + 32 * j;
+                        if constexpr (BITS == 4) {
+                            q_raw[n][j] = *reinterpret_cast<const uint4 *>(from + 8 * t);
+                        } else {
+                            const uint2 lo = *reinterpret_cast<const uint2 *>(from + 4 * t);
+                            const uint2 hi = *reinterpret_cast<const uint2 *>(from + 16 + 4 * t);
+                            q_raw[n][j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                        }
+                    }
+                }
+            }
+        };
+        loadQ();
         unit();
         look();
         const unsigned ring_addr = smemAddr(ring);
@@ -503,25 +530,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
                 const int h = g + 8 * n;
-                unsigned raw[HD / 16][2];
                 unsigned largest = 0;
-                const unsigned short *q = static_cast<const unsigned short *>(a.q) + work.seq * a.q_seq + (head_at + h) * a.q_head;
 #pragma unroll
-                for (int j = 0; j < HD / 32; ++j) { // 4 bits: 8 elements from 32 j + 8 t; 8 bits: 4 from 32 j + 4 t and 4 from + 16
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (h < heads) {
-                        if constexpr (BITS == 4) {
-                            x = *reinterpret_cast<const uint4 *>(q + 32 * j + 8 * t);
-                        } else {
-                            const uint2 lo = *reinterpret_cast<const uint2 *>(q + 32 * j + 4 * t);
-                            const uint2 hi = *reinterpret_cast<const uint2 *>(q + 32 * j + 16 + 4 * t);
-                            x = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                        }
-                    }
-                    raw[2 * j][0] = x.x;
-                    raw[2 * j][1] = x.y;
-                    raw[2 * j + 1][0] = x.z;
-                    raw[2 * j + 1][1] = x.w;
+                for (int j = 0; j < HD / 32; ++j) {
+                    const uint4 &x = q_raw[n][j];
                     const unsigned m = 0x7fff7fffu;
                     const unsigned b = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
                     largest = max(largest, max(b & 0xffffu, b >> 16));
@@ -543,12 +555,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 }
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
+                    const unsigned raw[4] = {q_raw[n][j].x, q_raw[n][j].y, q_raw[n][j].z, q_raw[n][j].w};
                     float x[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const unsigned w = raw[2 * j + (i >> 1)][i & 1];
-                        x[2 * i] = wide(w & 0xffffu) * scale_q;
-                        x[2 * i + 1] = wide(w >> 16) * scale_q;
+                        x[2 * i] = wide(raw[i] & 0xffffu) * scale_q;
+                        x[2 * i + 1] = wide(raw[i] >> 16) * scale_q;
                     }
                     if constexpr (BITS == 4) { // the order of codes4
                         qr[n][2 * j][0] = packHalves(x[0], x[4]);
@@ -836,8 +848,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 left = last ? w.step<TILE>(a, p.subs) : 0;
                 __syncwarp();
                 work = w;
+                __syncwarp();
+                if (left > 0) {
+                    loadQ();
+                }
             }
-            place = unit_first + done.tiles + kUnitCost; // if the range goes on, it does with the next unit
+            place = unit_first + done.tiles + unitCost(TILE); // if the range goes on, it does with the next unit
             tile = 0;
             float inv[NH][2];
 #pragma unroll
@@ -1102,13 +1118,13 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     const unsigned long long head_tiles = (group + var.heads - 1) / var.heads;
     const unsigned long long tiles = (static_cast<unsigned long long>(I.max_blocks) * P.block_size + var.tile - 1) / var.tile;
     const unsigned long long subs = head_tiles * P.num_kv_heads;
-    const long double line = static_cast<long double>(tiles + kUnitCost) * subs * I.num_seqs;
+    const long double line = static_cast<long double>(tiles + unitCost(var.tile)) * subs * I.num_seqs;
     const unsigned long long at_most = static_cast<unsigned long long>(props.sm_count) * var.ctas;
     if (tiles > 0x0fffffffull || line > 9e17L || line / at_most > 1e9L) {
         plan.eligible = false; // positions would not fit
         return plan;
     }
-    const unsigned long long useful = (static_cast<unsigned long long>(line) + kWarps * kMinRange - 1) / (kWarps * kMinRange);
+    const unsigned long long useful = (static_cast<unsigned long long>(line) + kWarps * minRange(var.tile) - 1) / (kWarps * minRange(var.tile));
     plan.grid = static_cast<int>(useful < at_most ? useful : at_most);
     plan.head_tiles = static_cast<int>(head_tiles);
     plan.subs = static_cast<int>(subs);
