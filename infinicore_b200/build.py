@@ -105,7 +105,8 @@ def _compile(src: str, verbose: bool, extra=()) -> Path:
 
 
 def _link(objs, out: Path, extra, verbose: bool) -> None:
-    cmd = [nvcc(), "-shared", *ARCH_FLAGS, "-o", str(out), *map(str, objs), "-cudart", "shared", *extra]
+    # with a soname, a module that needs the library gets the one the process has loaded, wherever that came from
+    cmd = [nvcc(), "-shared", *ARCH_FLAGS, "-Xlinker", f"-soname={out.name}", "-o", str(out), *map(str, objs), "-cudart", "shared", *extra]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
