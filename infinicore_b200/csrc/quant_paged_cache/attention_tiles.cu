@@ -62,9 +62,11 @@ struct Cfg {
     static constexpr int kRowBytes = HD * BITS / 8;
     static constexpr int kChunks = kRowBytes / 16;            // 16-byte chunks of a row
     static constexpr int kGroups = BITS == 4 ? HD / 32 : 1;   // scales of a row
-    // A tile is one or two times 16 tokens: the loop around the matrix instructions costs as many issue slots as 8 tokens' arithmetic,
-    // which is what bounds the 4-bit form.
-    static constexpr int kSubs = BITS == 4 && HD * HT <= 1024 ? 2 : 1;
+    // A tile is one, two or four times 16 tokens, about 4 KB of codes: what surrounds the matrix instructions costs as many issue slots
+    // as 8 tokens' arithmetic.  Measured at 64 x 4096 tokens, 32/8 heads (us): 4 bits, heads of 128, 16 tokens 85, 32 81; heads of 64,
+    // 32 tokens 53, 64 50; 8 bits, heads of 64, 16 tokens 63, 32 57.  With 16 heads the scores of 64 tokens do not fit the registers
+    // (64/4 heads of 64 at 4 bits: 32 tokens 41.7, 64 43.7).
+    static constexpr int kSubs = HD * BITS <= 256 && HT == 8 ? 4 : HD * BITS <= 512 ? 2 : 1;
     static constexpr int kTile = 16 * kSubs;
     static constexpr int kStage = 2 * kTile * kRowBytes + 2 * kTile * kGroups * 2;
     static constexpr int kHeadTiles = HT / 8;
@@ -74,7 +76,7 @@ struct Cfg {
     // resident CTAs: what the registers of q, outputs and scales leave room for
     static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 || HT == 16 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
-    static constexpr int kStages = kFit > 6 ? 6 : kFit;
+    static constexpr int kStages = kFit > 4 ? 4 : kFit;
     static_assert(kStages >= 2, "a ring of two tiles at least");
     static constexpr int kRing = kStages * kStage;
     static_assert(kRing >= kResult, "a finished ring holds a result");
