@@ -219,7 +219,8 @@ __device__ __forceinline__ long long costOf(int len) {
 // Where a walk over a warp's range is: the unit, how much of the range lies behind what it takes of that unit.  Kept in
 // shared memory, read and written by all lanes alike: the loop over a unit's tiles has no use for it.
 struct Walk {
-    int seq, sub, tiles, len, budget, pad;
+    int seq, sub, tiles, len, budget;
+    float shift; // of the scores of the unit in work, where they need one
 
     // To the next unit: how many of its tiles are in the range (0: the range has ended).
     template <int TILE>
@@ -594,7 +595,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 
             int token0 = tile * TILE;
             // from this token on a tile needs more than the plain arithmetic: a distance bias, tokens behind the end
-            const int special = a.alibi != nullptr ? 0 : len - TILE + 1;
+            int special = a.alibi != nullptr ? 0 : max(len - TILE + 1, 0);
+            // Beyond 2^20 a score's own rounding is as large as what the V scales add.  Then the maximum is the scores' alone, and p is
+            // taken relative to it and to 2^shift, which follows the V scales; `special` is -1 from there on, and shift in shared memory.
+            float &shift = walks[2 * warp + 1].shift;
             do {
                 waitCopies<S - 2>();
                 __syncwarp();
@@ -695,7 +699,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     f[n][0] = factor[n][0];
                     f[n][1] = factor[n][1];
                 }
+                bool move = false; // the maximum does rarely
                 if (token0 >= special) {
+                    move = special < 0;
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
                         f[n][0] = f[n][1] = 1.f;
@@ -735,7 +741,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     reach[r] = __uint_as_float(max(max(m & 0xffffu, m >> 16), kLeastScale) | 0x47800000u); // 2^16 (1 + bits / 2^23)
                 }
                 constexpr float kBias = 65536.f + 126.9f;
-                bool move = false; // the maximum does rarely
+                float base[NH][2]; // p = exp2(s * f - base)
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+                    base[n][0] = top[n][0];
+                    base[n][1] = top[n][1];
+                }
 #pragma unroll
                 for (int n = 0; n < NH; ++n) {
 #pragma unroll
@@ -760,25 +771,78 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         }
                         reach[r] = static_cast<float>(most) * 0.0078125f - 126.9f;
                     }
+                    float now[NH][2];
+                    auto largest = [&](float with_reach) {
+                        bool far = false;
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                float m = top[n][x];
+#pragma unroll
+                                for (int r = 0; r < 2 * SUBS; ++r) {
+                                    m = fmaxf(m, fmaf(s[r >> 1][n][2 * (r & 1) + x], f[n][x], with_reach * reach[r]));
+                                }
+                                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                                now[n][x] = m;
+                                far |= fabsf(m) >= 1048576.f;
+                            }
+                        }
+                        return far;
+                    };
+                    const bool was = special < 0, by_score = was || __any_sync(0xffffffffu, largest(1.f));
+                    const float shift_before = was ? shift : 0.f;
+                    float shift_now = 0.f;
+                    if (by_score) {
+                        special = -1;
+                        shift_now = reach[0];
+#pragma unroll
+                        for (int r = 1; r < 2 * SUBS; ++r) {
+                            shift_now = fmaxf(shift_now, reach[r]);
+                        }
+                        shift_now = fmaxf(shift_now, __shfl_xor_sync(0xffffffffu, shift_now, 4));
+                        shift_now = fmaxf(shift_now, __shfl_xor_sync(0xffffffffu, shift_now, 8));
+                        shift_now = ceilf(fmaxf(shift_now, __shfl_xor_sync(0xffffffffu, shift_now, 16)));
+                        shift_now = was ? fmaxf(shift_before, shift_now) : shift_now;
+                        __syncwarp();
+                        shift = shift_now;
+                        __syncwarp();
+                        // whole products, so that the largest one less the maximum is 0
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                                for (int r = 0; r < 2 * SUBS; ++r) {
+                                    s[r >> 1][n][2 * (r & 1) + x] = __fmul_rn(s[r >> 1][n][2 * (r & 1) + x], f[n][x]);
+                                }
+                                f[n][x] = 1.f;
+                            }
+                        }
+                        largest(0.f);
+                    }
+                    const float more = shift_before - shift_now;
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            float now = top[n][x];
-#pragma unroll
-                            for (int r = 0; r < 2 * SUBS; ++r) {
-                                now = fmaxf(now, fmaf(s[r >> 1][n][2 * (r & 1) + x], f[n][x], reach[r]));
-                            }
-                            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
-                            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
-                            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
-                            const float alpha = exp2Fast(top[n][x] - now); // the first time: 0
-                            top[n][x] = now;
+                            const float alpha = exp2Fast((top[n][x] - now[n][x]) + more); // the first time: 0
+                            top[n][x] = base[n][x] = now[n][x];
                             sum[n][x] *= alpha;
 #pragma unroll
                             for (int j = 0; j < HD / 16; ++j) {
                                 o[n][j][x] *= alpha;
                                 o[n][j][2 + x] *= alpha;
+                            }
+                            if (by_score) {
+#pragma unroll
+                                for (int r = 0; r < 2 * SUBS; ++r) {
+                                    float &score = s[r >> 1][n][2 * (r & 1) + x];
+                                    score = (score - top[n][x]) - shift_now;
+                                }
+                                base[n][x] = 0.f;
                             }
                         }
                     }
@@ -789,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     for (int n = 0; n < NH; ++n) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            s[u][n][i] = exp2Fast(fmaf(s[u][n][i], f[n][i & 1], -top[n][i & 1]));
+                            s[u][n][i] = exp2Fast(fmaf(s[u][n][i], f[n][i & 1], -base[n][i & 1]));
                         }
                         sum[n][0] += s[u][n][0] + s[u][n][2];
                         sum[n][1] += s[u][n][1] + s[u][n][3];
@@ -841,6 +905,21 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 stage = stage == ring_addr + (S - 1) * C::kStage ? ring_addr : stage + C::kStage;
             } while (--left > 0);
 
+            if (special < 0) { // back to the maximum alone
+                const float up = exp2Fast(shift);
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+                    sum[n][0] *= up;
+                    sum[n][1] *= up;
+#pragma unroll
+                    for (int j = 0; j < HD / 16; ++j) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[n][j][i] *= up;
+                        }
+                    }
+                }
+            }
             // the unit's rows, or this warp's piece of it
             const Walk done = work;
             const long long unit_first = place - tile;

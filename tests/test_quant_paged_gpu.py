@@ -1,6 +1,7 @@
 """GPU checks of the operators over quantised pools against plain 64-bit forms: codes and scales bit for bit, values read
 back bit for bit, attention within bounds that follow from the roundings of its arithmetic."""
 import contextlib
+import math
 import os
 
 import pytest
@@ -313,6 +314,43 @@ def test_attention_over_values_of_all_sizes(ib, bits):
     got = ib.quant_paged_attention(q, pools[0], pools[1], pools[2], big, tables, lens.cuda(), None, 0.1)
     want, bound = qh.attend_bound(q, (*pools[:3], big), tables, lens, 0.1, bits, BF16)
     qh.close(got, want, bound, "large V")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd", [64, 128, 192])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e9, 1e14])
+def test_attention_over_scores_of_any_size(ib, size, hd, bits):
+    """Scores of up to `size`: their softmax is one token's row (the largest score stands out by far more than fp32 loses of it), and
+    the output is that row rounded to the type."""
+    g = torch.Generator().manual_seed(hd)
+    lens, bs, kvh, heads = [300, 37, 1], 16, 2, 8
+    pools = qh.random_pools(g, 30, kvh, bs, hd, hd, bits)
+    pools[2].mul_(1e3)
+    pools[3].mul_(1e-3)
+    tables = qh.tables_for(g, lens, bs, 30)
+    lens_t = torch.tensor(lens)
+    q = torch.randn((3, heads, hd), generator=g).to(BF16).cuda()
+    for sign in (1.0, -1.0):
+        scale = sign * size / 1e3 / hd ** 0.5
+        got = ib.quant_paged_attention(q, *pools, tables, lens_t.cuda(), None, scale)
+        assert bool(torch.isfinite(got).all())
+        for i, n in enumerate(lens):
+            t = torch.arange(n, device="cuda")
+            block, off = tables[i][t // bs], t % bs
+            k, v = (qh.values(pools[x][block, :, off], pools[x + 2][block, :, off], bits) for x in (0, 1))
+            s = torch.einsum("hgd,nhd->hgn", q[i].double().view(kvh, 4, hd), k) * scale
+            best = s.max(-1)
+            second = s.scatter(-1, best.indices[..., None], -float("inf")).amax(-1)
+            # fp32 loses 2^-18 of sum |q k| at most, the bound of attend_bound; 40 more leave nothing of the second
+            lost = torch.einsum("hgd,nhd->hgn", q[i].double().view(kvh, 4, hd).abs(), k.abs()).amax(-1) * abs(scale) * 2.0 ** -17
+            clear = best.values - second > lost + 40
+            assert int(clear.sum()) >= (4 if size > 1e3 else 1)
+            want = torch.stack([v[best.indices[h], h] for h in range(kvh)])  # [kvh, g, hd]
+            err = (got[i].double().view(kvh, 4, hd) - want).abs()
+            # the weight is rounded to fp16 and the sum divided by p: 2^-11 + 2^-20, and half a step of bf16; the n - 1 other tokens weigh
+            # less than e^-40 each
+            ok = err <= want.abs() * (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) + n * math.exp(-40) * v.abs().max()
+            assert bool(ok[clear].all()), (size, sign, i)
 
 
 @pytest.mark.parametrize("bits", [4, 8])
