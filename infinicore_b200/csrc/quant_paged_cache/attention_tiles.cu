@@ -88,8 +88,14 @@ struct Cfg {
 
 __device__ __forceinline__ unsigned smemAddr(const void *p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
 
-__device__ __forceinline__ void copy16(unsigned dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void copy16(unsigned dst, const void *src, unsigned long long policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+}
+// Codes and scales are read once: they leave the L2 first, tables, q and partial results stay.
+__device__ __forceinline__ unsigned long long readOnce() {
+    unsigned long long p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
 }
 __device__ __forceinline__ void commitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -362,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     unsigned char *ring = smem + warp * C::kRing;
     if (start < total) {
         const Magic magic;
+        const unsigned long long policy = readOnce();
         Walk &copies = walks[2 * warp], &work = walks[2 * warp + 1];
         int tile, left;  // of the unit in work: present tile, tiles from there on in the range
         long long place; // of the present tile on the line
@@ -445,13 +452,13 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     const unsigned to = dst + r * C::kRowBytes + ((c ^ swz) << 4);
                     if constexpr (DENSE) {
                         constexpr int kOfRun = kCopies / kRuns; // copies of a run are 512 bytes apart
-                        copy16(to, k_run[j / kOfRun] + j % kOfRun * 512);
-                        copy16(to + TILE * C::kRowBytes, v_run[j / kOfRun] + j % kOfRun * 512);
+                        copy16(to, k_run[j / kOfRun] + j % kOfRun * 512, policy);
+                        copy16(to + TILE * C::kRowBytes, v_run[j / kOfRun] + j % kOfRun * 512, policy);
                     } else {
                         const int sub = SUBS == 1 ? 0 : 32 * j / CPR / 16; // where there are two, 16 rows are whole rounds of the warp
                         const unsigned in = static_cast<unsigned>(r & 7) * code_slot + c * 16;
-                        copy16(to, ((r & 8) ? k_run[kRuns == 1 ? 0 : 2 * sub + 1] : k_run[kRuns == 1 ? 0 : 2 * sub]) + in);
-                        copy16(to + TILE * C::kRowBytes, ((r & 8) ? v_run[kRuns == 1 ? 0 : 2 * sub + 1] : v_run[kRuns == 1 ? 0 : 2 * sub]) + in);
+                        copy16(to, ((r & 8) ? k_run[kRuns == 1 ? 0 : 2 * sub + 1] : k_run[kRuns == 1 ? 0 : 2 * sub]) + in, policy);
+                        copy16(to + TILE * C::kRowBytes, ((r & 8) ? v_run[kRuns == 1 ? 0 : 2 * sub + 1] : v_run[kRuns == 1 ? 0 : 2 * sub]) + in, policy);
                     }
                 }
                 // scales: 8 rows are one run of NG chunks
@@ -463,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         b = r == k ? block[k] : b;
                         at = r == k ? first_slot[k] : at;
                     }
-                    copy16(dst + 2 * TILE * C::kRowBytes + lane * 16, s_lane + static_cast<unsigned long long>(b) * scale_block + at * (2u * NG));
+                    copy16(dst + 2 * TILE * C::kRowBytes + lane * 16, s_lane + static_cast<unsigned long long>(b) * scale_block + at * (2u * NG), policy);
                 }
                 f_half += TILE / 8;
                 if (--f_left == 0) {
