@@ -13,7 +13,7 @@
  *                                                                     for each 32 elements)
  * Any block, head and slot strides; the last stride is 1.  Head sizes are multiples of 32 up to 1024.
  *
- * Quantising a group of values x with A = max |x| and Q = 127 (I8) or 7 (U8):
+ * Scales are never negative.  Quantising a group of values x with A = max |x| and Q = 127 (I8) or 7 (U8):
  *   scale = A / Q rounded to fp32, then to bf16 (both to nearest even), or 0 where that is below 2^-126;
  *   code  = x / scale to the nearest integer, halves away from zero, so |code| <= Q;
  *   a group that holds an infinity or a NaN gets the scale NaN and codes 0: it reads back as NaN.
