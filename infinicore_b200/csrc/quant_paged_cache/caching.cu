@@ -5,6 +5,8 @@
 // codes), a row a power of two of lanes, and let one lane move its elements of the K row and of the V row of kTokens
 // tokens, so that all loads are in flight before the first is used.  Consecutive lanes take consecutive words, so every
 // access of a warp covers whole rows.  A step's rows are a launch's latency; a prefill's are bound by HBM.
+// Measured with 8 heads of 128, bf16: 64 rows at 8 bits 2.2 us to write and 2.2 to read; 16384 rows at 4 bits 17.7 us
+// (4.9 TB/s) and 16.7 (5.1); 65536 rows at 4 bits read in 60.6 (5.7).
 //
 // Quantising without a division per element: with s the group's scale, code = x / s to the nearest, halves away from
 // zero, is the nearest integer to x * r for r = (1 + 2^-21) / s to 1.5 ulp.  x has at most 11 significant bits and s 8, so
