@@ -678,3 +678,67 @@ def test_refusals_reach_python(ib):
     assert e.value.status == 12
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ib.quant_paged_cache_read(*pools, slots.cpu())
+
+
+# ---- calls that share, repeat or leave out --------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_sequences_that_share_pages_and_a_page_twice_in_a_table(ib, hd, bits):
+    """One table for all sequences, by a stride of zero; and tables that repeat pages within a sequence and between them."""
+    g = torch.Generator().manual_seed(hd)
+    pools = qh.random_pools(g, 20, 2, 16, hd, hd, bits)
+    lens = torch.tensor([300, 1, 0, 257, 32, 299])
+    q = torch.randn((6, 8, hd), generator=g).to(BF16).cuda()
+    one = torch.randperm(20, generator=g)[:19].cuda()
+    shared = one[None].expand(6, 19)
+    assert shared.stride(0) == 0
+    repeated = torch.randint(0, 3, (6, 19), generator=g).cuda()
+    for tables in (shared, repeated):
+        got = ib.quant_paged_attention(q, *pools, tables, lens.cuda(), None, hd ** -0.5)
+        want, bound = qh.attend_bound(q, pools, tables, lens, hd ** -0.5, bits, BF16)
+        qh.close(got, want, bound, "shared" if tables is shared else "repeated")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("hd", [64, 128, 192])
+def test_a_query_that_is_no_number_spoils_its_own_row_only(ib, hd, dtype, bits):
+    """A NaN in q makes its scores NaN; an infinity makes them infinite or NaN, whose softmax is NaN.  Heads that share a pass
+    with such a one, and one of subnormal numbers, keep their values."""
+    g = torch.Generator().manual_seed(hd + bits)
+    lens = torch.tensor([200, 1, 33])
+    pools = qh.random_pools(g, 20, 2, 16, hd, hd, bits)
+    tables = qh.tables_for(g, lens.tolist(), 16, 20)
+    q = torch.randn((3, 8, hd), generator=g).to(dtype).cuda()
+    q[:, 3] *= torch.finfo(dtype).smallest_normal / 8
+    clean = q.clone()
+    q[0, 1, 5], q[1, 2, 0], q[2, 6, hd - 1] = float("nan"), float("inf"), -float("inf")
+    got = ib.quant_paged_attention(q, *pools, tables, lens.cuda(), None, hd ** -0.5)
+    want, bound = qh.attend_bound(clean, pools, tables, lens, hd ** -0.5, bits, dtype)
+    for i, h in ((0, 1), (1, 2), (2, 6)):
+        assert bool(got[i, h].isnan().all()), (i, h)
+        got[i, h], want[i, h], bound[i, h] = 0, 0, 0
+    qh.close(got, want, bound, "beside it")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("width", [1, 64, 900])
+def test_a_large_batch_that_is_mostly_empty(ib, width, bits):
+    """3001 sequences of which one in 37 has tokens, in tables of one page, of as many as a short table may have, and far wider
+    than any sequence: the rows of the empty ones stay as they were."""
+    g = torch.Generator().manual_seed(width)
+    lens = [int(torch.randint(1, min(16 * width, 200) + 1, (1,), generator=g)) if i % 37 == 5 else 0 for i in range(3001)]
+    blocks = sum(-(-n // 16) for n in lens)
+    pools = qh.random_pools(g, blocks, 2, 16, 64, 64, bits)
+    tables = torch.zeros((3001, width), dtype=torch.int64, device="cuda")
+    narrow = qh.tables_for(g, lens, 16, blocks)
+    tables[:, :narrow.shape[1]] = narrow
+    q = torch.randn((3001, 8, 64), generator=g).to(FP16).cuda()
+    out = torch.full_like(q, 3.0)
+    got = ib.quant_paged_attention(q, *pools, tables, torch.tensor(lens).cuda(), None, 0.125, out=out)
+    live = torch.tensor([i for i, n in enumerate(lens) if n]).cuda()
+    want, bound = qh.attend_bound(q[live], pools, tables[live], torch.tensor([n for n in lens if n]), 0.125, bits, FP16)
+    qh.close(got[live], want, bound, f"width {width}")
+    empty = torch.tensor([n == 0 for n in lens]).cuda()
+    assert bool((got[empty] == 3).all())
