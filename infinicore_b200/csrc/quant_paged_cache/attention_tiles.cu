@@ -44,7 +44,9 @@ constexpr int kThreads = kWarps * 32;
 // What a unit costs beside its tiles, in tiles: the time of 64 tokens.  Measured at 40 ragged sequences (64/8 heads of 128, 4 bits): 0
 // tokens 64 us, 32 43.5, 64 41.0, 128 40.7; at 62 sequences of 200 to 2000 32.1, 31.2, 30.2, 31.0.
 constexpr int unitCost(int tile) { return 64 / tile; }
-constexpr int minRange(int tile) { return unitCost(tile) + 2; } // of a warp: at least two tiles of a unit's first range
+// Of a warp: at least two tiles of a unit's first range.  More leaves fewer pieces to combine but warps idle: 6, 12, 24 instead of 2 take
+// 13 sequences of 1 to 30001 (16/1 heads of 256, 8 bits) from 25.6 us to 28.5, 29.9, 39.8, the 62 sequences from 28.7 to 28.7, 38.2, 45.0.
+constexpr int minRange(int tile) { return unitCost(tile) + 2; }
 constexpr float kSlack = 8.f;      // in the log2 domain; 2^8 is far inside fp16
 constexpr unsigned kLeastScale = 27u << 7; // V scales count as at least 2^-100 for the maximum: an all-zero row stays finite
 
@@ -1238,8 +1240,8 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     plan.combine_heads = static_cast<long long>(plan.tasks) * heads > 8ll * props.sm_count ? heads : 1;
     plan.combine_parts = heads / plan.combine_heads;
     if (!plan.unit_of_cta) {
-    plan.tasks_bytes = (sizeof(Task) * plan.tasks + 255) / 256 * 256;
-    plan.workspace_bytes = plan.tasks_bytes + sizeof(float) * 2 * plan.grid * static_cast<size_t>(var.record);
+        plan.tasks_bytes = (sizeof(Task) * plan.tasks + 255) / 256 * 256;
+        plan.workspace_bytes = plan.tasks_bytes + sizeof(float) * 2 * plan.grid * static_cast<size_t>(var.record);
     }
     // n / halves for n < 2^31 as mulhi(n, magic) >> shift: magic = floor(2^(32 + shift) / halves) + 1 with 2^shift < halves, which is
     // below 2^32 and off by at most halves, and n * halves < 2^(32 + shift); 2^(31) and one shift less for a power of two
