@@ -2,6 +2,7 @@
 #ifndef INFINIOP_B200_QUANT_ATTENTION_H
 #define INFINIOP_B200_QUANT_ATTENTION_H
 
+#include "lengths.h"
 #include "quant_pool.h"
 
 namespace b200::quant_paged_cache {
@@ -46,10 +47,7 @@ __device__ __forceinline__ long long indexAt(const AttentionArgs &a, const void 
 
 // Length of a sequence, never beyond what its row of the table can name.
 __device__ __forceinline__ int lengthOf(const AttentionArgs &a, int seq) {
-    const long long n = indexAt(a, a.seq_lens, seq);
-    const long long most = static_cast<long long>(a.max_blocks) * a.block_size;
-    const long long len = n < most ? n : most;
-    return len > 0x7fffffffLL ? 0x7fffffff : static_cast<int>(len);
+    return liveTokens(indexAt(a, a.seq_lens, seq), static_cast<long long>(a.max_blocks) * a.block_size);
 }
 
 // A block-table entry; in checked mode one outside the pool raises a flag and becomes block 0.
