@@ -220,6 +220,7 @@ static AttentionArgs makeArgs(const AttentionInfo &I) {
     a.block_size = static_cast<int>(I.pools.block_size);
     a.max_blocks = static_cast<int>(I.max_blocks);
     a.index_is_64 = I.index_dtype == INFINI_DTYPE_I64 ? 1 : 0;
+    a.length_kind = a.index_is_64 ? kLength64 : I.index_dtype == INFINI_DTYPE_U32 ? kLengthU32 : kLength32;
     a.is_bf16 = I.dtype == INFINI_DTYPE_BF16 ? 1 : 0;
     a.q_seq = I.q_seq;
     a.q_head = I.q_head;

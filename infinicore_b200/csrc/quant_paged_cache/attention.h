@@ -31,6 +31,7 @@ struct AttentionArgs {
     int num_seqs, num_heads, num_kv_heads, group; // group: q heads of a kv head
     int head_size, block_size, max_blocks;
     int index_is_64, is_bf16;
+    int length_kind; // LengthKind
     long long q_seq, q_head, o_seq, o_head, table_seq;
     long long k_block, k_head, k_slot, v_block, v_head, v_slot;             // bytes
     long long ks_block, ks_head, ks_slot, vs_block, vs_head, vs_slot;       // elements
@@ -47,7 +48,7 @@ __device__ __forceinline__ long long indexAt(const AttentionArgs &a, const void 
 
 // Length of a sequence, never beyond what its row of the table can name.
 __device__ __forceinline__ int lengthOf(const AttentionArgs &a, int seq) {
-    return liveTokens(indexAt(a, a.seq_lens, seq), static_cast<long long>(a.max_blocks) * a.block_size);
+    return liveTokens(storedLength(a.seq_lens, seq, a.length_kind), static_cast<long long>(a.max_blocks) * a.block_size);
 }
 
 // A block-table entry; in checked mode one outside the pool raises a flag and becomes block 0.

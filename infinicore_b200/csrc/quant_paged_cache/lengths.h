@@ -11,6 +11,15 @@
 
 namespace b200::quant_paged_cache {
 
+// How a length is stored: I64, I32 or U32.
+enum LengthKind : int { kLength64 = 0, kLength32 = 1, kLengthU32 = 2 };
+
+QUANT_HOST_DEVICE long long storedLength(const void *lens, long long i, int kind) {
+    return kind == kLength64   ? static_cast<const long long *>(lens)[i]
+         : kind == kLengthU32 ? static_cast<long long>(static_cast<const unsigned *>(lens)[i])
+                              : static_cast<long long>(static_cast<const int *>(lens)[i]);
+}
+
 // Tokens of a sequence whose stored length is n: none where n <= 0, never more than `most`, which its row of the table can
 // name.  Compared in 64 bits: a length below -2^31 that were narrowed first could come out positive.
 QUANT_HOST_DEVICE int liveTokens(long long n, long long most) {
