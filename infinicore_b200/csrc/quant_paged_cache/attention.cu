@@ -56,8 +56,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) quantAttentionRowsKernel(const
     extern __shared__ float smem[]; // q[head] | per warp: m, l, acc[head]
     const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.num_heads));
     const int seq = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.num_heads));
-    const int len = lengthOf(a, seq);
-    if (len <= 0) {
+    const long long len = tokensOf(a, seq);
+    if (len == 0) {
         return;
     }
     const int kv_head = head / a.group;
@@ -77,9 +77,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) quantAttentionRowsKernel(const
     for (int i = 0; i < kMaxPairs; ++i) {
         acc[i] = make_float2(0.f, 0.f);
     }
-    for (int t = warp; t < len; t += kRowWarps) {
-        const int page = t / a.block_size;
-        const long long off = t - page * a.block_size;
+    // a table may name more than 2^31 tokens: they are counted in 64 bits, and pages without a division
+    long long page = warp / a.block_size;
+    int off = warp % a.block_size;
+    for (long long t = warp; t < len; t += kRowWarps) {
         const long long block = blockAt(a, seq * a.table_seq, page);
         const unsigned char *k = a.k_codes + block * a.k_block + kv_head * a.k_head + off * a.k_slot;
         const unsigned char *v = a.v_codes + block * a.v_block + kv_head * a.v_head + off * a.v_slot;
@@ -112,6 +113,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) quantAttentionRowsKernel(const
                 acc[i].x = fmaf(p, x.x, acc[i].x * alpha);
                 acc[i].y = fmaf(p, x.y, acc[i].y * alpha);
             }
+        }
+        for (off += kRowWarps; off >= a.block_size; off -= a.block_size) {
+            ++page;
         }
     }
     float *mine = merge + warp * merge_stride;

@@ -47,12 +47,12 @@ __device__ __forceinline__ long long indexAt(const AttentionArgs &a, const void 
 }
 
 // Length of a sequence, never beyond what its row of the table can name.
-__device__ __forceinline__ int lengthOf(const AttentionArgs &a, int seq) {
+__device__ __forceinline__ long long tokensOf(const AttentionArgs &a, int seq) {
     return liveTokens(storedLength(a.seq_lens, seq, a.length_kind), static_cast<long long>(a.max_blocks) * a.block_size);
 }
 
 // A block-table entry; in checked mode one outside the pool raises a flag and becomes block 0.
-__device__ __forceinline__ long long blockAt(const AttentionArgs &a, long long row, int i) {
+__device__ __forceinline__ long long blockAt(const AttentionArgs &a, long long row, long long i) {
     const long long b = indexAt(a, a.block_tables, row + i);
     if (a.check_indices && static_cast<unsigned long long>(b) >= static_cast<unsigned long long>(a.num_blocks)) {
         atomicOr(a.kernel_flags, INFINIOP_KERNEL_FLAG_BLOCK_OUT_OF_RANGE);

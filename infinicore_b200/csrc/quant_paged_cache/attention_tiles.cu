@@ -219,6 +219,9 @@ struct TilesArgs {
     int out_words;            // rows of out can be stored 8 bytes at a time
 };
 
+// planTiles takes no table that names more than kMostTokensInt
+__device__ __forceinline__ int lengthOf(const AttentionArgs &a, int seq) { return static_cast<int>(tokensOf(a, seq)); }
+
 template <int TILE>
 __device__ __forceinline__ int tilesOf(int len) {
     return len > 0 ? (len + TILE - 1) / TILE : 0;
@@ -1211,11 +1214,12 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     const Variant var = variantFor(I);
     const unsigned long long group = I.num_heads / P.num_kv_heads;
     const unsigned long long head_tiles = (group + var.heads - 1) / var.heads;
-    const unsigned long long tiles = (static_cast<unsigned long long>(I.max_blocks) * P.block_size + var.tile - 1) / var.tile;
+    const unsigned long long tokens = static_cast<unsigned long long>(I.max_blocks) * P.block_size; // 31 and 17 bits
+    const unsigned long long tiles = (tokens + var.tile - 1) / var.tile;
     const unsigned long long subs = head_tiles * P.num_kv_heads;
     const long double line = static_cast<long double>(tiles + unitCost(var.tile)) * subs * I.num_seqs;
     const unsigned long long at_most = static_cast<unsigned long long>(props.sm_count) * var.ctas;
-    if (tiles > 0x0fffffffull || line > 9e17L || line / at_most > 1e9L) {
+    if (tokens > static_cast<unsigned long long>(kMostTokensInt) || line > 9e17L || line / at_most > 1e9L) {
         plan.eligible = false; // positions would not fit
         return plan;
     }

@@ -21,14 +21,11 @@ QUANT_HOST_DEVICE long long storedLength(const void *lens, long long i, int kind
 }
 
 // Tokens of a sequence whose stored length is n: none where n <= 0, never more than `most`, which its row of the table can
-// name.  Compared in 64 bits: a length below -2^31 that were narrowed first could come out positive.
-QUANT_HOST_DEVICE int liveTokens(long long n, long long most) {
-    if (n <= 0) {
-        return 0;
-    }
-    const long long len = n < most ? n : most;
-    return len > 0x7fffffffLL ? 0x7fffffff : static_cast<int>(len);
-}
+// name.  In 64 bits: a length below -2^31 that were narrowed could come out positive, and a table may name more than 2^31 tokens.
+QUANT_HOST_DEVICE long long liveTokens(long long n, long long most) { return n <= 0 ? 0 : n < most ? n : most; }
+
+// What a table may name for a kernel that counts tokens in an int, a whole tile of 64 behind the last one included.
+constexpr long long kMostTokensInt = 0x7fffffffLL - 127;
 
 } // namespace b200::quant_paged_cache
 

@@ -105,3 +105,22 @@ def test_unsigned_lengths_beyond_the_table_are_cut(bits, path, monkeypatch):
     for t in made:
         t.destroy_desc()
     destroy_handle(handle)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_table_that_names_more_tokens_than_an_int_holds(bits):
+    """32769 pages of 65536 slots in a table whose rows are one row; sequences of a few tokens, and one into the second page."""
+    import infinicore_b200 as ib
+
+    g = torch.Generator().manual_seed(bits)
+    pools = qh.random_pools(g, 2, 1, 65536, 64, 64, bits)
+    row = torch.full((32769,), 1 << 20, dtype=torch.int32)  # behind the sequences' ends: never looked at
+    row[:2] = torch.tensor([1, 0])
+    lens = torch.tensor([5, 65541, 0, 129], dtype=torch.int32)
+    q = torch.randn((4, 2, 64), generator=g).to(BF16).cuda()
+    out = torch.full_like(q, 5.0)
+    ib.quant_paged_attention(q, *pools, row.cuda()[None].expand(4, -1), lens.cuda(), None, 0.125, out=out)
+    want, bound = qh.attend_bound(q, pools, row[:2].cuda()[None].expand(4, -1), lens, 0.125, bits, BF16, None, torch.full_like(out, 5.0))
+    qh.close(out, want, bound)
+    assert bool((out[2] == 5).all())
