@@ -22,9 +22,11 @@
 // every second element of V keeps a factor of 16 that its output is rid of at the end.
 //   q is held in fp16 times a power of two that makes its largest element 1/2..1: exact for every element above
 // 2^-13 of that (fp16 and bf16 both have at most 11 bits).
-//   w is rounded once to fp16.  To keep it in range for scales of any size the running maximum is taken over
-// score + (exponent of the token's largest V scale), so that w <= 2^kSlack; p is relative to the same maximum.  The
-// maximum moves only when a score passes it by more than kSlack, and only then are outputs rescaled.
+//   w is rounded once to fp16, as w = p * v_scale * 2^k with an exponent k of its own for each head and group of V, so that every group of
+// an output has weights of full precision, whatever the sizes of the others.  k is settled at a unit's first tile: it makes the group's
+// largest weight 2^7..2^8.  It is settled again, from the same tile's scores once more, when a weight passes what fp16 holds; earlier
+// outputs are scaled then, by powers of two.  Where the k of a head's groups are within 2^6 of each other, as they are unless V's channels differ
+// in size by far more than that, the smallest serves them all, inside the maximum: w = p * v_scale ("even").
 //   Sums, maxima and outputs are fp32.
 //
 // Measured at 32/8 heads of 128, 64 x 4096 tokens, the combine kernel's share of 3 to 5 us included: 8 bits 96 us (5.7 TB/s of
@@ -47,8 +49,15 @@ constexpr int unitCost(int tile) { return 64 / tile; }
 // Of a warp: at least two tiles of a unit's first range.  More leaves fewer pieces to combine but warps idle: 6, 12, 24 instead of 2 take
 // 13 sequences of 1 to 30001 (16/1 heads of 256, 8 bits) from 25.6 us to 28.5, 29.9, 39.8, the 62 sequences from 28.7 to 28.7, 38.2, 45.0.
 constexpr int minRange(int tile) { return unitCost(tile) + 2; }
-constexpr float kSlack = 8.f;      // in the log2 domain; 2^8 is far inside fp16
-constexpr unsigned kLeastScale = 27u << 7; // V scales count as at least 2^-100 for the maximum: an all-zero row stays finite
+// What the weights are relative to is settled at a unit's first tile and again when a weight does not fit fp16 (or p comes to kMostP).
+// p = exp2(score - top), in the log2 domain: top is then kBelow above the largest score so far.
+constexpr float kBelow = 16.f;
+constexpr float kMostP = 1.2379400392853803e27f; // 2^90
+constexpr float kMostFactor = 126.f; // exponent of a group's factor at most (its reciprocal is a normal number), and at first
+constexpr float kLargest = 7.f;      // exponent of a group's largest weight when its factor is set: 2^8 below what fp16 holds
+constexpr float kEven = 6.f;         // factors of a head's groups whose exponents are this near count as one: the largest weight of each group
+                                     // is 2 or more then, and what is subnormal in fp16 is off by 2^-26 of it at most
+constexpr float kLeastCommon = -20.f, kMostCommon = 80.f; // exponents that such a one may have: p times it stays far inside fp32
 
 // What the combine kernel has to do for a unit: nothing, or to add this many pieces from this CTA's on.
 struct Task {
@@ -61,7 +70,7 @@ struct Piece {
     int seq, sub, tiles, used;
 };
 
-constexpr int kWalkBytes = 24;
+constexpr int kWalkBytes = 20;
 
 template <int BITS, int HD, int HT>
 struct Cfg {
@@ -78,7 +87,8 @@ struct Cfg {
     static constexpr int kHeadTiles = HT / 8;
     static constexpr int kStride = HD + 4;                    // floats: rows of two heads apart hit other banks
     static constexpr int kResult = HT * kStride * 4;
-    static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes);
+    static constexpr int kFactors = 2 * HT * (kGroups + 1) * 4; // of a warp: as they are, and as they are being settled
+    static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + kFactors + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes);
     // resident CTAs: what the registers of q, outputs and scales leave room for
     static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 || HT == 16 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
@@ -201,6 +211,35 @@ __device__ __forceinline__ unsigned codes8(const Magic &m, unsigned flipped) {
     return addHalves(__byte_perm(flipped, m.byte, SEL), kMinus1152);
 }
 
+// 2^e for a whole number e, -126 to 127
+__device__ __forceinline__ float powerOfTwo(float e) { return __uint_as_float(static_cast<unsigned>(static_cast<int>(e) + 127) << 23); }
+// x * 2^e for a whole number e up to 126, however low
+__device__ __forceinline__ float shifted(float x, float e) {
+    const float a = fmaxf(e, -126.f), b = fmaxf(e - a, -126.f);
+    return x * powerOfTwo(a) * powerOfTwo(b);
+}
+// The exponent of x >= 0; -127 of 0 and of subnormal numbers
+__device__ __forceinline__ float exponentOf(float x) { return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127); }
+// The largest among the eight lanes of a head
+__device__ __forceinline__ float largestOf(float m) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+    return fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+}
+
+// Columns x of a lane's outputs, those of a group's elements, times 2^e
+template <int BITS, int HD>
+__device__ __forceinline__ void scaleGroup(float (&o)[HD / 16][4], int group, int x, float e) {
+    const float by = e >= -126.f ? powerOfTwo(e) : 0.f;
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) {
+        if (BITS == 8 || j / 2 == group) {
+            o[j][x] *= by;
+            o[j][2 + x] *= by;
+        }
+    }
+}
+
 // ---- the line of tiles -------------------------------------------------------------------------------------
 
 struct TilesArgs {
@@ -235,7 +274,6 @@ __device__ __forceinline__ long long costOf(int len) {
 // shared memory, read and written by all lanes alike: the loop over a unit's tiles has no use for it.
 struct Walk {
     int seq, sub, tiles, len, budget;
-    float shift; // of the scores of the unit in work, where they need one
 
     // To the next unit: how many of its tiles are in the range (0: the range has ended).
     template <int TILE>
@@ -297,7 +335,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     extern __shared__ __align__(128) unsigned char smem[];
     float *results = reinterpret_cast<float *>(smem + kWarps * C::kRing);                                     // [warp][head][kStride]
     float2 *sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(results) + kWarps * C::kResult); // [warp][2][head]
-    Piece *pieces = reinterpret_cast<Piece *>(sums + kWarps * 2 * HT);                                        // [warp][2]
+    float *all_factors = reinterpret_cast<float *>(sums + kWarps * 2 * HT);                                   // [warp][old | new][group | least][head]
+    Piece *pieces = reinterpret_cast<Piece *>(all_factors + kWarps * (C::kFactors / 4));                                // [warp][2]
     Walk *walks = reinterpret_cast<Walk *>(pieces + kWarps * 2);                                              // [warp][copies | arithmetic]
     const int tid = static_cast<int>(pinned(threadIdx.x)), warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -609,12 +648,15 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 }
             }
 
+            // exponents of the groups' factors, and the least of a head's, which is in top and counts for all where `even`
+            float *const factors = all_factors + warp * (C::kFactors / 4);
+            bool even = false, fresh = true;
+
             int token0 = tile * TILE;
             // from this token on a tile needs more than the plain arithmetic: a distance bias, tokens behind the end
             int special = a.alibi != nullptr ? 0 : max(len - TILE + 1, 0);
-            // Beyond 2^20 a score's own rounding is as large as what the V scales add.  Then the maximum is the scores' alone, and p is
-            // taken relative to it and to 2^shift, which follows the V scales; `special` is -1 from there on, and shift in shared memory.
-            float &shift = walks[2 * warp + 1].shift;
+            // Beyond 2^20 a score's own rounding is seen in p.  Then scores are rounded before the maximum is taken off, so that the largest
+            // is off by nothing; `special` is -1 from there on.
             do {
                 waitCopies<S - 2>();
                 __syncwarp();
@@ -644,242 +686,267 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
                 };
 
-                // scores
-                float s[SUBS][NH][4]; // [.][.][token g, heads 2t and 2t + 1 | token g + 8]
+                unsigned weight[SUBS][NG][NH][2];
+                float add[NH][2];
+#pragma unroll 1
+                for (bool settle = fresh || special < 0;; settle = true) {
+                    // scores
+                    float s[SUBS][NH][4]; // [.][.][token g, heads 2t and 2t + 1 | token g + 8]
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) {
-                    unsigned ks[2][kWords];
-                    loadScales(ks[0], scales + u * (32 * NG));
-                    loadScales(ks[1], scales + u * (32 * NG) + 16 * NG);
-#pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[u][n][i] = 0.f;
-                        }
-                    }
-#pragma unroll
-                    for (int c = 0; c < CPR; c += 2) {
-                        unsigned w[4];
-                        loadMatrices(w, k_addr + u * (16 * C::kRowBytes) + (((c + m_chunk) ^ m_swz) << 4));
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) { // the two chunks
-                            const int j = c + x;
-                            if constexpr (BITS == 4) {
-                                unsigned lo[4], hi[4];
-                                codes4(magic, w[2 * x], lo);
-                                codes4(magic, w[2 * x + 1], hi);
-                                const float s0 = scaleAt(ks[0], j), s1 = scaleAt(ks[1], j);
-#pragma unroll
-                                for (int n = 0; n < NH; ++n) {
-                                    float d[4];
-                                    mmaFirst(d, lo[0], hi[0], lo[1], hi[1], qr[n][2 * j][0], qr[n][2 * j][1]);
-                                    mma(d, lo[2], hi[2], lo[3], hi[3], qr[n][2 * j + 1][0], qr[n][2 * j + 1][1]);
-                                    s[u][n][0] = fmaf(s0, d[0], s[u][n][0]);
-                                    s[u][n][1] = fmaf(s0, d[1], s[u][n][1]);
-                                    s[u][n][2] = fmaf(s1, d[2], s[u][n][2]);
-                                    s[u][n][3] = fmaf(s1, d[3], s[u][n][3]);
-                                }
-                            } else {
-                                const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
-                                const unsigned a0 = codes8<0x4140>(magic, lo), a1 = codes8<0x4140>(magic, hi);
-                                const unsigned a2 = codes8<0x4342>(magic, lo), a3 = codes8<0x4342>(magic, hi);
-#pragma unroll
-                                for (int n = 0; n < NH; ++n) {
-                                    mma(s[u][n], a0, a1, a2, a3, qr[n][j][0], qr[n][j][1]);
-                                }
-                            }
-                        }
-                    }
-                    if constexpr (BITS == 8) {
-                        const float s0 = scaleAt(ks[0], 0), s1 = scaleAt(ks[1], 0);
+                    for (int u = 0; u < SUBS; ++u) {
+                        unsigned ks[2][kWords];
+                        loadScales(ks[0], scales + u * (32 * NG));
+                        loadScales(ks[1], scales + u * (32 * NG) + 16 * NG);
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                s[u][n][i] *= i < 2 ? s0 : s1;
+                                s[u][n][i] = 0.f;
                             }
                         }
-                    }
-                }
-                unsigned vs[SUBS][2][kWords];
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) {
-                    loadScales(vs[u][0], scales + 2 * TILE * NG + u * (32 * NG));
-                    loadScales(vs[u][1], scales + 2 * TILE * NG + u * (32 * NG) + 16 * NG);
-                }
-                // scores in the log2 domain are s * f from here on
-                float f[NH][2];
+                        for (int c = 0; c < CPR; c += 2) {
+                            unsigned w[4];
+                            loadMatrices(w, k_addr + u * (16 * C::kRowBytes) + (((c + m_chunk) ^ m_swz) << 4));
 #pragma unroll
-                for (int n = 0; n < NH; ++n) {
-                    f[n][0] = factor[n][0];
-                    f[n][1] = factor[n][1];
-                }
-                bool move = false; // the maximum does rarely
-                if (token0 >= special) {
-                    move = special < 0;
+                            for (int x = 0; x < 2; ++x) { // the two chunks
+                                const int j = c + x;
+                                if constexpr (BITS == 4) {
+                                    unsigned lo[4], hi[4];
+                                    codes4(magic, w[2 * x], lo);
+                                    codes4(magic, w[2 * x + 1], hi);
+                                    const float s0 = scaleAt(ks[0], j), s1 = scaleAt(ks[1], j);
 #pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-                        f[n][0] = f[n][1] = 1.f;
-                    }
+                                    for (int n = 0; n < NH; ++n) {
+                                        float d[4];
+                                        mmaFirst(d, lo[0], hi[0], lo[1], hi[1], qr[n][2 * j][0], qr[n][2 * j][1]);
+                                        mma(d, lo[2], hi[2], lo[3], hi[3], qr[n][2 * j + 1][0], qr[n][2 * j + 1][1]);
+                                        s[u][n][0] = fmaf(s0, d[0], s[u][n][0]);
+                                        s[u][n][1] = fmaf(s0, d[1], s[u][n][1]);
+                                        s[u][n][2] = fmaf(s1, d[2], s[u][n][2]);
+                                        s[u][n][3] = fmaf(s1, d[3], s[u][n][3]);
+                                    }
+                                } else {
+                                    const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
+                                    const unsigned a0 = codes8<0x4140>(magic, lo), a1 = codes8<0x4140>(magic, hi);
+                                    const unsigned a2 = codes8<0x4342>(magic, lo), a3 = codes8<0x4342>(magic, hi);
 #pragma unroll
-                    for (int r = 0; r < 2 * SUBS; ++r) {
-                        const int u = r >> 1, i = 2 * (r & 1), token = token0 + 8 * r + g;
-                        const float far = static_cast<float>(token - (len - 1));
-#pragma unroll
-                        for (int n = 0; n < NH; ++n) {
-                            s[u][n][i] = fmaf(slope[n][0], far, s[u][n][i] * factor[n][0]);
-                            s[u][n][i + 1] = fmaf(slope[n][1], far, s[u][n][i + 1] * factor[n][1]);
+                                    for (int n = 0; n < NH; ++n) {
+                                        mma(s[u][n], a0, a1, a2, a3, qr[n][j][0], qr[n][j][1]);
+                                    }
+                                }
+                            }
                         }
-                        if (token >= len) { // no weight, whatever the scales are
+                        if constexpr (BITS == 8) {
+                            const float s0 = scaleAt(ks[0], 0), s1 = scaleAt(ks[1], 0);
 #pragma unroll
                             for (int n = 0; n < NH; ++n) {
-                                s[u][n][i] = s[u][n][i + 1] = -INFINITY;
-                            }
 #pragma unroll
-                            for (int k = 0; k < kWords; ++k) {
-                                vs[u][r & 1][k] = 0u;
+                                for (int i = 0; i < 4; ++i) {
+                                    s[u][n][i] *= i < 2 ? s0 : s1;
+                                }
                             }
                         }
                     }
-                }
+                    unsigned vs[SUBS][2][kWords];
+#pragma unroll
+                    for (int u = 0; u < SUBS; ++u) {
+                        loadScales(vs[u][0], scales + 2 * TILE * NG + u * (32 * NG));
+                        loadScales(vs[u][1], scales + 2 * TILE * NG + u * (32 * NG) + 16 * NG);
+                    }
+                    // scores in the log2 domain are s * f from here on
+                    float f[NH][2];
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        f[n][0] = factor[n][0];
+                        f[n][1] = factor[n][1];
+                    }
+                    if (token0 >= special) {
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+                            f[n][0] = f[n][1] = 1.f;
+                        }
+#pragma unroll
+                        for (int r = 0; r < 2 * SUBS; ++r) {
+                            const int u = r >> 1, i = 2 * (r & 1), token = token0 + 8 * r + g;
+                            const float far = static_cast<float>(token - (len - 1));
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                s[u][n][i] = fmaf(slope[n][0], far, s[u][n][i] * factor[n][0]);
+                                s[u][n][i + 1] = fmaf(slope[n][1], far, s[u][n][i + 1] * factor[n][1]);
+                            }
+                            if (token >= len) { // no weight, whatever the scales are
+#pragma unroll
+                                for (int n = 0; n < NH; ++n) {
+                                    s[u][n][i] = s[u][n][i + 1] = -INFINITY;
+                                }
+#pragma unroll
+                                for (int k = 0; k < kWords; ++k) {
+                                    vs[u][r & 1][k] = 0u;
+                                }
+                            }
+                        }
+                    }
 
-                // How far a token's weights can reach above its p: log2 of its largest V scale is at most bits / 128 - 126.9 for a
-                // bf16 with these bits (log2(1 + f) <= f + 0.0861).  The constant stays out; it is taken off with the maximum.
-                float reach[2 * SUBS]; // 65536 + bits / 128
-#pragma unroll
-                for (int r = 0; r < 2 * SUBS; ++r) {
-                    unsigned m = vs[r >> 1][r & 1][0];
-#pragma unroll
-                    for (int k = 1; k < kWords; ++k) {
-                        m = __vmaxu2(m, vs[r >> 1][r & 1][k]);
-                    }
-                    reach[r] = __uint_as_float(max(max(m & 0xffffu, m >> 16), kLeastScale) | 0x47800000u); // 2^16 (1 + bits / 2^23)
-                }
-                constexpr float kBias = 65536.f + 126.9f;
-                float base[NH][2]; // p = exp2(s * f - base)
-#pragma unroll
-                for (int n = 0; n < NH; ++n) {
-                    base[n][0] = top[n][0];
-                    base[n][1] = top[n][1];
-                }
-#pragma unroll
-                for (int n = 0; n < NH; ++n) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float high = fmaf(s[0][n][x], f[n][x], reach[0]);
-#pragma unroll
-                        for (int r = 1; r < 2 * SUBS; ++r) {
-                            high = fmaxf(high, fmaf(s[r >> 1][n][2 * (r & 1) + x], f[n][x], reach[r]));
-                        }
-                        move |= high > top[n][x] + (kSlack + kBias);
-                    }
-                }
-                if (__any_sync(0xffffffffu, move)) {
-                    // a NaN scale would count as 2^129: such a token counts without it
-#pragma unroll
-                    for (int r = 0; r < 2 * SUBS; ++r) {
-                        unsigned most = kLeastScale;
-#pragma unroll
-                        for (int k = 0; k < kWords; ++k) {
-                            const unsigned lo = vs[r >> 1][r & 1][k] & 0xffffu, hi = vs[r >> 1][r & 1][k] >> 16;
-                            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-                        }
-                        reach[r] = static_cast<float>(most) * 0.0078125f - 126.9f;
-                    }
-                    float now[NH][2];
-                    auto largest = [&](float with_reach) {
-                        bool far = false;
+                    if (__builtin_expect(settle, 0)) {
+                        float *const mine = factors + 2 * t; // of this lane's heads: eight lanes, the same
+                        bool far = special < 0;
+                        float now[NH][2];
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
-                                float m = top[n][x];
+                                float m = -INFINITY;
 #pragma unroll
                                 for (int r = 0; r < 2 * SUBS; ++r) {
-                                    m = fmaxf(m, fmaf(s[r >> 1][n][2 * (r & 1) + x], f[n][x], with_reach * reach[r]));
+                                    m = fmaxf(m, __fmul_rn(s[r >> 1][n][2 * (r & 1) + x], f[n][x]));
                                 }
-                                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                                now[n][x] = m;
-                                far |= fabsf(m) >= 1048576.f;
+                                m = largestOf(m);
+                                far |= fabsf(m) >= 1048576.f && m != -INFINITY;
+                                now[n][x] = ceilf(m) + kBelow; // a whole number
                             }
                         }
-                        return far;
+                        far = __any_sync(0xffffffffu, far);
+                        if (far) {
+                            special = -1;
+#pragma unroll
+                            for (int u = 0; u < SUBS; ++u) {
+#pragma unroll
+                                for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        s[u][n][i] = __fmul_rn(s[u][n][i], f[n][i & 1]);
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                f[n][0] = f[n][1] = 1.f;
+                            }
+                        }
+                        // p of before are smaller by 2^up now, and factors as much larger, up to their limit.  A group whose largest weight of this tile
+                        // would be 2^8 or more gets a factor that makes it 2^7.
+                        float up[NH][2];
+                        float *const next = mine + (NG + 1) * HT;
+                        bool near = !far;
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                top[n][x] += even ? mine[NG * HT + 8 * n + x] : 0.f;
+                                now[n][x] = fmaxf(now[n][x], top[n][x]);
+                                up[n][x] = now[n][x] - top[n][x];
+                                top[n][x] = now[n][x];
+                                float most = -INFINITY, least = INFINITY;
+#pragma unroll
+                                for (int j = 0; j < NG; ++j) {
+                                    float m = 0.f;
+#pragma unroll
+                                    for (int r = 0; r < 2 * SUBS; ++r) {
+                                        const float p = exp2Fast(fmaf(s[r >> 1][n][2 * (r & 1) + x], f[n][x], -now[n][x]));
+                                        m = fmaxf(m, fabsf(p * scaleAt(vs[r >> 1][r & 1], j)));
+                                    }
+                                    const float high = exponentOf(largestOf(m));
+                                    const float was = fresh ? kMostFactor : fminf(mine[j * HT + 8 * n + x] + up[n][x], kMostFactor);
+                                    const float is = high + was > kLargest ? kLargest - high : was;
+                                    next[j * HT + 8 * n + x] = is;
+                                    least = fminf(least, is);
+                                    most = fmaxf(most, is);
+                                }
+                                next[NG * HT + 8 * n + x] = least;
+                                near = near && most - least <= kEven && least >= kLeastCommon && least <= kMostCommon;
+                            }
+                        }
+                        const bool was_even = even;
+                        even = __all_sync(0xffffffffu, near);
+                        if (!fresh) {
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) {
+                                    const float common = mine[NG * HT + 8 * n + x], least = next[NG * HT + 8 * n + x];
+#pragma unroll
+                                    for (int j = 0; j < NG; ++j) {
+                                        const float was = was_even ? common : mine[j * HT + 8 * n + x];
+                                        scaleGroup<BITS, HD>(o[n], j, x, ((even ? least : next[j * HT + 8 * n + x]) - was) - up[n][x]);
+                                    }
+                                    sum[n][x] = shifted(shifted(shifted(sum[n][x], was_even ? -common : 0.f), -up[n][x]), even ? least : 0.f);
+                                }
+                            }
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                                for (int j = 0; j <= NG; ++j) {
+                                    mine[j * HT + 8 * n + x] = next[j * HT + 8 * n + x];
+                                }
+                                top[n][x] -= even ? next[NG * HT + 8 * n + x] : 0.f;
+                            }
+                        }
+                        __syncwarp();
+                        fresh = false;
+                    }
+                    // p, and the weights p * v_scale * factor in fp16: the one rounding to fewer bits
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        add[n][0] = add[n][1] = 0.f;
+                    }
+#pragma unroll
+                    for (int u = 0; u < SUBS; ++u) {
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                s[u][n][i] = exp2Fast(fmaf(s[u][n][i], f[n][i & 1], -top[n][i & 1]));
+                            }
+                            add[n][0] += s[u][n][0] + s[u][n][2];
+                            add[n][1] += s[u][n][1] + s[u][n][3];
+                        }
+                    }
+                    unsigned largest = 0;
+                    auto weigh = [&](auto factor) {
+#pragma unroll
+                        for (int j = 0; j < NG; ++j) {
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                const float by0 = factor(j, n, 0), by1 = factor(j, n, 1);
+#pragma unroll
+                                for (int u = 0; u < SUBS; ++u) {
+                                    const float v0 = scaleAt(vs[u][0], j), v1 = scaleAt(vs[u][1], j);
+                                    weight[u][j][n][0] = packHalves(s[u][n][0] * by0 * v0, s[u][n][1] * by1 * v0);
+                                    weight[u][j][n][1] = packHalves(s[u][n][2] * by0 * v1, s[u][n][3] * by1 * v1);
+                                    largest = __vmaxu2(largest, __vmaxu2(weight[u][j][n][0], weight[u][j][n][1]));
+                                }
+                            }
+                        }
                     };
-                    const bool was = special < 0, by_score = was || __any_sync(0xffffffffu, largest(1.f));
-                    const float shift_before = was ? shift : 0.f;
-                    float shift_now = 0.f;
-                    if (by_score) {
-                        special = -1;
-                        shift_now = reach[0];
-#pragma unroll
-                        for (int r = 1; r < 2 * SUBS; ++r) {
-                            shift_now = fmaxf(shift_now, reach[r]);
-                        }
-                        shift_now = fmaxf(shift_now, __shfl_xor_sync(0xffffffffu, shift_now, 4));
-                        shift_now = fmaxf(shift_now, __shfl_xor_sync(0xffffffffu, shift_now, 8));
-                        shift_now = ceilf(fmaxf(shift_now, __shfl_xor_sync(0xffffffffu, shift_now, 16)));
-                        shift_now = was ? fmaxf(shift_before, shift_now) : shift_now;
-                        __syncwarp();
-                        shift = shift_now;
-                        __syncwarp();
-                        // whole products, so that the largest one less the maximum is 0
-#pragma unroll
-                        for (int n = 0; n < NH; ++n) {
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                                for (int r = 0; r < 2 * SUBS; ++r) {
-                                    s[r >> 1][n][2 * (r & 1) + x] = __fmul_rn(s[r >> 1][n][2 * (r & 1) + x], f[n][x]);
-                                }
-                                f[n][x] = 1.f;
-                            }
-                        }
-                        largest(0.f);
+                    if (even) {
+                        weigh([](int, int, int) { return 1.f; });
+                    } else {
+                        weigh([&](int j, int n, int x) { return powerOfTwo(factors[j * HT + 8 * n + 2 * t + x]); });
                     }
-                    const float more = shift_before - shift_now;
+                    bool again = max(largest & 0xffffu, largest >> 16) >= 0x7c00u; // an infinity, or no number
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const float alpha = exp2Fast((top[n][x] - now[n][x]) + more); // the first time: 0
-                            top[n][x] = base[n][x] = now[n][x];
-                            sum[n][x] *= alpha;
-#pragma unroll
-                            for (int j = 0; j < HD / 16; ++j) {
-                                o[n][j][x] *= alpha;
-                                o[n][j][2 + x] *= alpha;
-                            }
-                            if (by_score) {
-#pragma unroll
-                                for (int r = 0; r < 2 * SUBS; ++r) {
-                                    float &score = s[r >> 1][n][2 * (r & 1) + x];
-                                    score = (score - top[n][x]) - shift_now;
-                                }
-                                base[n][x] = 0.f;
-                            }
-                        }
+                        again |= fmaxf(add[n][0], add[n][1]) > kMostP;
+                    }
+                    if (__builtin_expect(settle || !__any_sync(0xffffffffu, again), 1)) {
+                        break;
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) {
-#pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[u][n][i] = exp2Fast(fmaf(s[u][n][i], f[n][i & 1], -base[n][i & 1]));
-                        }
-                        sum[n][0] += s[u][n][0] + s[u][n][2];
-                        sum[n][1] += s[u][n][1] + s[u][n][3];
-                    }
+                for (int n = 0; n < NH; ++n) {
+                    sum[n][0] += add[n][0];
+                    sum[n][1] += add[n][1];
                 }
 
                 // outputs
 #pragma unroll
                 for (int u = 0; u < SUBS; ++u) {
-                    unsigned weight[NH][2];
+                    unsigned turned[NH][2];
 #pragma unroll
                     for (int c = 0; c < CPR; c += 2) {
                         unsigned w[4];
@@ -888,11 +955,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         for (int x = 0; x < 2; ++x) {
                             const int j = c + x;
                             if (BITS == 4 || j == 0) { // the weights of this group
-                                const float v0 = scaleAt(vs[u][0], BITS == 4 ? j : 0), v1 = scaleAt(vs[u][1], BITS == 4 ? j : 0);
 #pragma unroll
                                 for (int n = 0; n < NH; ++n) {
-                                    weight[n][0] = transposed(packHalves(s[u][n][0] * v0, s[u][n][1] * v0));
-                                    weight[n][1] = transposed(packHalves(s[u][n][2] * v1, s[u][n][3] * v1));
+                                    turned[n][0] = transposed(weight[u][BITS == 4 ? j : 0][n][0]);
+                                    turned[n][1] = transposed(weight[u][BITS == 4 ? j : 0][n][1]);
                                 }
                             }
                             if constexpr (BITS == 4) {
@@ -901,8 +967,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                                 codes4Odd16(magic, w[2 * x + 1], hi);
 #pragma unroll
                                 for (int n = 0; n < NH; ++n) {
-                                    mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], weight[n][0], weight[n][1]);
-                                    mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], weight[n][0], weight[n][1]);
+                                    mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], turned[n][0], turned[n][1]);
+                                    mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], turned[n][0], turned[n][1]);
                                 }
                             } else {
                                 const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
@@ -910,7 +976,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                                 const unsigned a2 = codes8<0x4240>(magic, hi), a3 = codes8<0x4341>(magic, hi);
 #pragma unroll
                                 for (int n = 0; n < NH; ++n) {
-                                    mma(o[n][j], a0, a1, a2, a3, weight[n][0], weight[n][1]);
+                                    mma(o[n][j], a0, a1, a2, a3, turned[n][0], turned[n][1]);
                                 }
                             }
                         }
@@ -921,17 +987,14 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 stage = stage == ring_addr + (S - 1) * C::kStage ? ring_addr : stage + C::kStage;
             } while (--left > 0);
 
-            if (special < 0) { // back to the maximum alone
-                const float up = exp2Fast(shift);
+            if (!even) { // the factors off
 #pragma unroll
                 for (int n = 0; n < NH; ++n) {
-                    sum[n][0] *= up;
-                    sum[n][1] *= up;
 #pragma unroll
-                    for (int j = 0; j < HD / 16; ++j) {
+                    for (int x = 0; x < 2; ++x) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            o[n][j][i] *= up;
+                        for (int j = 0; j < NG; ++j) {
+                            scaleGroup<BITS, HD>(o[n], j, x, -factors[j * HT + 8 * n + 2 * t + x]);
                         }
                     }
                 }
