@@ -18,6 +18,9 @@
  *   code  = x / scale to the nearest integer, halves away from zero, so |code| <= Q;
  *   a group that holds an infinity or a NaN gets the scale NaN and codes 0: it reads back as NaN.
  * A code stands for the value code * scale.  A pool of zero bytes stands for zeros.
+ *
+ * Pools may have no blocks, and null addresses then: no sequence has a token there, every slot is outside and
+ * treated as padding, reported as in checked mode (include/infiniop/ops/kernel_status.h) where it is not negative.
  */
 #ifndef __INFINIOP_QUANT_PAGED_CACHING_API_H__
 #define __INFINIOP_QUANT_PAGED_CACHING_API_H__

@@ -315,10 +315,12 @@ __INFINI_C infiniStatus_t infiniopQuantPagedAttention(
     if (I.num_seqs == 0 || I.num_heads == 0 || I.max_blocks == 0) {
         return INFINI_STATUS_SUCCESS; // no row, or no row with a token
     }
-    B200_RETURN_IF(out == nullptr || q == nullptr || k_cache == nullptr || v_cache == nullptr || k_scales == nullptr || v_scales == nullptr
-                       || block_tables == nullptr || seq_lens == nullptr,
-                   INFINI_STATUS_NULL_POINTER);
+    B200_RETURN_IF(out == nullptr || q == nullptr || block_tables == nullptr || seq_lens == nullptr, INFINI_STATUS_NULL_POINTER);
     B200_RETURN_IF(I.has_alibi && alibi_slopes == nullptr, INFINI_STATUS_NULL_POINTER);
+    if (I.pools.num_blocks == 0) {
+        return INFINI_STATUS_SUCCESS; // no sequence has a token, and there is no block that a bad table entry could stand for
+    }
+    B200_RETURN_IF(k_cache == nullptr || v_cache == nullptr || k_scales == nullptr || v_scales == nullptr, INFINI_STATUS_NULL_POINTER);
     B200_RETURN_IF(workspace_size < d->tiles.workspace_bytes, INFINI_STATUS_INSUFFICIENT_WORKSPACE);
     B200_RETURN_IF(d->tiles.workspace_bytes > 0 && workspace == nullptr, INFINI_STATUS_NULL_POINTER);
     qc::AttentionArgs a = qc::makeArgs(I);

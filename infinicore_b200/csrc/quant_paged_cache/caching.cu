@@ -516,7 +516,8 @@ static infiniStatus_t launch(const CachingDescriptor &d, void *k_cache, void *v_
     a.block_size = static_cast<int>(P.block_size);
     a.kernel_flags = d.base.props->kernel_flags;
     a.num_slots = static_cast<long long>(P.num_blocks) * static_cast<long long>(P.block_size);
-    a.check_indices = (d.check_indices && a.kernel_flags != nullptr) ? 1 : 0;
+    // a pool without blocks, which may have no address, is checked always
+    a.check_indices = ((d.check_indices || P.num_blocks == 0) && a.kernel_flags != nullptr) ? 1 : 0;
 
     const int widest = a.k.width > a.v.width ? a.k.width : a.v.width;
     a.lanes_log2 = 1; // a group of 32 elements is two lanes
@@ -555,8 +556,8 @@ static infiniStatus_t execute(InfiniopDescriptor *desc, OpKind kind, void *k_cac
     if (d->num_tokens == 0 || d->pools.num_kv_heads == 0) {
         return INFINI_STATUS_SUCCESS;
     }
-    B200_RETURN_IF(k_cache == nullptr || v_cache == nullptr || k_scales == nullptr || v_scales == nullptr || k == nullptr || v == nullptr
-                       || slots == nullptr,
+    B200_RETURN_IF(k == nullptr || v == nullptr || slots == nullptr, INFINI_STATUS_NULL_POINTER);
+    B200_RETURN_IF(d->pools.num_blocks > 0 && (k_cache == nullptr || v_cache == nullptr || k_scales == nullptr || v_scales == nullptr),
                    INFINI_STATUS_NULL_POINTER);
     return launch(*d, k_cache, v_cache, k_scales, v_scales, k, v, slots, static_cast<cudaStream_t>(stream));
 }
