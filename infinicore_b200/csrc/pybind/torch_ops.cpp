@@ -2,9 +2,10 @@
 //
 // What ops.py does in Python for the other operators is done here in C++: the checks of devices, the key of the
 // descriptor cache (the cache of include/infinicore_b200/ops.hpp: one for each thread and device, least recently used
-// evicted), the current stream, the call through the C ABI.  Scratch comes from torch's caching allocator for each call:
-// it is reused in the order of the stream, and a call that is captured into a CUDA graph gets memory of that graph, so
-// that graphs may be replayed at the same time.
+// evicted), the current stream, the call through the C ABI.  Scratch comes from torch's caching allocator for each call and
+// is reused in the order of the stream.  While a stream is being captured into a CUDA graph, by torch.cuda.graph or by any other
+// means, its calls share one scratch buffer that stays allocated for as long as the graph, or one instantiated from it, lives: graphs may
+// be replayed at the same time, and beside anything else that torch allocates.
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
@@ -13,7 +14,12 @@
 
 #include "infinicore_b200/ops.hpp"
 
+#include <cuda_runtime_api.h>
+
 #include <array>
+#include <atomic>
+#include <memory>
+#include <mutex>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -158,6 +164,88 @@ const ib::detail::Entry &lookup(const char *op, const std::array<const at::Tenso
     return *st.cache.put(key, e);
 }
 
+// Scratch buffers whose graphs are gone.  A graph's last reference is dropped by the CUDA driver, on a thread of its own and where no CUDA
+// call may be made: the buffer goes to this list, and back to the allocator at a later call.
+struct Released {
+    std::mutex mutex;
+    std::vector<at::Tensor> tensors;
+    std::atomic<bool> any{false};
+};
+Released &released() {
+    static Released *r = new Released; // never destroyed: graphs may outlive static objects
+    return *r;
+}
+void CUDART_CB releaseScratch(void *tensor) {
+    Released &r = released();
+    const std::lock_guard<std::mutex> lock(r.mutex);
+    r.tensors.push_back(*static_cast<at::Tensor *>(tensor));
+    delete static_cast<at::Tensor *>(tensor);
+    r.any = true;
+}
+
+// The buffer of the calls that are being captured on a stream.
+struct Captured {
+    unsigned long long id = 0; // of the capture; unique in the process
+    void *stream = nullptr;
+    at::Tensor tensor;
+};
+
+void checkCuda(cudaError_t e, const char *what) {
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+    }
+}
+
+at::Tensor scratch(const at::Tensor &like, size_t bytes, void *stream) {
+    thread_local std::vector<Captured> captures;
+    const auto fresh = [&] { return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)); };
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id, &graph) != cudaSuccess) {
+        (void)cudaGetLastError(); // the legacy stream while another one is captured: the launch will say so
+        return fresh();
+    }
+    if (status != cudaStreamCaptureStatusActive) {
+        captures.clear(); // their graphs hold them
+        Released &r = released();
+        if (r.any) {
+            std::vector<at::Tensor> gone;
+            {
+                const std::lock_guard<std::mutex> lock(r.mutex);
+                gone.swap(r.tensors);
+                r.any = false;
+            }
+        }
+        return fresh();
+    }
+    size_t kept = 0;
+    for (size_t i = 0; i < captures.size(); ++i) { // of earlier captures, what is left is their graphs' business
+        if (captures[i].id == id) {
+            std::swap(captures[kept++], captures[i]);
+        }
+    }
+    captures.resize(kept);
+    for (const Captured &c : captures) {
+        if (c.stream == stream && c.tensor.numel() >= static_cast<int64_t>(bytes)) {
+            return c.tensor;
+        }
+    }
+    auto held = std::make_unique<at::Tensor>(fresh());
+    const at::Tensor tensor = *held;
+    cudaUserObject_t owner = nullptr;
+    checkCuda(cudaUserObjectCreate(&owner, held.get(), releaseScratch, 1, cudaUserObjectNoDestructorSync), "cudaUserObjectCreate");
+    (void)held.release();
+    const cudaError_t e = cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+        (void)cudaUserObjectRelease(owner, 1);
+        checkCuda(e, "cudaGraphRetainUserObject");
+    }
+    captures.push_back({id, stream, tensor});
+    return tensor;
+}
+
 void quantPagedCaching(const at::Tensor &k_cache, const at::Tensor &v_cache, const at::Tensor &k_scales, const at::Tensor &v_scales,
                        const at::Tensor &k, const at::Tensor &v, const at::Tensor &slot_mapping) {
     const std::array<const at::Tensor *, 7> t = {&k_cache, &v_cache, &k_scales, &v_scales, &k, &v, &slot_mapping};
@@ -220,9 +308,9 @@ void quantPagedAttention(const at::Tensor &out, const at::Tensor &q, const at::T
         },
         infiniopGetQuantPagedAttentionWorkspaceSize, infiniopDestroyQuantPagedAttentionDescriptor,
         "infiniopCreateQuantPagedAttentionDescriptor");
-    at::Tensor workspace; // back to the allocator on return: reused behind this call on its stream
+    at::Tensor workspace; // back to the allocator on return, unless a graph holds it: reused behind this call on its stream
     if (e.workspace_bytes > 0) {
-        workspace = at::empty({static_cast<int64_t>(e.workspace_bytes)}, q.options().dtype(at::kByte));
+        workspace = scratch(q, e.workspace_bytes, call.stream);
     }
     ib::check(infiniopQuantPagedAttention(e.desc, e.workspace_bytes > 0 ? workspace.data_ptr() : nullptr, e.workspace_bytes, out.data_ptr(),
                                           q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),

@@ -437,7 +437,7 @@ def quant_paged_attention(q, k_cache, v_cache, k_scales, v_scales, block_tables,
     """paged_attention over pools that quant_paged_caching wrote: decode attention of one query token per sequence,
     q [num_seqs, num_heads, head_size] with head sizes 64, 128, 192 and 256; block_tables [num_seqs, max_blocks] and
     cache_lens [num_seqs] int64 or int32.  A sequence of length 0 leaves its rows of `out` as they are (zeros when
-    `out` is allocated here).  Captured into a CUDA graph, each call has scratch of its own.  Returns `out`."""
+    `out` is allocated here).  Calls captured into a CUDA graph have scratch that lives as long as the graph.  Returns `out`."""
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     _quant().quant_paged_attention(out, q, k_cache, v_cache, k_scales, v_scales, block_tables, cache_lens, alibi_slopes, scale)
