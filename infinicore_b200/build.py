@@ -117,7 +117,7 @@ def _link(objs, out: Path, extra, verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = False) -> dict:
     """Compiles what is stale and returns {"infinirt": path, "infiniop": path, "infiniccl": path, "pybind": path,
-    "torch_ops": path}."""
+    "torch_ops": path}, without the last where torch is not installed."""
     LIB.mkdir(exist_ok=True)
     OBJ.mkdir(exist_ok=True)
     if force:
@@ -137,8 +137,11 @@ def build(force: bool = False, verbose: bool = False) -> dict:
         _link(op_objs, libop, [f"-L{LIB}", "-linfinirt", "-Xlinker", "-rpath=$ORIGIN"], verbose)
     if force or not libccl.exists() or libccl.stat().st_mtime < newest_obj:
         _link(ccl_objs, libccl, [f"-L{LIB}", "-linfinirt", "-lnccl", "-Xlinker", "-rpath=$ORIGIN"], verbose)
-    return {"infinirt": librt, "infiniop": libop, "infiniccl": libccl, "pybind": build_pybind(force, verbose),
-            "torch_ops": build_torch_ops(force, verbose)}
+    out = {"infinirt": librt, "infiniop": libop, "infiniccl": libccl, "pybind": build_pybind(force, verbose)}
+    torch_ops = build_torch_ops(force, verbose)
+    if torch_ops is not None:
+        out["torch_ops"] = torch_ops
+    return out
 
 
 def build_pybind(force: bool = False, verbose: bool = False) -> Path:
@@ -172,13 +175,19 @@ def build_pybind(force: bool = False, verbose: bool = False) -> Path:
     return out
 
 
-def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
+def build_torch_ops(force: bool = False, verbose: bool = False) -> Path | None:
     """Compiles the operators on torch tensors (csrc/pybind/torch_ops.cpp) with g++ against torch's own headers, in-tree, linked
-    to the libraries in lib/ (found again at run time through $ORIGIN/lib) and to torch's (loaded by `import torch`)."""
+    to the libraries in lib/ (found again at run time through $ORIGIN/lib) and to torch's (loaded by `import torch`).  None
+    where there is no torch with CUDA: callers of the C ABI and of the C++ layer need none."""
     import sysconfig
 
-    import torch
-
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    if torch is None or torch.version.cuda is None:
+        print("no torch with CUDA: the quant_paged_* operators on its tensors (_torch_ops) are not built", file=sys.stderr)
+        return None
     base = Path(torch.__file__).resolve().parent
     src = CSRC / "pybind" / "torch_ops.cpp"
     out = PKG / ("_torch_ops" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
