@@ -87,7 +87,7 @@ struct Cfg {
     static constexpr int kHeadTiles = HT / 8;
     static constexpr int kStride = HD + 4;                    // floats: rows of two heads apart hit other banks
     static constexpr int kResult = HT * kStride * 4;
-    static constexpr int kFactors = 2 * HT * (kGroups + 1) * 4; // of a warp: as they are, and as they are being settled
+    static constexpr int kFactors = HT * (kGroups + 1) * 4; // bytes of a warp
     static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + kFactors + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes);
     // resident CTAs: what the registers of q, outputs and scales leave room for
     static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 || HT == 16 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
     extern __shared__ __align__(128) unsigned char smem[];
     float *results = reinterpret_cast<float *>(smem + kWarps * C::kRing);                                     // [warp][head][kStride]
     float2 *sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(results) + kWarps * C::kResult); // [warp][2][head]
-    float *all_factors = reinterpret_cast<float *>(sums + kWarps * 2 * HT);                                   // [warp][old | new][group | least][head]
+    float *all_factors = reinterpret_cast<float *>(sums + kWarps * 2 * HT);                                   // [warp][group | least][head]
     Piece *pieces = reinterpret_cast<Piece *>(all_factors + kWarps * (C::kFactors / 4));                                // [warp][2]
     Walk *walks = reinterpret_cast<Walk *>(pieces + kWarps * 2);                                              // [warp][copies | arithmetic]
     const int tid = static_cast<int>(pinned(threadIdx.x)), warp = tid >> 5, lane = tid & 31;
@@ -826,18 +826,18 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         }
                         // p of before are smaller by 2^up now, and factors as much larger, up to their limit.  A group whose largest weight of this tile
                         // would be 2^8 or more gets a factor that makes it 2^7.
-                        float up[NH][2];
-                        float *const next = mine + (NG + 1) * HT;
+                        float common[NH][2], up[NH][2], is[NH][2][NG], least[NH][2];
                         bool near = !far;
 #pragma unroll
                         for (int n = 0; n < NH; ++n) {
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
-                                top[n][x] += even ? mine[NG * HT + 8 * n + x] : 0.f;
+                                common[n][x] = even ? mine[NG * HT + 8 * n + x] : 0.f;
+                                top[n][x] += common[n][x];
                                 now[n][x] = fmaxf(now[n][x], top[n][x]);
                                 up[n][x] = now[n][x] - top[n][x];
-                                top[n][x] = now[n][x];
-                                float most = -INFINITY, least = INFINITY;
+                                float most = -INFINITY;
+                                least[n][x] = INFINITY;
 #pragma unroll
                                 for (int j = 0; j < NG; ++j) {
                                     float m = 0.f;
@@ -848,13 +848,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                                     }
                                     const float high = exponentOf(largestOf(m));
                                     const float was = fresh ? kMostFactor : fminf(mine[j * HT + 8 * n + x] + up[n][x], kMostFactor);
-                                    const float is = high + was > kLargest ? kLargest - high : was;
-                                    next[j * HT + 8 * n + x] = is;
-                                    least = fminf(least, is);
-                                    most = fmaxf(most, is);
+                                    is[n][x][j] = high + was > kLargest ? kLargest - high : was;
+                                    least[n][x] = fminf(least[n][x], is[n][x][j]);
+                                    most = fmaxf(most, is[n][x][j]);
                                 }
-                                next[NG * HT + 8 * n + x] = least;
-                                near = near && most - least <= kEven && least >= kLeastCommon && least <= kMostCommon;
+                                near = near && most - least[n][x] <= kEven && least[n][x] >= kLeastCommon && least[n][x] <= kMostCommon;
                             }
                         }
                         const bool was_even = even;
@@ -864,13 +862,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                             for (int n = 0; n < NH; ++n) {
 #pragma unroll
                                 for (int x = 0; x < 2; ++x) {
-                                    const float common = mine[NG * HT + 8 * n + x], least = next[NG * HT + 8 * n + x];
 #pragma unroll
                                     for (int j = 0; j < NG; ++j) {
-                                        const float was = was_even ? common : mine[j * HT + 8 * n + x];
-                                        scaleGroup<BITS, HD>(o[n], j, x, ((even ? least : next[j * HT + 8 * n + x]) - was) - up[n][x]);
+                                        const float was = was_even ? common[n][x] : mine[j * HT + 8 * n + x];
+                                        scaleGroup<BITS, HD>(o[n], j, x, ((even ? least[n][x] : is[n][x][j]) - was) - up[n][x]);
                                     }
-                                    sum[n][x] = shifted(shifted(shifted(sum[n][x], was_even ? -common : 0.f), -up[n][x]), even ? least : 0.f);
+                                    sum[n][x] = shifted(shifted(shifted(sum[n][x], -common[n][x]), -up[n][x]), even ? least[n][x] : 0.f);
                                 }
                             }
                         }
@@ -879,11 +876,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         for (int n = 0; n < NH; ++n) {
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
+                                top[n][x] = now[n][x] - (even ? least[n][x] : 0.f);
 #pragma unroll
-                                for (int j = 0; j <= NG; ++j) {
-                                    mine[j * HT + 8 * n + x] = next[j * HT + 8 * n + x];
+                                for (int j = 0; j < NG; ++j) {
+                                    mine[j * HT + 8 * n + x] = is[n][x][j];
                                 }
-                                top[n][x] -= even ? next[NG * HT + 8 * n + x] : 0.f;
+                                mine[NG * HT + 8 * n + x] = least[n][x];
                             }
                         }
                         __syncwarp();
