@@ -138,3 +138,20 @@ def test_the_smallest_and_largest_values_that_a_pool_holds(ib):  # noqa: F811
         scaled[3] = (pools[3].float() * torch.exp2(torch.tensor(e).float()).cuda()).to(BF16)
         check(ib, q, scaled, tables, lens, hd ** -0.5, 4, BF16, f"{e}")
         assert math.isfinite(float(scaled[3].float().max()))
+
+
+@pytest.mark.parametrize("hd,heads,kvh", [(64, 8, 2), (128, 8, 2), (128, 16, 1), (192, 4, 1), (256, 8, 2)])
+@pytest.mark.parametrize("later", [None, 0, -30, 30])
+def test_groups_that_are_zero_for_a_while(ib, hd, heads, kvh, later):  # noqa: F811
+    """Groups of zeros, as padded heads have, for all tokens or up to some token, where values of 2^later times the others' size begin."""
+    lens = [700, 64, 1]
+    for first in (1, 17, 500):
+        g, pools, tables, q = case(hd + first, 4, hd, heads, kvh, lens, BF16, 1.0)
+        factor = torch.zeros(pools[3].shape)
+        if later is not None:
+            for i, n in enumerate(lens):
+                for t in range(min(first * (i + 1), n), n):
+                    factor[int(tables[i, t // 16]), :, t % 16] = 2.0 ** later
+        factor[..., 0] = 1.0
+        pools[3].copy_((pools[3].float() * factor.cuda()).to(BF16))
+        check(ib, q, pools, tables, lens, 1.5 * hd ** -0.5, 4, BF16, f"from token {first}")
