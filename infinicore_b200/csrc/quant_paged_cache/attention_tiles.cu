@@ -22,7 +22,7 @@
 // every second element of V keeps a factor of 16 that its output is rid of at the end.
 //   q is held in fp16 times a power of two that makes its largest element 1/2..1: exact for every element above
 // 2^-13 of that (fp16 and bf16 both have at most 11 bits).
-//   w is rounded once to fp16, as w = p * v_scale * 2^k with an exponent k of its own for each head and group of V, so that every group of
+//   w is rounded to fp16 (once, or as two halves: see Split), as w = p * v_scale * 2^k with an exponent k of its own for each head and group of V, so that every group of
 // an output has weights of full precision, whatever the sizes of the others.  k is settled at a unit's first tile: it makes the group's
 // largest weight 2^7..2^8.  It is settled again, from the same tile's scores once more, when a weight passes what fp16 holds; earlier
 // outputs are scaled then, by powers of two.  Where the k of a head's groups are within 2^6 of each other, as they are unless V's channels differ
@@ -58,6 +58,14 @@ constexpr float kLargest = 7.f;      // exponent of a group's largest weight whe
 constexpr float kEven = 6.f;         // factors of a head's groups whose exponents are this near count as one: the largest weight of each group
                                      // is 2 or more then, and what is subnormal in fp16 is off by 2^-26 of it at most
 constexpr float kLeastCommon = -20.f, kMostCommon = 80.f; // exponents that such a one may have: p times it stays far inside fp32
+
+// One rounding of the weights to fp16 is not seen in bf16 outputs, which are rounded to 8 bits (error against 64 bits 1.66e-3 instead of
+// 1.65e-3), but is in fp16 ones (2.9e-4 instead of 2.1e-4, and its whole 2^-11 where a sequence has one token).  There weights are split
+// in two: p' * v_scale with the three leading bits of p, which is exact, and the rest.  kColumns: with groups of up to 4 q heads the rests
+// take the other half of an instruction's 8 columns, whose q are the same heads again.  kTwice: a second product.  Measured at 64 x 4096
+// tokens, 32/8 heads of 128 (us, whole | columns | twice): 4 bits 77.9 | 79.5 | 93.4, 8 bits 97.8 | 98.6 | 106.7; 64/4 heads of 128 (whole | twice):
+// 69.7 | 84.7, 72.0 | 82.0.
+enum Split : int { kWhole = 0, kColumns = 1, kTwice = 2 };
 
 // What the combine kernel has to do for a unit: nothing, or to add this many pieces from this CTA's on.
 struct Task {
@@ -218,6 +226,8 @@ __device__ __forceinline__ float shifted(float x, float e) {
     const float a = fmaxf(e, -126.f), b = fmaxf(e - a, -126.f);
     return x * powerOfTwo(a) * powerOfTwo(b);
 }
+// The three leading bits of p
+__device__ __forceinline__ float leading(float p) { return __uint_as_float(__float_as_uint(p) & 0xffe00000u); }
 // The exponent of x >= 0; -127 of 0 and of subnormal numbers
 __device__ __forceinline__ float exponentOf(float x) { return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127); }
 // The largest among the eight lanes of a head
@@ -328,7 +338,8 @@ __device__ __forceinline__ void storeOut(const AttentionArgs &a, const TilesArgs
 
 // DENSE: blocks are multiples of 16 tokens and the rows of a head follow one another in a block, so 16 tokens are one run of
 // memory; otherwise blocks are multiples of 8 tokens, rows lie anywhere, and 8 tokens' scales are one run.
-template <int BITS, int HD, int HT, bool DENSE>
+// SPLIT: of the weights.
+template <int BITS, int HD, int HT, bool DENSE, Split SPLIT>
 __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAttentionTilesKernel(const AttentionArgs a, const TilesArgs p) {
     using C = Cfg<BITS, HD, HT>;
     constexpr int NG = C::kGroups, NH = C::kHeadTiles, CPR = C::kChunks, S = C::kStages, TILE = C::kTile, SUBS = C::kSubs;
@@ -541,14 +552,15 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
         uint4 q_raw[NH][HD / 32];
         auto loadQ = [&]() {
             const int kv = work.sub / p.head_tiles, head0 = (work.sub - kv * p.head_tiles) * HT;
+            const int row = SPLIT == kColumns ? g & 3 : g; // columns 4 to 7 are heads 0 to 3 again
             const unsigned short *q = static_cast<const unsigned short *>(a.q) + work.seq * a.q_seq
-                                    + (static_cast<long long>(kv) * a.group + head0 + g) * a.q_head;
+                                    + (static_cast<long long>(kv) * a.group + head0 + row) * a.q_head;
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
                     q_raw[n][j] = make_uint4(0, 0, 0, 0);
-                    if (head0 + g + 8 * n < a.group) {
+                    if (head0 + row + 8 * n < a.group) {
                         const unsigned short *from = q + 8 * n * a.q_head + 32 * j;
                         if constexpr (BITS == 4) {
                             q_raw[n][j] = *reinterpret_cast<const uint4 *>(from + 8 * t);
@@ -587,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
             float factor[NH][2], slope[NH][2];       // of the scores' columns, heads 2t and 2t + 1
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
-                const int h = g + 8 * n;
+                const int h = (SPLIT == kColumns ? g & 3 : g) + 8 * n;
                 unsigned largest = 0;
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
@@ -686,12 +698,13 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                     return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
                 };
 
+                float s[SUBS][NH][4]; // [.][.][token g, heads 2t and 2t + 1 | token g + 8]: scores, p
+                unsigned vs[SUBS][2][kWords];
                 unsigned weight[SUBS][NG][NH][2];
                 float add[NH][2];
 #pragma unroll 1
                 for (bool settle = fresh || special < 0;; settle = true) {
                     // scores
-                    float s[SUBS][NH][4]; // [.][.][token g, heads 2t and 2t + 1 | token g + 8]
 #pragma unroll
                     for (int u = 0; u < SUBS; ++u) {
                         unsigned ks[2][kWords];
@@ -748,7 +761,6 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                             }
                         }
                     }
-                    unsigned vs[SUBS][2][kWords];
 #pragma unroll
                     for (int u = 0; u < SUBS; ++u) {
                         loadScales(vs[u][0], scales + 2 * TILE * NG + u * (32 * NG));
@@ -887,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                         __syncwarp();
                         fresh = false;
                     }
-                    // p, and the weights p * v_scale * factor in fp16: the one rounding to fewer bits
+                    // p, and the weights p * v_scale * factor in fp16
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
                         add[n][0] = add[n][1] = 0.f;
@@ -902,10 +914,17 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                             }
                             add[n][0] += s[u][n][0] + s[u][n][2];
                             add[n][1] += s[u][n][1] + s[u][n][3];
+                            if constexpr (SPLIT == kColumns) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float p = leading(s[u][n][i]);
+                                    s[u][n][i] = t < 2 ? p : s[u][n][i] - p;
+                                }
+                            }
                         }
                     }
                     unsigned largest = 0;
-                    auto weigh = [&](auto factor) {
+                    auto weigh = [&](auto part, auto factor) {
 #pragma unroll
                         for (int j = 0; j < NG; ++j) {
 #pragma unroll
@@ -914,17 +933,17 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 #pragma unroll
                                 for (int u = 0; u < SUBS; ++u) {
                                     const float v0 = scaleAt(vs[u][0], j), v1 = scaleAt(vs[u][1], j);
-                                    weight[u][j][n][0] = packHalves(s[u][n][0] * by0 * v0, s[u][n][1] * by1 * v0);
-                                    weight[u][j][n][1] = packHalves(s[u][n][2] * by0 * v1, s[u][n][3] * by1 * v1);
+                                    weight[u][j][n][0] = packHalves(part(s[u][n][0]) * by0 * v0, part(s[u][n][1]) * by1 * v0);
+                                    weight[u][j][n][1] = packHalves(part(s[u][n][2]) * by0 * v1, part(s[u][n][3]) * by1 * v1);
                                     largest = __vmaxu2(largest, __vmaxu2(weight[u][j][n][0], weight[u][j][n][1]));
                                 }
                             }
                         }
                     };
                     if (even) {
-                        weigh([](int, int, int) { return 1.f; });
+                        weigh([](float p) { return SPLIT == kTwice ? leading(p) : p; }, [](int, int, int) { return 1.f; });
                     } else {
-                        weigh([&](int j, int n, int x) { return powerOfTwo(factors[j * HT + 8 * n + 2 * t + x]); });
+                        weigh([](float p) { return p; }, [&](int j, int n, int x) { return powerOfTwo(factors[j * HT + 8 * n + 2 * t + x]); });
                     }
                     bool again = max(largest & 0xffffu, largest >> 16) >= 0x7c00u; // an infinity, or no number
 #pragma unroll
@@ -942,8 +961,21 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 }
 
                 // outputs
+                if constexpr (SPLIT == kTwice) { // what the weights are short of; not even, they were rounded whole
+#pragma unroll
+                    for (int u = 0; u < SUBS; ++u) {
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                s[u][n][i] = even ? s[u][n][i] - leading(s[u][n][i]) : 0.f;
+                            }
+                        }
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < SUBS; ++u) {
+                    [[maybe_unused]] unsigned rest[NH][2];
                     unsigned turned[NH][2];
 #pragma unroll
                     for (int c = 0; c < CPR; c += 2) {
@@ -957,6 +989,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                                 for (int n = 0; n < NH; ++n) {
                                     turned[n][0] = transposed(weight[u][BITS == 4 ? j : 0][n][0]);
                                     turned[n][1] = transposed(weight[u][BITS == 4 ? j : 0][n][1]);
+                                    if constexpr (SPLIT == kTwice) {
+                                        const float v0 = scaleAt(vs[u][0], BITS == 4 ? j : 0), v1 = scaleAt(vs[u][1], BITS == 4 ? j : 0);
+                                        rest[n][0] = transposed(packHalves(s[u][n][0] * v0, s[u][n][1] * v0));
+                                        rest[n][1] = transposed(packHalves(s[u][n][2] * v1, s[u][n][3] * v1));
+                                    }
                                 }
                             }
                             if constexpr (BITS == 4) {
@@ -967,6 +1004,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                                 for (int n = 0; n < NH; ++n) {
                                     mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], turned[n][0], turned[n][1]);
                                     mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], turned[n][0], turned[n][1]);
+                                    if constexpr (SPLIT == kTwice) {
+                                        mma(o[n][2 * j], lo[0], lo[1], hi[0], hi[1], rest[n][0], rest[n][1]);
+                                        mma(o[n][2 * j + 1], lo[2], lo[3], hi[2], hi[3], rest[n][0], rest[n][1]);
+                                    }
                                 }
                             } else {
                                 const unsigned lo = w[2 * x] ^ 0x80808080u, hi = w[2 * x + 1] ^ 0x80808080u;
@@ -975,6 +1016,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
 #pragma unroll
                                 for (int n = 0; n < NH; ++n) {
                                     mma(o[n][j], a0, a1, a2, a3, turned[n][0], turned[n][1]);
+                                    if constexpr (SPLIT == kTwice) {
+                                        mma(o[n][j], a0, a1, a2, a3, rest[n][0], rest[n][1]);
+                                    }
                                 }
                             }
                         }
@@ -985,6 +1029,18 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BITS, HD, HT>::kCtas)) quantAtt
                 stage = stage == ring_addr + (S - 1) * C::kStage ? ring_addr : stage + C::kStage;
             } while (--left > 0);
 
+            if constexpr (SPLIT == kColumns) { // the halves together: columns 4 to 7 belong to the lanes with t + 2
+#pragma unroll
+                for (int n = 0; n < NH; ++n) {
+#pragma unroll
+                    for (int j = 0; j < HD / 16; ++j) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[n][j][i] += __shfl_xor_sync(0xffffffffu, o[n][j][i], 2);
+                        }
+                    }
+                }
+            }
             if (!even) { // the factors off
 #pragma unroll
                 for (int n = 0; n < NH; ++n) {
@@ -1226,32 +1282,43 @@ struct Variant {
     int ctas, smem, record, heads, tile;
 };
 
-template <int BITS, int HD, int HT>
+template <int BITS, int HD, int HT, Split SPLIT>
 Variant variant() {
     using C = Cfg<BITS, HD, HT>;
-    return {{quantAttentionTilesKernel<BITS, HD, HT, false>, quantAttentionTilesKernel<BITS, HD, HT, true>}, quantAttentionCombineKernel<HD, HT>, C::kCtas, C::kSmem, C::kRecord, HT, C::kTile};
+    return {{quantAttentionTilesKernel<BITS, HD, HT, false, SPLIT>, quantAttentionTilesKernel<BITS, HD, HT, true, SPLIT>}, quantAttentionCombineKernel<HD, HT>, C::kCtas, C::kSmem, C::kRecord, HT, C::kTile};
+}
+
+template <int BITS, int HD, int HT>
+Variant variantFor(bool fp16, size_t group) {
+    if constexpr (HT == 8) {
+        if (fp16 && group <= 4) {
+            return variant<BITS, HD, HT, kColumns>();
+        }
+    }
+    return fp16 ? variant<BITS, HD, HT, kTwice>() : variant<BITS, HD, HT, kWhole>();
 }
 
 template <int BITS>
-Variant variantFor(size_t head, size_t group) {
+Variant variantFor(size_t head, bool fp16, size_t group) {
     // 16 heads share a pass over the codes where a group has more than 8; at heads of 192 and 256 their outputs would not
     // fit the registers.  Measured at 64/4 heads, 64 x 4096 tokens (us, one pass | two of 8 heads): heads of 128 63 | 80 at
     // 4 bits, 68 | 95 at 8; heads of 64 42 | 50, 43 | 56.
     switch (head) {
     case 64:
-        return group > 8 ? variant<BITS, 64, 16>() : variant<BITS, 64, 8>();
+        return group > 8 ? variantFor<BITS, 64, 16>(fp16, group) : variantFor<BITS, 64, 8>(fp16, group);
     case 128:
-        return group > 8 ? variant<BITS, 128, 16>() : variant<BITS, 128, 8>();
+        return group > 8 ? variantFor<BITS, 128, 16>(fp16, group) : variantFor<BITS, 128, 8>(fp16, group);
     case 192:
-        return variant<BITS, 192, 8>();
+        return variantFor<BITS, 192, 8>(fp16, group);
     default:
-        return variant<BITS, 256, 8>();
+        return variantFor<BITS, 256, 8>(fp16, group);
     }
 }
 
 Variant variantFor(const AttentionInfo &I) {
     const size_t group = I.num_heads / I.pools.num_kv_heads;
-    return I.pools.bits == 4 ? variantFor<4>(I.head_size, group) : variantFor<8>(I.head_size, group);
+    const bool fp16 = I.dtype == INFINI_DTYPE_F16;
+    return I.pools.bits == 4 ? variantFor<4>(I.head_size, fp16, group) : variantFor<8>(I.head_size, fp16, group);
 }
 
 } // namespace

@@ -13,11 +13,11 @@ pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
 
 
-def group_bound(q, pools, tables, lens, scale, bits, dtype):
+def group_bound(q, pools, tables, lens, scale, bits, dtype, weight=2.0 ** -11):
     """The output in 64 bits and how far a kernel's may be from it, by the sizes of an element's own group.
 
     An output sum_j p_j v_j / sum_j p_j is off by at most
-      sum_j p_j |v_j| (2^-11 + x_j)      one rounding of the weight p_j * scale_jg to fp16, and x_j of the rest
+      sum_j p_j |v_j| (2^-11 + x_j)      one rounding of the weight p_j * scale_jg to fp16 (`weight`), and x_j of the rest
       |out| sum_j p_j x_j                the denominator adds p in fp32
       n 2^-25 max_j p_j s_jg             weights that are subnormal in fp16 are off by 2^-25; the largest of a group (p_j times its scale) has come
                                          to 2^7 times its own factor, and the factor in use is at most 2^6 below that: 2^-26 of it, a token's
@@ -50,7 +50,7 @@ def group_bound(q, pools, tables, lens, scale, bits, dtype):
         x = torch.expm1(2 * d) + 2.0 ** -19 + (n / 4 + 64) * 2.0 ** -23
         o = torch.einsum("hgn,nhd->hgd", p, v)
         few = n * 2.0 ** -25 * torch.einsum("hgn,nhc->hgnc", p, s_v).amax(2).repeat_interleave(size, -1)
-        b = torch.einsum("hgn,nhd->hgd", p * (2.0 ** -11 + x), v.abs()) + o.abs() * (p * x).sum(-1, keepdim=True) + few
+        b = torch.einsum("hgn,nhd->hgd", p * (weight + x), v.abs()) + o.abs() * (p * x).sum(-1, keepdim=True) + few
         want[i] = o.reshape(heads, hd)
         bound[i] = ((b + n * 2.0 ** -131) * (1 + half)).reshape(heads, hd) + half * want[i].abs() + torch.finfo(dtype).smallest_normal * half
     return want, bound
@@ -155,3 +155,25 @@ def test_groups_that_are_zero_for_a_while(ib, hd, heads, kvh, later):  # noqa: F
         factor[..., 0] = 1.0
         pools[3].copy_((pools[3].float() * factor.cuda()).to(BF16))
         check(ib, q, pools, tables, lens, 1.5 * hd ** -0.5, 4, BF16, f"from token {first}")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 64), (8, 2, 128), (3, 3, 128), (6, 2, 192), (8, 2, 256), (7, 1, 128), (16, 2, 64), (16, 1, 128), (12, 1, 64), (8, 1, 256)])
+def test_fp16_outputs_are_as_exact_as_32_bit_arithmetic(ib, bits, heads, kvh, hd):  # noqa: F811
+    """Weights for fp16 outputs are exact to 2^-13: p' * scale with the three leading bits of p (3 + 8 bits: exact), and the rest, less than
+    a quarter of it, rounded once.  Element by element where a sequence has few tokens, so that the rounding of a weight shows in full;
+    over many tokens by the norm of the error: the roundings of n weights add up like independent ones, 2^-13 of sqrt(sum p_j^2 v_j^2)
+    at most, which for values of either sign is the size of the outputs, whose own rounding has a norm of at least 2^-12 / sqrt(3) of that
+    over 2^-11 / sqrt(3): between 1.4e-4 and 2.8e-4, 2.0e-4 for outputs of all sizes, against 2^-13 = 1.2e-4 at most: 1.17 together."""
+    lens = [1, 2, 3, 4, 1, 1, 17, 2]
+    for seed in range(3):
+        g, pools, tables, q = case(seed, bits, hd, heads, kvh, lens, FP16, 1.0)
+        want, bound = group_bound(q, pools, tables, torch.tensor(lens), hd ** -0.5, bits, FP16, 2.0 ** -13)
+        got = ib.quant_paged_attention(q, *pools, tables, torch.tensor(lens).cuda(), None, hd ** -0.5)
+        qh.close(got, want, bound, f"seed {seed}")
+    lens = [3000, 700, 1500]
+    g, pools, tables, q = case(9, bits, hd, heads, kvh, lens, FP16, 1.0)
+    want, _ = group_bound(q, pools, tables, torch.tensor(lens), hd ** -0.5, bits, FP16)
+    got = ib.quant_paged_attention(q, *pools, tables, torch.tensor(lens).cuda(), None, hd ** -0.5)
+    err, rounding = ((x.double() - want).norm() / want.norm() for x in (got, want.to(FP16)))
+    assert float(err) <= 1.2 * float(rounding), (float(err), float(rounding))
