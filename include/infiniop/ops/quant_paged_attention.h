@@ -13,11 +13,17 @@
  *   alibi_slopes  [num_heads] F32, optional (descriptor and pointer may be NULL)
  *
  * With k and v the values that the codes stand for and n = seq_lens[i] (at most block_size times the
- * table's width):
+ * table's width, also where a U32 length is 2^31 or more):
  *   out[i, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[i, h] . k_j + slope_h (j - (n - 1))),  0 <= j < n,
  * where token j of sequence i is at cache[block_tables[i][j / block_size], h / (num_heads /
  * num_kv_heads), j % block_size].  A sequence with n <= 0 leaves its output rows untouched; what the
- * pools hold behind a sequence's last token does not matter, NaN scales included.
+ * pools hold behind a sequence's last token does not matter, NaN scales included.  With pools of no blocks no
+ * sequence has a token, and their addresses may be NULL.
+ *
+ * Scores, sums and outputs are held in 32 bits.  The weights p_j times the V scale of a group (of 32 elements, or of the
+ * row) are rounded to fp16 relative to the largest of their head and group, once for BF16 outputs, in two halves
+ * (2^-13) for F16 ones, so that groups of any size keep their precision; those with scales below 2^-100 keep less, and F16
+ * outputs of more than 4 q heads a kv head whose groups differ in size by more than 2^6 have the one rounding.
  *
  * The workspace is caller-owned scratch of at least GetWorkspaceSize bytes, 256-byte aligned, contents
  * undefined on entry; calls that may overlap on the GPU need one each.  Execute is asynchronous on

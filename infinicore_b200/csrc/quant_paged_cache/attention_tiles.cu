@@ -29,9 +29,10 @@
 // in size by far more than that, the smallest serves them all, inside the maximum: w = p * v_scale ("even").
 //   Sums, maxima and outputs are fp32.
 //
-// Measured at 32/8 heads of 128, 64 x 4096 tokens, the combine kernel's share of 3 to 5 us included: 8 bits 96 us (5.7 TB/s of
-// codes and scales, bound by HBM), 4 bits 78 us (3.9 TB/s; issue slots 62 %, ALU 50 %, no single pipe full: bound by turning codes
-// into operands).
+// Measured at 32/8 heads of 128, 64 x 4096 tokens, bf16, the combine kernel's share of 3.5 to 4.6 us included: 8 bits 98 us in a graph of
+// ten calls (5.6 TB/s of codes and scales), 100 to 112 over thousands in a row; 4 bits 78 us (3.9 TB/s).  At 4 bits nothing is full (issue slots 63 %,
+// ALU 49 %, HBM 46 %): warps wait for their own last instruction, 2.8 to a scheduler.  About 15 us are there at any length: 64 sequences
+// of 256, 1024, 4096 tokens on the line take 18.7, 31.1, 78.0 us at 4 bits, 21.3, 36.6, 97.6 at 8.
 #include "attention.h"
 
 #include <cuda_bf16.h>
@@ -44,10 +45,10 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 // What a unit costs beside its tiles, in tiles: the time of 64 tokens.  Measured at 40 ragged sequences (64/8 heads of 128, 4 bits): 0
-// tokens 64 us, 32 43.5, 64 41.0, 128 40.7; at 62 sequences of 200 to 2000 32.1, 31.2, 30.2, 31.0.
+// tokens 67.5 us, 32 44.5, 64 40.7, 128 40.4; at 62 sequences of 200 to 2000 with their append 31.9, 31.4, 29.5, 30.5.
 constexpr int unitCost(int tile) { return 64 / tile; }
 // Of a warp: at least two tiles of a unit's first range.  More leaves fewer pieces to combine but warps idle: 6, 12, 24 instead of 2 take
-// 13 sequences of 1 to 30001 (16/1 heads of 256, 8 bits) from 25.6 us to 28.5, 29.9, 39.8, the 62 sequences from 28.7 to 28.7, 38.2, 45.0.
+// 13 sequences of 1 to 30001 (16/1 heads of 256, 8 bits) from 26.3 us to 28.8, 31.0, 40.7, the 62 sequences from 29.5 to 29.5, 38.6, 46.4.
 constexpr int minRange(int tile) { return unitCost(tile) + 2; }
 // What the weights are relative to is settled at a unit's first tile and again when a weight does not fit fp16 (or p comes to kMostP).
 // p = exp2(score - top), in the log2 domain: top is then kBelow above the largest score so far.
@@ -86,9 +87,9 @@ struct Cfg {
     static constexpr int kChunks = kRowBytes / 16;            // 16-byte chunks of a row
     static constexpr int kGroups = BITS == 4 ? HD / 32 : 1;   // scales of a row
     // A tile is one, two or four times 16 tokens, about 4 KB of codes: what surrounds the matrix instructions costs as many issue slots
-    // as 8 tokens' arithmetic.  Measured at 64 x 4096 tokens, 32/8 heads (us): 4 bits, heads of 128, 16 tokens 85, 32 81; heads of 64,
-    // 32 tokens 53, 64 50; 8 bits, heads of 64, 16 tokens 63, 32 57.  With 16 heads the scores of 64 tokens do not fit the registers
-    // (64/4 heads of 64 at 4 bits: 32 tokens 41.7, 64 43.7).
+    // as 8 tokens' arithmetic.  Measured at 64 x 4096 tokens, 32/8 heads (us): 4 bits, heads of 128, 16 tokens 88.5, 32 77.8; heads of 64,
+    // 32 tokens 54.2, 64 50.4; 8 bits, heads of 64, 16 tokens 66.0, 32 57.3.  With 16 heads the weights of 64 tokens do not fit the registers
+    // (64/4 heads of 64 at 4 bits: 32 tokens 44.8, 64 50.1).
     static constexpr int kSubs = HD * BITS <= 256 && HT == 8 ? 4 : HD * BITS <= 512 ? 2 : 1;
     static constexpr int kTile = 16 * kSubs;
     static constexpr int kStage = 2 * kTile * kRowBytes + 2 * kTile * kGroups * 2;
@@ -97,7 +98,8 @@ struct Cfg {
     static constexpr int kResult = HT * kStride * 4;
     static constexpr int kFactors = HT * (kGroups + 1) * 4; // bytes of a warp
     static constexpr int kFixed = kWarps * (kResult + 2 * HT * 8 + kFactors + 2 * static_cast<int>(sizeof(Piece)) + 2 * kWalkBytes);
-    // resident CTAs: what the registers of q, outputs and scales leave room for
+    // resident CTAs: what the registers of q, outputs and scales leave room for; 8 bits at heads of 128, heads of 192, 16 q heads and two products
+    // spill 4 to 170 bytes
     static constexpr int kCtas = HD * HT <= 1024 ? (BITS == 4 || HT == 16 ? 3 : 4) : HD * HT <= 1536 ? 3 : 2;
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - kFixed) / (kWarps * kStage);
     static constexpr int kStages = kFit > 4 ? 4 : kFit;
@@ -115,7 +117,8 @@ __device__ __forceinline__ unsigned smemAddr(const void *p) { return static_cast
 __device__ __forceinline__ void copy16(unsigned dst, const void *src, unsigned long long policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
-// Codes and scales are read once: they leave the L2 first, tables, q and partial results stay.
+// Codes and scales are read once: they leave the L2 first, tables, q and partial results stay.  Measured with | without (us): 64 x 4096
+// tokens at 8 bits 97.7 | 100.5, 62 sequences of 200 to 2000 at 4 bits with their append 29.5 | 31.0.
 __device__ __forceinline__ unsigned long long readOnce() {
     unsigned long long p;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
@@ -1301,8 +1304,8 @@ Variant variantFor(bool fp16, size_t group) {
 template <int BITS>
 Variant variantFor(size_t head, bool fp16, size_t group) {
     // 16 heads share a pass over the codes where a group has more than 8; at heads of 192 and 256 their outputs would not
-    // fit the registers.  Measured at 64/4 heads, 64 x 4096 tokens (us, one pass | two of 8 heads): heads of 128 63 | 80 at
-    // 4 bits, 68 | 95 at 8; heads of 64 42 | 50, 43 | 56.
+    // fit the registers.  Measured at 64/4 heads, 64 x 4096 tokens, bf16 (us, one pass | two of 8 heads): heads of 128 70 | 80 at
+    // 4 bits, 72 | 100 at 8; heads of 64 45 | 50, 45 | 58.
     switch (head) {
     case 64:
         return group > 8 ? variantFor<BITS, 64, 16>(fp16, group) : variantFor<BITS, 64, 8>(fp16, group);
@@ -1358,8 +1361,8 @@ TilesPlan planTiles(const AttentionInfo &I, const DeviceProps &props) {
     const unsigned long long units = subs * I.num_seqs; // below 2^64: the line is longer
     // A unit to each CTA saves the combine kernel, but lets the longest unit set the time; it is for units that are known to be short
     // and few enough to run at once.  Measured at 32/8 heads of 128 (us, a unit to each CTA | the line): 4 sequences of 256 tokens
-    // 7.6 | 11.5 at 4 bits, 8.0 | 11.5 at 8; of 1024 13.1 | 12.0, 15.4 | 12.5; 16 of 1024 13.4 | 16.4, 15.6 | 17.6; 64 of 1024
-    // at 8 bits 29 | 35; 256 of 256 (more units than fit) 48 | 35, 43 | 38.
+    // 7.6 | 13.4 at 4 bits, 8.8 | 14.1 at 8; of 1024 13.1 | 13.6, 18.1 | 14.6; 16 of 1024 14.9 | 18.1, 20.4 | 20.2; 64 of 1024
+    // at 8 bits 31 | 39; 256 of 256 (more units than fit) 41.5 | 35.3, 48 | 46.
     const size_t longest = P.block_size * I.max_blocks;
     plan.unit_of_cta = units <= at_most && longest <= (units >= 64 ? 1024u : 512u);
     if (plan.unit_of_cta) {
