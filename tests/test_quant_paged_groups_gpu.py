@@ -177,3 +177,47 @@ def test_fp16_outputs_are_as_exact_as_32_bit_arithmetic(ib, bits, heads, kvh, hd
     got = ib.quant_paged_attention(q, *pools, tables, torch.tensor(lens).cuda(), None, hd ** -0.5)
     err, rounding = ((x.double() - want).norm() / want.norm() for x in (got, want.to(FP16)))
     assert float(err) <= 1.2 * float(rounding), (float(err), float(rounding))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (16, 2, 64), (16, 1, 128), (8, 1, 256)])
+@pytest.mark.parametrize("size", [1e4, 1e7, 1e12])
+def test_fp16_outputs_over_scores_of_any_size(ib, bits, heads, kvh, hd, size):  # noqa: F811
+    """Scores of up to `size`: the output is the row of the token that leads (by more than fp32 loses of the scores, 2^-17 of sum |q k|, and 40), its
+    weight off by 2^-11 at most where scores pass 2^20 (one rounding), and the output's own rounding of 2^-11."""
+    lens = [300, 37, 1]
+    g, pools, tables, q = case(hd, bits, hd, heads, kvh, lens, FP16, 1.0)
+    pools[2].mul_(1e3)
+    for sign in (1.0, -1.0):
+        scale = sign * size / 1e3 / hd ** 0.5
+        got = ib.quant_paged_attention(q, *pools, tables, torch.tensor(lens).cuda(), None, scale)
+        for i, n in enumerate(lens):
+            t = torch.arange(n, device="cuda")
+            block, off = tables[i][t // 16], t % 16
+            k, v = (qh.values(pools[x][block, :, off], pools[x + 2][block, :, off], bits) for x in (0, 1))
+            qq = q[i].double().view(kvh, heads // kvh, hd)
+            s = torch.einsum("hgd,nhd->hgn", qq, k) * scale
+            best = s.max(-1)
+            second = s.scatter(-1, best.indices[..., None], -float("inf")).amax(-1)
+            lost = torch.einsum("hgd,nhd->hgn", qq.abs(), k.abs()).amax(-1) * abs(scale) * 2.0 ** -17
+            clear = best.values - second > lost + 40
+            assert int(clear.sum()) >= 4
+            want = torch.stack([v[best.indices[h], h] for h in range(kvh)])
+            err = (got[i].double().view(kvh, heads // kvh, hd) - want).abs()
+            assert bool((err <= want.abs() * (2.0 ** -10 + 2.0 ** -20) + n * math.exp(-40) * v.abs().max() + 2.0 ** -25)[clear].all()), (sign, i)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("heads,kvh", [(16, 2), (16, 1), (6, 2)])
+def test_a_head_that_is_no_number_leaves_the_others_of_its_pass(ib, bits, heads, kvh):  # noqa: F811
+    """NaN and infinite q in groups of 3, 8 and 16, fp16: the columns of an instruction that other heads share with them stay right."""
+    lens = [200, 1, 33]
+    g, pools, tables, q = case(heads, bits, 128, heads, kvh, lens, FP16, 1.0)
+    want, bound = group_bound(q, pools, tables, torch.tensor(lens), 0.09, bits, FP16)
+    bad = q.clone()
+    bad[0, 1, 5], bad[1, 2, 0], bad[2, heads - 1, 127] = float("nan"), float("inf"), float("nan")
+    got = ib.quant_paged_attention(bad, *pools, tables, torch.tensor(lens).cuda(), None, 0.09)
+    for i, h in ((0, 1), (1, 2), (2, heads - 1)):
+        assert bool(got[i, h].isnan().all()), (i, h)
+        got[i, h], want[i, h], bound[i, h] = 0, 0, 0
+    qh.close(got, want, bound, "beside it")
